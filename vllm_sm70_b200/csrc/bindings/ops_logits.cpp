@@ -1,0 +1,220 @@
+// torch.ops._b200_C: operators over rows of logits (log-probabilities of
+// given tokens, distillation from a teacher's top values).
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/library.h>
+#include <torch/torch.h>
+
+#include <cmath>
+#include <tuple>
+
+#include "logits/logits_api.h"
+
+namespace b200 {
+namespace {
+
+using OptTensor = c10::optional<at::Tensor>;
+
+cudaStream_t stream_now() { return at::cuda::getCurrentCUDAStream().stream(); }
+
+LogitRows check_logits(const at::Tensor& x, const char* what) {
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2, what, ": logits must be a 2-D CUDA tensor [rows, V]");
+  const bool bf = x.scalar_type() == at::kBFloat16;
+  TORCH_CHECK(bf || x.scalar_type() == at::kFloat, what, ": logits must be bf16 or fp32");
+  TORCH_CHECK(x.size(1) >= 1 && x.size(1) <= kMaxVocab, what, ": vocabulary outside [1, 2^22]");
+  TORCH_CHECK(x.size(1) == 1 || x.stride(1) == 1, what, ": logits need a unit inner stride");
+  return LogitRows{x.data_ptr(), bf, x.size(0), x.stride(0), (int)x.size(1)};
+}
+
+void check_temperature(double t, const char* what) {
+  TORCH_CHECK(std::isfinite(t) && t >= 1e-3 && t <= 1e3, what,
+              ": temperature must be in [1e-3, 1e3], got ", t);
+}
+
+void check_like(const at::Tensor& t, const at::Tensor& x, at::ScalarType type, const char* what,
+                const char* name) {
+  TORCH_CHECK(t.device() == x.device(), what, ": ", name, " must be on the logits' device");
+  TORCH_CHECK(t.scalar_type() == type, what, ": ", name, " must be ", type);
+  TORCH_CHECK(t.is_contiguous(), what, ": ", name, " must be contiguous");
+}
+
+void check_ids(const at::Tensor& ids, const at::Tensor& x, const char* what) {
+  TORCH_CHECK(ids.device() == x.device(), what, ": token_ids must be on the logits' device");
+  TORCH_CHECK(ids.scalar_type() == at::kInt || ids.scalar_type() == at::kLong, what,
+              ": token_ids must be int32 or int64");
+  TORCH_CHECK(ids.dim() == 1 && ids.size(0) == x.size(0) && ids.is_contiguous(), what,
+              ": token_ids must be contiguous [rows]");
+}
+
+using Six = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor,
+                       at::Tensor>;
+
+Six token_logprobs(const at::Tensor& logits, const at::Tensor& ids, int64_t top_n,
+                   double temperature) {
+  const char* what = "token_logprobs";
+  TokenLogprobsArgs a{};
+  a.in = check_logits(logits, what);
+  check_ids(ids, logits, what);
+  check_temperature(temperature, what);
+  TORCH_CHECK(top_n >= 0 && top_n <= kMaxTopN && top_n <= a.in.V, what,
+              ": top_n must be in [0, min(64, V)], got ", top_n);
+  c10::cuda::CUDAGuard g(logits.device());
+  const auto f = logits.options().dtype(at::kFloat), i = logits.options().dtype(at::kInt);
+  const int64_t T = a.in.rows;
+  auto lp = at::empty({T}, f), ent = at::empty({T}, f), lse = at::empty({T}, f);
+  auto rank = at::empty({T}, i), stats = at::empty({T, 4}, f);
+  auto top_ids = at::empty({T, top_n}, i), top_lp = at::empty({T, top_n}, f);
+  a.ids = ids.data_ptr();
+  a.ids64 = ids.scalar_type() == at::kLong;
+  a.top_n = (int)top_n;
+  a.temperature = (float)temperature;
+  a.logprob = lp.data_ptr<float>();
+  a.rank = rank.data_ptr<int>();
+  a.entropy = ent.data_ptr<float>();
+  a.lse = lse.data_ptr<float>();
+  a.top_ids = top_ids.data_ptr<int>();
+  a.top_lp = top_lp.data_ptr<float>();
+  a.stats = stats.data_ptr<float>();
+  token_logprobs_launch(a, stream_now());
+  return {lp, rank, ent, lse, top_ids, top_lp, stats};
+}
+
+at::Tensor token_logprobs_bwd(const at::Tensor& logits, const at::Tensor& ids,
+                              const at::Tensor& stats, const OptTensor& g_logprob,
+                              const OptTensor& g_entropy, double temperature) {
+  const char* what = "token_logprobs_bwd";
+  TokenLogprobsBwdArgs a{};
+  a.in = check_logits(logits, what);
+  check_ids(ids, logits, what);
+  check_temperature(temperature, what);
+  check_like(stats, logits, at::kFloat, what, "stats");
+  TORCH_CHECK(stats.numel() == 4 * a.in.rows, what, ": stats must be [rows, 4]");
+  for (const OptTensor* t : {&g_logprob, &g_entropy})
+    if (t->has_value()) {
+      check_like(**t, logits, at::kFloat, what, "upstream gradient");
+      TORCH_CHECK((*t)->numel() == a.in.rows, what, ": upstream gradients must be [rows]");
+    }
+  c10::cuda::CUDAGuard g(logits.device());
+  auto grad = at::empty({a.in.rows, a.in.V}, logits.options());
+  a.ids = ids.data_ptr();
+  a.ids64 = ids.scalar_type() == at::kLong;
+  a.temperature = (float)temperature;
+  a.stats = stats.data_ptr<float>();
+  a.g_logprob = g_logprob ? g_logprob->data_ptr<float>() : nullptr;
+  a.g_entropy = g_entropy ? g_entropy->data_ptr<float>() : nullptr;
+  a.grad = grad.data_ptr();
+  token_logprobs_bwd_launch(a, stream_now());
+  return grad;
+}
+
+void check_teacher(const at::Tensor& logits, const at::Tensor& t_ids, const at::Tensor& t_lp,
+                   const OptTensor& weights, const char* what) {
+  check_like(t_ids, logits, at::kInt, what, "teacher_ids");
+  check_like(t_lp, logits, at::kFloat, what, "teacher_logprobs");
+  TORCH_CHECK(t_ids.dim() == 2 && t_ids.size(0) == logits.size(0) && t_ids.sizes() == t_lp.sizes(),
+              what, ": teacher_ids and teacher_logprobs must be [rows, K]");
+  TORCH_CHECK(t_ids.size(1) >= 1 && t_ids.size(1) <= kMaxTeacherK, what,
+              ": K must be in [1, 128], got ", t_ids.size(1));
+  if (weights) {
+    check_like(*weights, logits, at::kFloat, what, "weights");
+    TORCH_CHECK(weights->dim() == 1 && weights->size(0) == logits.size(0), what,
+                ": weights must be [rows]");
+  }
+}
+
+// (row losses, numbers for distill_loss_bwd, gradient or empty, loss or empty)
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> distill_loss(
+    const at::Tensor& logits, const at::Tensor& t_ids, const at::Tensor& t_lp,
+    const OptTensor& weights, double temperature, bool tail, double scale, bool with_loss,
+    bool with_grad) {
+  const char* what = "distill_loss";
+  DistillArgs a{};
+  a.in = check_logits(logits, what);
+  check_teacher(logits, t_ids, t_lp, weights, what);
+  check_temperature(temperature, what);
+  c10::cuda::CUDAGuard g(logits.device());
+  const auto f = logits.options().dtype(at::kFloat);
+  auto rows = at::empty({a.in.rows}, f), stats = at::empty({a.in.rows, 4}, f);
+  auto grad = at::empty({with_grad ? a.in.rows : 0, a.in.V}, logits.options());
+  auto loss = at::empty({}, f);
+  a.t_ids = t_ids.data_ptr<int>();
+  a.t_lp = t_lp.data_ptr<float>();
+  a.K = (int)t_ids.size(1);
+  a.weights = weights ? weights->data_ptr<float>() : nullptr;
+  a.temperature = (float)temperature;
+  a.tail = tail;
+  a.grad_scale = (float)scale;
+  a.row_loss = rows.data_ptr<float>();
+  a.stats = stats.data_ptr<float>();
+  a.grad = with_grad ? grad.data_ptr() : nullptr;
+  a.loss = with_loss ? loss.data_ptr<float>() : nullptr;
+  distill_launch(a, stream_now());
+  return {rows, stats, grad, loss};
+}
+
+at::Tensor distill_loss_bwd(const at::Tensor& logits, const at::Tensor& t_ids,
+                            const at::Tensor& t_lp, const OptTensor& weights, double temperature,
+                            bool tail, const at::Tensor& stats, const at::Tensor& g_rows,
+                            double scale) {
+  const char* what = "distill_loss_bwd";
+  DistillBwdArgs a{};
+  a.in = check_logits(logits, what);
+  check_teacher(logits, t_ids, t_lp, weights, what);
+  check_temperature(temperature, what);
+  check_like(stats, logits, at::kFloat, what, "stats");
+  check_like(g_rows, logits, at::kFloat, what, "upstream gradient");
+  TORCH_CHECK(stats.numel() == 4 * a.in.rows, what, ": stats must be [rows, 4]");
+  TORCH_CHECK(g_rows.dim() == 0 || g_rows.numel() == a.in.rows, what,
+              ": the upstream gradient must be a scalar or [rows]");
+  c10::cuda::CUDAGuard g(logits.device());
+  auto grad = at::empty({a.in.rows, a.in.V}, logits.options());
+  a.t_ids = t_ids.data_ptr<int>();
+  a.t_lp = t_lp.data_ptr<float>();
+  a.K = (int)t_ids.size(1);
+  a.weights = weights ? weights->data_ptr<float>() : nullptr;
+  a.temperature = (float)temperature;
+  a.tail = tail;
+  a.stats = stats.data_ptr<float>();
+  a.g_rows = g_rows.data_ptr<float>();
+  a.g_stride = g_rows.dim() == 0 ? 0 : 1;
+  a.g_scale = (float)scale;
+  a.grad = grad.data_ptr();
+  distill_bwd_launch(a, stream_now());
+  return grad;
+}
+
+void scale_by(at::Tensor& x, const at::Tensor& scale) {
+  const bool bf = x.scalar_type() == at::kBFloat16;
+  TORCH_CHECK(x.is_cuda() && x.is_contiguous() && (bf || x.scalar_type() == at::kFloat),
+              "scale_by: contiguous bf16 or fp32 CUDA tensor");
+  TORCH_CHECK((reinterpret_cast<uintptr_t>(x.data_ptr()) & 15) == 0, "scale_by: 16-byte aligned");
+  TORCH_CHECK(scale.device() == x.device() && scale.scalar_type() == at::kFloat &&
+              scale.numel() == 1, "scale_by: one fp32 value on the tensor's device");
+  c10::cuda::CUDAGuard g(x.device());
+  scale_by_launch(x.data_ptr(), bf, x.numel(), scale.data_ptr<float>(), stream_now());
+}
+
+}  // namespace
+}  // namespace b200
+
+TORCH_LIBRARY_FRAGMENT(_b200_C, m) {
+  m.def("token_logprobs(Tensor logits, Tensor token_ids, int top_n, float temperature) -> "
+        "(Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def("token_logprobs_bwd(Tensor logits, Tensor token_ids, Tensor stats, Tensor? g_logprob, "
+        "Tensor? g_entropy, float temperature) -> Tensor");
+  m.def("distill_loss(Tensor logits, Tensor teacher_ids, Tensor teacher_logprobs, "
+        "Tensor? weights, float temperature, bool tail, float scale, bool with_loss, "
+        "bool with_grad) -> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("distill_loss_bwd(Tensor logits, Tensor teacher_ids, Tensor teacher_logprobs, "
+        "Tensor? weights, float temperature, bool tail, Tensor stats, Tensor g_rows, "
+        "float scale) -> Tensor");
+  m.def("scale_by(Tensor(a!) x, Tensor scale) -> ()");
+}
+
+TORCH_LIBRARY_IMPL(_b200_C, CUDA, m) {
+  m.impl("token_logprobs", &b200::token_logprobs);
+  m.impl("token_logprobs_bwd", &b200::token_logprobs_bwd);
+  m.impl("distill_loss", &b200::distill_loss);
+  m.impl("distill_loss_bwd", &b200::distill_loss_bwd);
+  m.impl("scale_by", &b200::scale_by);
+}

@@ -58,7 +58,33 @@ def register_all() -> None:
     def _gemm(a, w, cfg=-1):
         return a.new_empty(a.shape[0], w.shape[0])
 
-    explicit = {"gemm_bf16"}
+    @torch.library.register_fake(f"{LIB}::token_logprobs")
+    def _token_logprobs(logits, ids, top_n, temperature):
+        T = logits.shape[0]
+
+        def f(*shape, dt=torch.float32):
+            return logits.new_empty(shape, dtype=dt)
+
+        return (f(T), f(T, dt=torch.int32), f(T), f(T), f(T, top_n, dt=torch.int32), f(T, top_n),
+                f(T, 4))
+
+    @torch.library.register_fake(f"{LIB}::token_logprobs_bwd")
+    def _token_logprobs_bwd(logits, *a):
+        return logits.new_empty(logits.shape)
+
+    @torch.library.register_fake(f"{LIB}::distill_loss")
+    def _distill_loss(logits, ids, lp, weights, temperature, tail, scale, with_loss, with_grad):
+        T, V = logits.shape
+        f = torch.float32
+        return (logits.new_empty(T, dtype=f), logits.new_empty((T, 4), dtype=f),
+                logits.new_empty((T if with_grad else 0, V)), logits.new_empty((), dtype=f))
+
+    @torch.library.register_fake(f"{LIB}::distill_loss_bwd")
+    def _distill_loss_bwd(logits, *a):
+        return logits.new_empty(logits.shape)
+
+    explicit = {"gemm_bf16", "token_logprobs", "token_logprobs_bwd", "distill_loss",
+                "distill_loss_bwd"}
     for s in _schemas():
         name = s.name.split("::", 1)[1]
         if name in explicit or name in NO_FAKE:
