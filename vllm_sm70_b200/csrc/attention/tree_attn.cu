@@ -22,16 +22,19 @@
 // kernel joins in share order; whole units are written directly. The split
 // depends on the lengths only, so results repeat bit for bit.
 //
-// Seven warps a CTA:
+// Eleven warps a CTA:
 //   warp 0     K / V producer: one (cache block, 64-column) box a lane, one
 //              warp-wide bulk-tensor instruction a tile, into one ring in the
 //              order of use K0 K1 V0 K2 V1 ...
 //   warp 1     TMEM owner and MMA issuer: S = Q K^T into one of two S buffers,
 //              then O += P V of the tile before it
-//   warps 2-5  softmax, a row a thread: exponentials in base 2 with a lazily
-//              raised reference (O is rescaled when a row's max grows by more
-//              than 2^8 over it), P as bf16 to TMEM; the unit's epilogue
-//   warp 6     Q loader: the next unit's rows while the present one runs
+//   warps 2-9  softmax: two threads a row, one for each half of the tile's
+//              keys (warps w and w + 4 of the same 32 TMEM lanes), which
+//              exchange their maxima through shared memory. Exponentials in
+//              base 2 with a lazily raised reference (O is rescaled when a
+//              row's max grows by more than 2^8 over it), P as bf16 to TMEM;
+//              the unit's epilogue, half of O's columns each
+//   warp 10    Q loader: the next unit's rows while the present one runs
 // The pipeline runs across units: the next unit's first S is issued before
 // the last P V of the present one.
 //
@@ -56,8 +59,10 @@ namespace b200 {
 namespace {
 
 constexpr int FM = 128;
-constexpr int kThreads = 224;
+constexpr int kThreads = 352;
+constexpr int kSoftmaxWarps = 8;
 constexpr int kBarBytes = 512;
+constexpr int kMaxBytes = 2 * 2 * FM * 4;  // [tile parity][half][row] floats
 constexpr int kMinShare = 2;  // key tiles of a CTA, at least
 
 template <int D_>
@@ -71,7 +76,7 @@ struct Cfg {
   static constexpr int kTile = kDC * kChunk;      // K or V of a tile
   static constexpr int NQ = D <= 128 ? 2 : 1;     // Q buffers
   static constexpr int NS = D == 64 ? 10 : 5;     // ring slots
-  static constexpr int kSmem = NQ * kQBytes + NS * kTile + kBarBytes + 1024;
+  static constexpr int kSmem = NQ * kQBytes + NS * kTile + kBarBytes + kMaxBytes;
   static_assert(2 * FN + D + FN <= 512, "TMEM columns");
   static_assert(kSmem <= 232448, "shared memory");
 };
@@ -188,9 +193,9 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
                  const Params p) {
   using C = Cfg<D_>;
   constexpr int D = C::D, FN = C::FN, kDC = C::kDC, NS = C::NS, NQ = C::NQ;
-  extern __shared__ uint8_t smem_raw[];
-  const uint32_t raw_addr = smem_u32(smem_raw);
-  uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
+  // The 128-byte swizzle wants 1024-byte aligned tiles: all shared memory is
+  // dynamic, and there is no room for a margin.
+  extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* sQ = smem;
   uint8_t* sKV = sQ + NQ * C::kQBytes;
   uint64_t* full = reinterpret_cast<uint64_t*>(sKV + NS * C::kTile);  // [NS]
@@ -203,10 +208,12 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
   uint64_t* p_free = p_full + 2;
   uint64_t* o_full = p_free + 2;
   uint64_t* o_free = o_full + 1;
-  uint64_t* done = o_free + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
-  __shared__ int sh_seq;
-  __shared__ long long sh_off, sh_n;
+  uint64_t* pair = o_free + 1;                                        // [4]
+  uint64_t* done = pair + 4;
+  long long* share_of = reinterpret_cast<long long*>(done + 1);  // sequence, offset, tiles
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(share_of + 3);
+  static_assert((2 * NS + 2 * NQ + 8 + 2 + 4 + 1 + 3) * 8 + 4 <= kBarBytes, "barriers");
+  float(*sh_max)[2][FM] = reinterpret_cast<float(*)[2][FM]>(sKV + NS * C::kTile + kBarBytes);
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   pdl_wait();
@@ -221,12 +228,13 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&s_free[i], 4);
-      mbar_init(&p_full[i], 4);
+      mbar_init(&s_free[i], kSoftmaxWarps);
+      mbar_init(&p_full[i], kSoftmaxWarps);
       mbar_init(&p_free[i], 1);
     }
     mbar_init(o_full, 1);
-    mbar_init(o_free, 4);
+    mbar_init(o_free, kSoftmaxWarps);
+    for (int i = 0; i < 4; ++i) mbar_init(&pair[i], 2);
     mbar_init(done, 1);
     fence_barrier_init();
     tma_prefetch_desc(&tmk);
@@ -236,7 +244,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
-  if (warp == 6) {
+  if (warp == 10) {
     // The share: a scan over the sequences, 32 at a time, for the total and
     // then for the sequence in which this CTA's first tile lies.
     long long total = 0;
@@ -281,9 +289,9 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
       seen += __shfl_sync(0xffffffffu, c, 31);
     }
     if (lane == 0) {
-      sh_seq = seq;
-      sh_off = off;
-      sh_n = n > 0 ? n : 0;
+      share_of[0] = seq;
+      share_of[1] = off;
+      share_of[2] = n > 0 ? n : 0;
     }
   }
   tc_fence_before();
@@ -292,8 +300,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
   if (threadIdx.x == 0) pdl_trigger();
   const uint32_t tmem_base = *tmem_slot;
   const uint32_t tS = tmem_base, tO = tmem_base + 2 * FN, tP = tO + D;
-  const int N = (int)sh_n;  // key tiles of this CTA
-  Walk<FN> walk(p, sh_seq, sh_off, sh_n);
+  const int N = (int)share_of[2];  // key tiles of this CTA
+  Walk<FN> walk(p, (int)share_of[0], share_of[1], share_of[2]);
   // Ring position of V_n; K_n sits at 2n - 1 (K_0 at 0).
   auto pos_v = [&](int n) { return n == N - 1 ? 2 * N - 1 : 2 * n + 2; };
 
@@ -416,7 +424,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
       mbar_wait(done, 0, p.err);
     }
     __syncwarp();
-  } else if (warp == 6) {
+  } else if (warp == 10) {
     // -------------------------------------------------------------- Q loader
     int units = 0;
     while (walk.next(p)) {
@@ -446,14 +454,26 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
     }
   } else {
     // --------------------------------------------------------------- softmax
-    const int q4 = warp & 3;  // TMEM lanes a warp may touch: 32 (warp % 4) ...
+    const int q4 = warp & 3;         // the 32 TMEM lanes this warp may touch
+    const int half = (warp - 2) / 4; // which half of the tile's keys
     const int row = q4 * 32 + lane;
-    const int stid = (int)threadIdx.x - 64;
+    const int stid = (int)threadIdx.x - 64;  // 0 .. 255
+    constexpr int HN = FN / 2;               // keys of a half
+    constexpr int HD = D / 2;                // O columns of a half
     const uint32_t lane_base = (uint32_t)(q4 * 32) << 16;
     const float sc = p.scale_log2;
     const uint64_t sc2 = f32x2_pack(sc, sc);
     bool ok = true;
-    int n = 0, units = 0;
+    int n = 0, units = 0, meets = 0;
+    // Both warps of these 32 rows meet (a wait with a limit, like the others:
+    // either may have given up).
+    auto meet = [&]() -> bool {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&pair[q4]);
+      const bool r = mbar_wait(&pair[q4], (uint32_t)(meets & 1), p.err);
+      ++meets;
+      return __all_sync(0xffffffffu, r);
+    };
     while (ok && walk.next(p)) {
       const int row0 = walk.row0(), kvh = walk.kvh();
       const int n_rows = walk.q.q_len * p.G - row0;
@@ -472,94 +492,48 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
           depth += __popc(mask_word(mrow, p.mask_words, nodes, i));
         key_lo = prefix + max(depth - 1, 0) - p.window + 1;
       }
-      float m_used = -INFINITY, l = 0.f;  // exponent reference (log2 units), row sum
+      // Exponent reference (log2 units; the same in both halves), this half's sum.
+      float m_used = -INFINITY, l = 0.f;
       for (int j = walk.j0; j < walk.j1; ++j, ++n) {
         const int sb = n & 1;
         ok = __all_sync(0xffffffffu, mbar_wait(&s_full[sb], (uint32_t)((n >> 1) & 1), p.err));
         if (!ok) break;
         tc_fence_after();
         const int kbase = walk.q.k_lo + j * FN;
+        const int kb = kbase + half * HN;
         if (warp_on) {
-          const bool masked =
-              __any_sync(0xffffffffu, key_lo > kbase) || kbase + FN > prefix;  // uniform
-          uint32_t vis[FN / 32];
+          // The half row of scores, masked, and its maximum.
+          uint32_t r[HN / 32][32];
 #pragma unroll
-          for (int w = 0; w < FN / 32; ++w) {
-            vis[w] = 0xffffffffu;
-            if (masked) {
-              const int k0 = kbase + 32 * w;
-              vis[w] = valid ? range_bits(key_lo - k0, prefix - k0) |
-                                   mask_bits(mrow, p.mask_words, nodes, k0 - prefix)
-                             : 0u;
+          for (int w = 0; w < HN / 32; ++w)
+            tmem_ld_32x32b_x32(tS + lane_base + sb * FN + half * HN + w * 32, r[w]);
+          tmem_wait_ld();
+          if (__any_sync(0xffffffffu, key_lo > kb) || kb + HN > prefix) {
+#pragma unroll
+            for (int w = 0; w < HN / 32; ++w) {
+              const int k0 = kb + 32 * w;
+              const uint32_t vis = valid ? range_bits(key_lo - k0, prefix - k0) |
+                                               mask_bits(mrow, p.mask_words, nodes, k0 - prefix)
+                                         : 0u;
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (!((vis >> i) & 1u)) r[w][i] = 0xff800000u;
             }
           }
-          const uint32_t s_row = tS + lane_base + sb * FN;
-          const uint32_t p_row = tP + lane_base + sb * (FN / 2);
-          // One sweep over the row's scores, 64 a TMEM wait; with WRITE: P =
-          // exp2(S scale - mu) as bf16 pairs, row sum into *rs. Returns the
-          // row max in log2 units.
-          auto sweep = [&](auto masked_c, auto write_c, float mu, float* rs) -> float {
-            constexpr bool kMasked = decltype(masked_c)::value;
-            constexpr bool kWrite = decltype(write_c)::value;
-            float mxa = -INFINITY, mxb = -INFINITY;
-            uint64_t acc = f32x2_pack(0.f, 0.f);
-            const float mu_eff = mu == -INFINITY ? 0.f : mu;
-            const uint64_t nmu2 = f32x2_pack(-mu_eff, -mu_eff);
-#pragma unroll 1
-            for (int hf = 0; hf < FN / 64; ++hf) {
-              uint32_t r[2][32];
-              tmem_ld_32x32b_x32(s_row + hf * 64, r[0]);
-              tmem_ld_32x32b_x32(s_row + hf * 64 + 32, r[1]);
-              const uint32_t v0 = hf == 0 ? vis[0] : vis[FN / 32 - 2];
-              const uint32_t v1 = hf == 0 ? vis[1] : vis[FN / 32 - 1];
-              tmem_wait_ld();
-              uint32_t w[32];
+          float mxs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                float va = __uint_as_float(r[i >> 4][(2 * i) & 31]);
-                float vb = __uint_as_float(r[i >> 4][(2 * i + 1) & 31]);
-                if constexpr (kMasked) {
-                  const uint32_t vw = i < 16 ? v0 : v1;
-                  if (!((vw >> ((2 * i) & 31)) & 1u)) va = -INFINITY;
-                  if (!((vw >> ((2 * i + 1) & 31)) & 1u)) vb = -INFINITY;
-                }
-                mxa = fmaxf(mxa, va);
-                mxb = fmaxf(mxb, vb);
-                if constexpr (kWrite) {
-                  float ea, eb;
-                  f32x2_unpack(f32x2_fma(f32x2_pack(va, vb), sc2, nmu2), ea, eb);
-                  ea = fast_exp2(ea);
-                  eb = fast_exp2(eb);
-                  acc = f32x2_add(acc, f32x2_pack(ea, eb));
-                  w[i] = pack_bf16x2(ea, eb);
-                }
-              }
-              if constexpr (kWrite) tmem_st_32x32b_x32(p_row + hf * 32, w);
-            }
-            if constexpr (kWrite) {
-              float a0, a1;
-              f32x2_unpack(acc, a0, a1);
-              *rs = a0 + a1;
-            }
-            const float mx = fmaxf(mxa, mxb);
-            return mx == -INFINITY ? mx : mx * sc;
-          };
-          using T_ = std::true_type;
-          using F_ = std::false_type;
-          if (__any_sync(0xffffffffu, m_used == -INFINITY)) {
-            const float mx =
-                masked ? sweep(T_{}, F_{}, 0.f, nullptr) : sweep(F_{}, F_{}, 0.f, nullptr);
-            if (m_used == -INFINITY) m_used = mx;
-          }
-          // This P buffer is free once P V of tile n - 2 has completed.
-          if (n >= 2) ok = mbar_wait(&p_free[sb], (uint32_t)(((n - 2) >> 1) & 1), p.err);
-          ok = __all_sync(0xffffffffu, ok);
+          for (int w = 0; w < HN / 32; ++w)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) mxs[i & 3] = fmaxf(mxs[i & 3], __uint_as_float(r[w][i]));
+          const float own = fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3]));
+          sh_max[sb][half][row] = own;
+          ok = meet();
           if (!ok) break;
-          float rs = 0.f;
-          float mx = masked ? sweep(T_{}, T_{}, m_used, &rs) : sweep(F_{}, T_{}, m_used, &rs);
-          const bool resc = mx > m_used + 8.f;
+          float mx = fmaxf(own, sh_max[sb][half ^ 1][row]);
+          mx = mx == -INFINITY ? mx : mx * sc;
+          const bool resc = mx > m_used + 8.f || (m_used == -INFINITY && mx != -INFINITY);
           if (__any_sync(0xffffffffu, resc)) {
-            const float alpha = resc ? exp2f(m_used - mx) : 1.f;
+            const float alpha = !resc ? 1.f : m_used == -INFINITY ? 0.f : exp2f(m_used - mx);
             if (resc) {
               l *= alpha;
               m_used = mx;
@@ -571,21 +545,45 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
               if (!ok) break;
               tc_fence_after();
 #pragma unroll 1
-              for (int c = 0; c < D / 32; ++c) {
+              for (int c = 0; c < HD / 32; ++c) {
                 uint32_t o[32];
-                tmem_ld_32x32b_x32(tO + lane_base + c * 32, o);
+                tmem_ld_32x32b_x32(tO + lane_base + half * HD + c * 32, o);
                 tmem_wait_ld();
 #pragma unroll
                 for (int e = 0; e < 32; ++e)
                   o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-                tmem_st_32x32b_x32(tO + lane_base + c * 32, o);
+                tmem_st_32x32b_x32(tO + lane_base + half * HD + c * 32, o);
               }
             }
-            tmem_wait_st();
-            // P once more, against the new reference.
-            masked ? sweep(T_{}, T_{}, m_used, &rs) : sweep(F_{}, T_{}, m_used, &rs);
           }
-          l += rs;
+          const float mu = m_used == -INFINITY ? 0.f : m_used;
+          const uint64_t nmu2 = f32x2_pack(-mu, -mu);
+          uint64_t acc[2] = {f32x2_pack(0.f, 0.f), f32x2_pack(0.f, 0.f)};
+          uint32_t w[HN / 2];
+#pragma unroll
+          for (int i = 0; i < HN / 2; ++i) {
+            float ea, eb;
+            f32x2_unpack(f32x2_fma(f32x2_pack(__uint_as_float(r[i >> 4][(2 * i) & 31]),
+                                              __uint_as_float(r[i >> 4][(2 * i + 1) & 31])),
+                                   sc2, nmu2),
+                         ea, eb);
+            ea = fast_exp2(ea);
+            eb = fast_exp2(eb);
+            acc[i & 1] = f32x2_add(acc[i & 1], f32x2_pack(ea, eb));
+            w[i] = pack_bf16x2(ea, eb);
+          }
+          float a0, a1;
+          f32x2_unpack(f32x2_add(acc[0], acc[1]), a0, a1);
+          l += a0 + a1;
+          // This P buffer is free once P V of tile n - 2 has completed.
+          if (n >= 2) ok = mbar_wait(&p_free[sb], (uint32_t)(((n - 2) >> 1) & 1), p.err);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          const uint32_t p_row = tP + lane_base + sb * (FN / 2) + half * (HN / 2);
+          if constexpr (HN == 64)
+            tmem_st_32x32b_x32(p_row, *reinterpret_cast<uint32_t(*)[32]>(w));
+          else
+            tmem_st_32x32b_x16(p_row, *reinterpret_cast<uint32_t(*)[16]>(w));
           tmem_wait_st();
         }
         tc_fence_before();
@@ -600,7 +598,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
           if (!ok) break;
           uint8_t* sv = sKV + (pos % NS) * C::kTile;
           constexpr int kU = D / 8;
-          for (int i = stid; i < FN * kU; i += 128) {
+          for (int i = stid; i < FN * kU; i += kSoftmaxWarps * 32) {
             const int k = i / kU, c16 = i % kU;
             if (kbase + k >= seq_len || kbase + k < walk.q.k_first)
               *reinterpret_cast<uint4*>(sv + (c16 >> 3) * C::kChunk + sw_off(k, c16 & 7)) =
@@ -613,6 +611,15 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
       }
       if (!ok) break;
       // ---------------------------------------------------- the unit's epilogue
+      if (warp_on) {
+        // (The buffer is the next unit's first tile's, hence the second meeting.)
+        sh_max[n & 1][half][row] = l;
+        ok = meet();
+        if (!ok) break;
+        l = sh_max[n & 1][0][row] + sh_max[n & 1][1][row];
+        ok = meet();
+        if (!ok) break;
+      }
       ok = __all_sync(0xffffffffu, mbar_wait(o_full, (uint32_t)(units & 1), p.err));
       if (!ok) break;
       ++units;
@@ -627,14 +634,15 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
                                       : l + exp2f(p.sinks[head] * 1.4426950408889634f - m_used);
           f = den > 0.f ? 1.f / den : 0.f;
         }
-        __nv_bfloat16* dst = p.out + (long long)(walk.q.q0 + node) * p.o_stride + (long long)head * D;
+        __nv_bfloat16* dst = p.out + (long long)(walk.q.q0 + node) * p.o_stride +
+                             (long long)head * D + half * HD;
         const long long piece = ((long long)blockIdx.x * 2 + (walk.j0 > 0 ? 0 : 1)) * FM + row;
-        float* part = p.part_o + piece * D;
-        if (!whole && valid) p.part_ml[piece] = make_float2(m_used, l);
+        float* part = p.part_o + piece * D + half * HD;
+        if (!whole && valid && half == 0) p.part_ml[piece] = make_float2(m_used, l);
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
+        for (int c = 0; c < HD / 32; ++c) {
           uint32_t o[32];
-          tmem_ld_32x32b_x32(tO + lane_base + c * 32, o);  // warp-collective
+          tmem_ld_32x32b_x32(tO + lane_base + half * HD + c * 32, o);  // warp-collective
           tmem_wait_ld();
           if (!valid) continue;
           if (whole) {
