@@ -141,7 +141,7 @@ def test_strides_workspace_stream(b200_ops):
     _, kc, vc, bt, sl, cu, m = _setup([700, 90], [9, 5], (32, 8, 128), 16)
     qkv = torch.randn(14, 48, 128, device="cuda").bfloat16()
     q = qkv[:, :32]
-    ws = ops.tree_attention_workspace(2, 128, "cuda")
+    ws = ops.tree_attention_workspace(128, "cuda")
     a = _check(q, kc, vc, bt, sl, cu, m, workspace=ws)
     buf = torch.zeros(14, 40, 128, device="cuda", dtype=torch.bfloat16)
     b = _check(q, kc, vc, bt, sl, cu, m, out=buf[:, 4:36], workspace=ws)
@@ -162,7 +162,7 @@ def test_strides_workspace_stream(b200_ops):
 
 def test_graph_replays_with_new_lengths(b200_ops):
     q, kc, vc, bt, sl, cu, m = _setup([900, 500], [6, 6], (32, 8, 128), 16)
-    ws = ops.tree_attention_workspace(2, 128, "cuda")
+    ws = ops.tree_attention_workspace(128, "cuda")
     out, lens = torch.empty_like(q), sl.clone()
     ops.tree_attention(out, q, kc, vc, bt, lens, cu, m, 0.09, workspace=ws)
     torch.cuda.synchronize()

@@ -42,6 +42,7 @@
 #include <type_traits>
 
 #include "attention/attn_api.h"
+#include "attention/exp2.cuh"
 #include "common/launch.h"
 #include "common/ptx.cuh"
 #include "common/tmap.h"
@@ -92,13 +93,6 @@ struct FaParams {
 // Optional per-CTA timeline (profiling aid, off unless a buffer is installed
 // with fa_tc_set_timeline): %globaltimer stamps, 8 slots per CTA.
 __device__ unsigned long long* g_fa_timeline = nullptr;
-
-// 2^x on the multi-function unit (P values lie in [0, 2^8]).
-__device__ __forceinline__ float fast_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 __device__ __forceinline__ uint32_t sw_off(int row, int chunk) {
   return (uint32_t)(row * 128 + ((chunk ^ (row & 7)) << 4));

@@ -22,21 +22,32 @@
 // kernel joins in share order; whole units are written directly. The split
 // depends on the lengths only, so results repeat bit for bit.
 //
-// Eleven warps a CTA:
-//   warp 0     K / V producer: one (cache block, 64-column) box a lane, one
-//              warp-wide bulk-tensor instruction a tile, into one ring in the
-//              order of use K0 K1 V0 K2 V1 ...
+// Twelve warps a CTA:
+//   warp 0     K producer, warp 10 V producer: one (cache block, 64-column)
+//              box a lane, one warp-wide bulk-tensor instruction a tile (that
+//              costs its warp ~80 cycles a box, hence two warps), into one
+//              ring in the order of use K0 K1 V0 K2 V1 ... Warp 0 also walks
+//              the share and publishes each unit's numbers, one unit ahead, so
+//              that nobody else waits for lengths or divides.
 //   warp 1     TMEM owner and MMA issuer: S = Q K^T into one of two S buffers,
-//              then O += P V of the tile before it
+//              then O += P V of the tile before it. Q and P are TMEM operands,
+//              so shared memory feeds the tensor core with K and V alone.
 //   warps 2-9  softmax: two threads a row, one for each half of the tile's
 //              keys (warps w and w + 4 of the same 32 TMEM lanes), which
 //              exchange their maxima through shared memory. Exponentials in
 //              base 2 with a lazily raised reference (O is rescaled when a
-//              row's max grows by more than 2^8 over it), P as bf16 to TMEM;
-//              the unit's epilogue, half of O's columns each
-//   warp 10    Q loader: the next unit's rows while the present one runs
-// The pipeline runs across units: the next unit's first S is issued before
-// the last P V of the present one.
+//              row's max grows by more than 2^8 over it), P as bf16 over the
+//              first half of its S buffer. In a unit's last tile they bring
+//              the next unit's Q rows to TMEM; a unit's epilogue (half of O's
+//              columns each) comes after the next unit's first tile, when the
+//              last P V has long finished.
+//   warp 11    zeroes V rows that no node sees (past the end, before the
+//              window): they may hold anything, and 0 x NaN is not 0.
+// TMEM columns: S0 | S1 | O | Q.
+//
+// Bound: HBM for up to 128 rows a key head (a 64 KB key tile takes ~2800 SM
+// cycles to arrive; the softmax, the longest chain, ~2400, of which 1024 are
+// the multi-function unit's), the softmax beyond.
 //
 // Rounding: P is rounded to bf16 for the tensor core (relative 2^-8 a term at
 // most, as the output's own rounding); scores, maxima, sums and O are fp32.
@@ -49,6 +60,7 @@
 #include <string>
 #include <type_traits>
 
+#include "attention/exp2.cuh"
 #include "attention/tree_attn.h"
 #include "common/launch.h"
 #include "common/ptx.cuh"
@@ -59,9 +71,10 @@ namespace b200 {
 namespace {
 
 constexpr int FM = 128;
-constexpr int kThreads = 352;
+constexpr int kThreads = 384;
 constexpr int kSoftmaxWarps = 8;
-constexpr int kBarBytes = 512;
+constexpr int kBarBytes = 768;  // barriers and published units
+constexpr int kUnits = 4;       // published units
 constexpr int kMaxBytes = 2 * 2 * FM * 4;  // [tile parity][half][row] floats
 constexpr int kMinShare = 2;  // key tiles of a CTA, at least
 
@@ -70,15 +83,17 @@ struct Cfg {
   static constexpr int D = D_;
   static constexpr int FN = D <= 128 ? 128 : 64;  // keys of a tile
   static constexpr int kDC = D / 64;              // 64-column chunks of a row
-  static constexpr int kQChunk = FM * 128;
-  static constexpr int kQBytes = kDC * kQChunk;
   static constexpr int kChunk = FN * 128;
   static constexpr int kTile = kDC * kChunk;      // K or V of a tile
-  static constexpr int NQ = D <= 128 ? 2 : 1;     // Q buffers
-  static constexpr int NS = D == 64 ? 10 : 5;     // ring slots
-  static constexpr int kSmem = NQ * kQBytes + NS * kTile + kBarBytes + kMaxBytes;
-  static_assert(2 * FN + D + FN <= 512, "TMEM columns");
+  static constexpr int NS = D == 64 ? 14 : 7;     // ring slots: 224 KB
+  static constexpr int kSmem = NS * kTile + kBarBytes + kMaxBytes;
+  static_assert(2 * FN + D + D / 2 <= 512, "TMEM columns");
   static_assert(kSmem <= 232448, "shared memory");
+};
+
+// The unit in which a CTA's share begins (tree_join_kernel).
+struct Cut {
+  int seq, unit, j0, pad;
 };
 
 struct Params {
@@ -91,7 +106,8 @@ struct Params {
   const float* sinks;
   float* part_o;        // [grid][2][FM][D]
   float2* part_ml;      // [grid][2][FM]
-  long long* seq_tile;  // [num_seqs + 1]: first tile of each sequence, then the share
+  Cut* cut;             // [grid]
+  long long* share;     // key tiles of a CTA
   int num_seqs, Hq, Hkv, G, block_size, block_shift, max_blocks, num_blocks;
   int mask_words, window;
   long long T, q_stride, o_stride;
@@ -99,24 +115,27 @@ struct Params {
   unsigned int* err;
 };
 
-__device__ __forceinline__ float fast_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ uint32_t sw_off(int row, int chunk) {
   return (uint32_t)(row * 128 + ((chunk ^ (row & 7)) << 4));
 }
-__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool valid) {
-  const int sz = valid ? 16 : 0;
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(sz)
-               : "memory");
+// (volatile: issued where they stand, ahead of the tile's work)
+__device__ __forceinline__ uint32_t ld_word(const uint32_t* p) {
+  uint32_t v;
+  asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint4 ld_q(const __nv_bfloat16* p) {
+  uint4 v;
+  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
 }
 
 // One sequence's part of the work.
 struct Seq {
   int q0, q_len, seq_len, nodes, prefix, k_first, k_lo, n_tiles, n_rt;
-  long long total;  // tiles of all its units
+  int total;  // tiles of all its units (the host bounds it)
 };
 template <int FN>
 __device__ __forceinline__ Seq load_seq(const Params& p, int s) {
@@ -131,7 +150,7 @@ __device__ __forceinline__ Seq load_seq(const Params& p, int s) {
   r.k_lo = r.k_first / FN * FN;
   r.n_tiles = max(1, (r.seq_len - r.k_lo + FN - 1) / FN);
   r.n_rt = (r.q_len * p.G + FM - 1) / FM;
-  r.total = (long long)r.n_tiles * r.n_rt * p.Hkv;
+  r.total = r.n_tiles * r.n_rt * p.Hkv;
   return r;
 }
 
@@ -139,10 +158,10 @@ __device__ __forceinline__ Seq load_seq(const Params& p, int s) {
 // key tiles [j0, j1) of it.
 template <int FN>
 struct Walk {
-  int s, unit, j0, j1;
-  long long off, left;
+  int s, unit, j0, j1, kvh, row0;
+  int off, left;
   Seq q;
-  __device__ __forceinline__ Walk(const Params& p, int s0, long long off0, long long n)
+  __device__ __forceinline__ Walk(const Params& p, int s0, int off0, int n)
       : s(s0), off(off0), left(n) {
     if (left > 0) q = load_seq<FN>(p, s);
   }
@@ -153,31 +172,50 @@ struct Walk {
       q = load_seq<FN>(p, s);
       off = 0;
     }
-    unit = (int)(off / q.n_tiles);
-    j0 = (int)(off - (long long)unit * q.n_tiles);
-    j1 = j0 + (int)min((long long)(q.n_tiles - j0), left);
-    off += j1 - j0;
-    left -= j1 - j0;
+    unit = off / q.n_tiles;
+    kvh = unit / q.n_rt;
+    row0 = (unit - kvh * q.n_rt) * FM;
+    j0 = off - unit * q.n_tiles;
+    const int n = min(q.n_tiles - j0, left);
+    j1 = j0 + n;
+    off += n;
+    left -= n;
     return true;
   }
-  __device__ __forceinline__ int kvh() const { return unit / q.n_rt; }
-  __device__ __forceinline__ int row0() const { return unit % q.n_rt * FM; }
+};
+
+// A unit as warp 0 publishes it. j0 == j1: no more units.
+struct __align__(16) Unit {
+  int seq, kvh, j0, j1;
+  int q0, row0, rows, whole;  // first token; first row; rows from it on; not cut
+  int nodes, prefix, seq_len, k_lo;
+  int k_first, pad[3];
+  template <int FN>
+  __device__ __forceinline__ bool dirty(int j) const {
+    // Has tile j rows of V that no node sees?
+    const int kbase = k_lo + j * FN;
+    return kbase + FN > seq_len || kbase < k_first;
+  }
 };
 
 // 32 bits of a node's mask row from node `o` on (o may be negative); bits of
 // nodes outside [0, nodes) are 0.
-__device__ __forceinline__ uint32_t mask_word(const uint32_t* row, int words, int nodes, int i) {
-  if (i < 0 || i >= words || 32 * i >= nodes) return 0u;
-  const int n = nodes - 32 * i;
-  const uint32_t w = __ldg(row + i);
-  return n >= 32 ? w : w & ((1u << n) - 1u);
-}
-__device__ __forceinline__ uint32_t mask_bits(const uint32_t* row, int words, int nodes, int o) {
-  if (o <= -32 || o >= nodes) return 0u;
-  const int i = o >> 5;
-  return __funnelshift_r(mask_word(row, words, nodes, i), mask_word(row, words, nodes, i + 1),
-                         o & 31);
-}
+struct MaskRow {
+  const uint32_t* row;
+  int words, nodes;
+  uint32_t w0, w1;  // the first two words (64 nodes), fetched ahead
+  __device__ __forceinline__ uint32_t word(int i) const {
+    if (i < 0 || i >= words || 32 * i >= nodes) return 0u;
+    const int n = nodes - 32 * i;
+    const uint32_t w = i == 0 ? w0 : i == 1 ? w1 : __ldg(row + i);
+    return n >= 32 ? w : w & ((1u << n) - 1u);
+  }
+  __device__ __forceinline__ uint32_t bits(int o) const {
+    if (o <= -32 || o >= nodes) return 0u;
+    const int i = o >> 5;
+    return __funnelshift_r(word(i), word(i + 1), o & 31);
+  }
+};
 // Bits [lo, hi) of a 32-bit word, clamped to it.
 __device__ __forceinline__ uint32_t range_bits(int lo, int hi) {
   lo = max(lo, 0);
@@ -192,27 +230,30 @@ __global__ void __launch_bounds__(kThreads, 1)
 tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
                  const Params p) {
   using C = Cfg<D_>;
-  constexpr int D = C::D, FN = C::FN, kDC = C::kDC, NS = C::NS, NQ = C::NQ;
+  constexpr int D = C::D, FN = C::FN, kDC = C::kDC, NS = C::NS;
   // The 128-byte swizzle wants 1024-byte aligned tiles: all shared memory is
   // dynamic, and there is no room for a margin.
   extern __shared__ __align__(1024) uint8_t smem[];
-  uint8_t* sQ = smem;
-  uint8_t* sKV = sQ + NQ * C::kQBytes;
+  uint8_t* sKV = smem;
   uint64_t* full = reinterpret_cast<uint64_t*>(sKV + NS * C::kTile);  // [NS]
   uint64_t* empty = full + NS;                                        // [NS]
-  uint64_t* q_full = empty + NS;                                      // [NQ]
-  uint64_t* q_empty = q_full + NQ;                                    // [NQ]
-  uint64_t* s_full = q_empty + NQ;                                    // [2]
-  uint64_t* s_free = s_full + 2;
-  uint64_t* p_full = s_free + 2;
-  uint64_t* p_free = p_full + 2;
-  uint64_t* o_full = p_free + 2;
+  uint64_t* s_full = empty + NS;                                      // [2]
+  uint64_t* p_full = s_full + 2;                                      // [2]
+  uint64_t* pair = p_full + 2;                                        // [4]
+  uint64_t* q_full = pair + 4;
+  uint64_t* pv_done = q_full + 1;
+  uint64_t* o_full = pv_done + 1;
   uint64_t* o_free = o_full + 1;
-  uint64_t* pair = o_free + 1;                                        // [4]
-  uint64_t* done = pair + 4;
-  long long* share_of = reinterpret_cast<long long*>(done + 1);  // sequence, offset, tiles
+  uint64_t* done = o_free + 1;
+  uint64_t* u_full = done + 1;                                        // [kUnits]
+  uint64_t* u_empty = u_full + kUnits;                                // [kUnits]
+  uint64_t* v_dirty = u_empty + kUnits;                               // [2]
+  uint64_t* v_clean = v_dirty + 2;                                    // [2]
+  int* share_of = reinterpret_cast<int*>(v_clean + 2);  // sequence, offset, tiles
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(share_of + 3);
-  static_assert((2 * NS + 2 * NQ + 8 + 2 + 4 + 1 + 3) * 8 + 4 <= kBarBytes, "barriers");
+  static_assert((2 * NS + 8 + 5 + 2 * kUnits + 4) * 8 + 16 + kUnits * (int)sizeof(Unit) <= kBarBytes,
+                "barriers and units");
+  Unit* units_sh = reinterpret_cast<Unit*>(sKV + NS * C::kTile + kBarBytes) - kUnits;
   float(*sh_max)[2][FM] = reinterpret_cast<float(*)[2][FM]>(sKV + NS * C::kTile + kBarBytes);
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -222,20 +263,22 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
-    for (int i = 0; i < NQ; ++i) {
-      mbar_init(&q_full[i], 1);
-      mbar_init(&q_empty[i], 1);
-    }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&s_free[i], kSoftmaxWarps);
       mbar_init(&p_full[i], kSoftmaxWarps);
-      mbar_init(&p_free[i], 1);
+      mbar_init(&v_dirty[i], 1);
+      mbar_init(&v_clean[i], 1);
     }
+    for (int i = 0; i < 4; ++i) mbar_init(&pair[i], 2);
+    mbar_init(q_full, kSoftmaxWarps);
+    mbar_init(pv_done, 1);
     mbar_init(o_full, 1);
     mbar_init(o_free, kSoftmaxWarps);
-    for (int i = 0; i < 4; ++i) mbar_init(&pair[i], 2);
     mbar_init(done, 1);
+    for (int i = 0; i < kUnits; ++i) {
+      mbar_init(&u_full[i], 1);
+      mbar_init(&u_empty[i], kSoftmaxWarps + 3);  // and the MMA, V and cleaning warps
+    }
     fence_barrier_init();
     tma_prefetch_desc(&tmk);
     tma_prefetch_desc(&tmv);
@@ -247,7 +290,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
   if (warp == 10) {
     // The share: a scan over the sequences, 32 at a time, for the total and
     // then for the sequence in which this CTA's first tile lies.
-    long long total = 0;
+    long long total = 0, first32 = 0;
     for (int b = 0; b < p.num_seqs; b += 32) {
       const int s = b + lane;
       long long n = s < p.num_seqs ? load_seq<FN>(p, s).total : 0;
@@ -256,34 +299,33 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
         const long long up = __shfl_up_sync(0xffffffffu, n, o);
         if (lane >= o) n += up;
       }
-      if (blockIdx.x == 0 && s < p.num_seqs) p.seq_tile[s + 1] = total + n;
+      if (b == 0) first32 = n;
       total += __shfl_sync(0xffffffffu, n, 31);
     }
     const long long share =
         max((long long)kMinShare, (total + gridDim.x - 1) / (long long)gridDim.x);
-    if (blockIdx.x == 0 && lane == 0) {
-      p.seq_tile[0] = 0;
-      p.seq_tile[p.num_seqs + 1] = share;
-    }
     const long long t0 = share * blockIdx.x;
     const long long n = min(share, total - t0);
-    int seq = 0;
-    long long off = 0, seen = 0;
+    int seq = 0, off = 0;
+    long long seen = 0;
     bool found = n <= 0;
     for (int b = 0; b < p.num_seqs && !found; b += 32) {
-      const int s = b + lane;
-      const long long own = s < p.num_seqs ? load_seq<FN>(p, s).total : 0;
-      long long c = own;
+      long long c = first32;  // sums up to and with this lane's sequence
+      if (b > 0) {
+        const int s = b + lane;
+        c = s < p.num_seqs ? load_seq<FN>(p, s).total : 0;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long up = __shfl_up_sync(0xffffffffu, c, o);
-        if (lane >= o) c += up;
+        for (int o = 1; o < 32; o <<= 1) {
+          const long long up = __shfl_up_sync(0xffffffffu, c, o);
+          if (lane >= o) c += up;
+        }
       }
+      const long long before = __shfl_up_sync(0xffffffffu, c, 1);
       const uint32_t hit = __ballot_sync(0xffffffffu, seen + c > t0);
       if (hit) {
         const int l = __ffs(hit) - 1;
         seq = b + l;
-        off = t0 - (seen + __shfl_sync(0xffffffffu, c - own, l));
+        off = (int)(t0 - seen - __shfl_sync(0xffffffffu, lane > 0 ? before : 0, l));
         found = true;
       }
       seen += __shfl_sync(0xffffffffu, c, 31);
@@ -291,7 +333,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
     if (lane == 0) {
       share_of[0] = seq;
       share_of[1] = off;
-      share_of[2] = n > 0 ? n : 0;
+      share_of[2] = (int)max(0ll, n);
+      if (blockIdx.x == 0) *p.share = share;
     }
   }
   tc_fence_before();
@@ -299,71 +342,110 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
   tc_fence_after();
   if (threadIdx.x == 0) pdl_trigger();
   const uint32_t tmem_base = *tmem_slot;
-  const uint32_t tS = tmem_base, tO = tmem_base + 2 * FN, tP = tO + D;
-  const int N = (int)share_of[2];  // key tiles of this CTA
-  Walk<FN> walk(p, (int)share_of[0], share_of[1], share_of[2]);
-  // Ring position of V_n; K_n sits at 2n - 1 (K_0 at 0).
+  const uint32_t tS = tmem_base, tO = tS + 2 * FN, tQ = tO + D;
+  const int N = share_of[2];  // key tiles of this CTA
+  // Ring positions.
+  auto pos_k = [&](int n) { return n == 0 ? 0 : 2 * n - 1; };
   auto pos_v = [&](int n) { return n == N - 1 ? 2 * N - 1 : 2 * n + 2; };
 
-  if (warp == 0) {
-    // -------------------------------------------------------------- producer
+  // Unit u for a reader (a warp, or one thread with `alone`).
+  auto take = [&](int u, Unit& x, bool alone) -> bool {
+    const int e = u % kUnits;
+    const bool ok = mbar_wait(&u_full[e], (uint32_t)((u / kUnits) & 1), p.err);
+    x = units_sh[e];
+    if (!alone) __syncwarp();
+    if (alone || lane == 0) mbar_arrive(&u_empty[e]);
+    return alone ? ok : __all_sync(0xffffffffu, ok);
+  };
+
+  if (warp == 0 || warp == 10) {
+    // ------------------------------------------------ producers (K: 0, V: 10)
+    const bool is_v = warp == 10;
+    const CUtensorMap* tm = is_v ? &tmv : &tmk;
     const int BS = p.block_size;
     const int nb = BS >= FN ? 1 : FN / BS;
     const int rows_box = BS >= FN ? FN : BS;
     const int bi = lane % nb, h = lane / nb;
+    Walk<FN> walk(p, share_of[0], share_of[1], is_v ? 0 : N);
+    int published = 0;
+    auto publish = [&](Unit& x) -> bool {  // the next unit, to the others and to x
+      const int e = published % kUnits;
+      int ok = 1;
+      if (lane == 0)
+        ok = mbar_wait(&u_empty[e], (uint32_t)(((published / kUnits) & 1) ^ 1), p.err) ? 1 : 0;
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      const bool more = walk.next(p);
+      x.seq = walk.s;
+      x.kvh = walk.kvh;
+      x.j0 = more ? walk.j0 : 0;
+      x.j1 = more ? walk.j1 : 0;
+      x.q0 = walk.q.q0;
+      x.row0 = walk.row0;
+      x.rows = walk.q.q_len * p.G - walk.row0;
+      x.whole = walk.j0 == 0 && walk.j1 == walk.q.n_tiles;
+      x.nodes = walk.q.nodes;
+      x.prefix = walk.q.prefix;
+      x.seq_len = walk.q.seq_len;
+      x.k_lo = walk.q.k_lo;
+      x.k_first = walk.q.k_first;
+      if (ok && lane == 0) {
+        units_sh[e] = x;
+        mbar_arrive(&u_full[e]);
+        if (published == 0) p.cut[blockIdx.x] = Cut{x.seq, more ? walk.unit : 0, x.j0, 0};
+      }
+      ++published;
+      return ok != 0;
+    };
+    int taken = 0;
+    auto fetch = [&](Unit& x) -> bool { return is_v ? take(taken++, x, false) : publish(x); };
     struct Box {
       int blk, y;
     };
-    // Tile j of the present unit: this lane's cache block and row.
-    auto box_of = [&](int j) {
-      const int kbase = walk.q.k_lo + j * FN;
-      const int last = min(max(0, (walk.q.seq_len - 1) >> p.block_shift), p.max_blocks - 1);
+    // Tile j of a unit: this lane's cache block and row.
+    auto box_of = [&](const Unit& x, int j) {
+      const int kbase = x.k_lo + j * FN;
+      const int last = min(max(0, (x.seq_len - 1) >> p.block_shift), p.max_blocks - 1);
       const int b = min((kbase >> p.block_shift) + bi, last);
-      const int id = __ldg(p.block_table + (long long)walk.s * p.max_blocks + b);
-      Box x;
-      x.blk = in_bounds(id >= 0 && id < p.num_blocks, p.err) ? id : 0;
-      x.y = walk.kvh() * BS + (BS > FN ? (kbase & (BS - 1)) : 0);
-      return x;
+      const int id = __ldg(p.block_table + (long long)x.seq * p.max_blocks + b);
+      Box r;
+      r.blk = in_bounds(id >= 0 && id < p.num_blocks, p.err) ? id : 0;
+      r.y = x.kvh * BS + (BS > FN ? (kbase & (BS - 1)) : 0);
+      return r;
     };
-    int pos = 0;
-    auto put = [&](const CUtensorMap* tm, const Box& x) -> bool {
-      const int st = pos % NS;
-      int ok = 1;
-      if (lane == 0) {
-        ok = mbar_wait(&empty[st], (uint32_t)(((pos / NS) & 1) ^ 1), p.err) ? 1 : 0;
-        if (ok) mbar_arrive_expect_tx(&full[st], (uint32_t)C::kTile);
+    Unit unit, next;
+    bool ok = fetch(unit);
+    Box cur{0, 0};
+    if (ok && unit.j0 < unit.j1) cur = box_of(unit, unit.j0);
+    int n = 0;
+    while (ok && unit.j0 < unit.j1) {
+      ok = fetch(next);
+      for (int j = unit.j0; j < unit.j1 && ok; ++j, ++n) {
+        // Ids one tile ahead of their use.
+        Box nxt = cur;
+        if (j + 1 < unit.j1) nxt = box_of(unit, j + 1);
+        else if (next.j0 < next.j1) nxt = box_of(next, next.j0);
+        const int pos = is_v ? pos_v(n) : pos_k(n), st = pos % NS;
+        int go = 1;
+        if (lane == 0) {
+          go = mbar_wait(&empty[st], (uint32_t)(((pos / NS) & 1) ^ 1), p.err) ? 1 : 0;
+          if (go) mbar_arrive_expect_tx(&full[st], (uint32_t)C::kTile);
+        }
+        ok = __shfl_sync(0xffffffffu, go, 0);
+        if (ok && h < kDC)
+          tma_load_3d(sKV + st * C::kTile + h * C::kChunk + bi * rows_box * 128, tm, &full[st],
+                      h * 64, cur.y, cur.blk);
+        cur = nxt;
       }
-      if (!__shfl_sync(0xffffffffu, ok, 0)) return false;
-      if (h < kDC)
-        tma_load_3d(sKV + st * C::kTile + h * C::kChunk + bi * rows_box * 128, tm, &full[st],
-                    h * 64, x.y, x.blk);
-      ++pos;
-      return true;
-    };
-    bool ok = true, more = walk.next(p);
-    int j = more ? walk.j0 : 0;
-    Box cur{0, 0}, before{0, 0};
-    if (more) cur = box_of(j);
-    for (int n = 0; n < N && ok; ++n) {
-      // Ids one tile ahead of their use.
-      Box nxt = cur;
-      if (more && ++j == walk.j1) {
-        more = walk.next(p);
-        j = more ? walk.j0 : 0;
-      }
-      if (more) nxt = box_of(j);
-      ok = put(&tmk, cur) && (n == 0 || put(&tmv, before));
-      before = cur;
-      cur = nxt;
+      unit = next;
     }
-    if (ok && N > 0) put(&tmv, before);
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
     if (lane == 0 && N > 0) {
       constexpr uint32_t idesc_s = umma_idesc_f16(FM, FN, true);
       constexpr uint32_t idesc_pv = umma_idesc_f16(FM, D, true) | (1u << 16);  // B MN-major
-      int units_s = 0, units_o = 0;  // units whose S / whose P V has begun
-      auto pv = [&](int n, bool first, bool last) -> bool {
+      int units = 0, units_o = 0;  // units whose S / whose P V has begun
+      int sent = 0, cleaned = 0;  // dirty V tiles given to the cleaner / taken back
+      auto pv = [&](int n, bool first, bool last, bool dirty) -> bool {
         const int pos = pos_v(n), st = pos % NS, pb = n & 1;
         if (first) {
           // O is free once the epilogue of the unit before has read it.
@@ -373,98 +455,110 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
         if (!mbar_wait(&p_full[pb], (uint32_t)((n >> 1) & 1), p.err) ||
             !mbar_wait(&full[st], (uint32_t)((pos / NS) & 1), p.err))
           return false;
+        if (dirty) {
+          if (!mbar_wait(&v_clean[cleaned & 1], (uint32_t)((cleaned >> 1) & 1), p.err))
+            return false;
+          ++cleaned;
+        }
         tc_fence_after();
         const uint32_t sv = smem_u32(sKV + st * C::kTile);
 #pragma unroll
         for (int s = 0; s < FN / 16; ++s) {
           const uint64_t bv = umma_desc_sw128_mn(sv + s * 16 * 128, C::kChunk, 1024u);
-          umma_f16_ts(tO, tP + pb * (FN / 2) + s * 8, bv, idesc_pv, (!first || s > 0) ? 1u : 0u);
+          umma_f16_ts(tO, tS + pb * FN + s * 8, bv, idesc_pv, (!first || s > 0) ? 1u : 0u);
         }
-        umma_commit(&p_free[pb]);
+        umma_commit(pv_done);
         umma_commit(&empty[st]);
         if (last) umma_commit(o_full);
         return true;
       };
-      bool ok = true, first_b = false, last_b = false;
+      bool ok = true, first_b = false, dirty_b = false;
       int n = 0;
-      while (ok && walk.next(p)) {
-        const int qb = units_s % NQ;
-        ok = mbar_wait(&q_full[qb], (uint32_t)((units_s / NQ) & 1), p.err);
-        ++units_s;
-        for (int j = walk.j0; j < walk.j1 && ok; ++j, ++n) {
-          const int pos = n == 0 ? 0 : 2 * n - 1, st = pos % NS, sb = n & 1;
-          if (!mbar_wait(&s_free[sb], (uint32_t)(((n >> 1) & 1) ^ 1), p.err) ||
-              !mbar_wait(&full[st], (uint32_t)((pos / NS) & 1), p.err)) {
+      Unit x;
+      while (ok && take(units, x, true) && x.j0 < x.j1) {
+        // The unit before ends first: its epilogue waits for it.
+        if (n > 0) ok = pv(n - 1, first_b, true, dirty_b);
+        ok = ok && mbar_wait(q_full, (uint32_t)(units & 1), p.err);
+        ++units;
+        for (int j = x.j0; j < x.j1 && ok; ++j, ++n) {
+          const int pos = pos_k(n), st = pos % NS, sb = n & 1;
+          // The S buffer is free: P V of tile n - 2, which reads P from it,
+          // was issued before, and MMAs run in order.
+          if (!mbar_wait(&full[st], (uint32_t)((pos / NS) & 1), p.err)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t sq = smem_u32(sQ + qb * C::kQBytes);
           const uint32_t sk = smem_u32(sKV + st * C::kTile);
 #pragma unroll
           for (int kb = 0; kb < kDC; ++kb) {
-            const uint64_t aq = umma_desc_sw128(sq + kb * C::kQChunk);
             const uint64_t bk = umma_desc_sw128(sk + kb * C::kChunk);
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              umma_f16(tS + sb * FN, aq + (uint64_t)(2 * k), bk + (uint64_t)(2 * k), idesc_s,
-                       (kb > 0 || k > 0) ? 1u : 0u);
+              umma_f16_ts(tS + sb * FN, tQ + (kb * 4 + k) * 8, bk + (uint64_t)(2 * k), idesc_s,
+                          (kb > 0 || k > 0) ? 1u : 0u);
           }
           umma_commit(&s_full[sb]);
           umma_commit(&empty[st]);
-          if (j == walk.j1 - 1) umma_commit(&q_empty[qb]);
-          if (n > 0) ok = pv(n - 1, first_b, last_b);
-          first_b = j == walk.j0;
-          last_b = j == walk.j1 - 1;
+          const bool dirty = x.template dirty<FN>(j);
+          // (At most two are out at a time: V_n comes back before S of tile
+          // n + 2. That tile n is at work also means that V_n's slot is in its
+          // present round, which is what the cleaner's wait for it relies on.)
+          if (dirty) mbar_arrive(&v_dirty[sent++ & 1]);
+          if (j > x.j0) ok = pv(n - 1, first_b, false, dirty_b);
+          first_b = j == x.j0;
+          dirty_b = dirty;
         }
       }
-      if (ok) pv(N - 1, first_b, last_b);
+      if (ok && n == N) pv(N - 1, first_b, true, dirty_b);
       // Every MMA done before the TMEM goes.
       umma_commit(done);
       mbar_wait(done, 0, p.err);
     }
     __syncwarp();
-  } else if (warp == 10) {
-    // -------------------------------------------------------------- Q loader
-    int units = 0;
-    while (walk.next(p)) {
-      const int qb = units % NQ;
-      int ok = 1;
-      if (lane == 0) ok = mbar_wait(&q_empty[qb], (uint32_t)(((units / NQ) & 1) ^ 1), p.err) ? 1 : 0;
-      if (!__shfl_sync(0xffffffffu, ok, 0)) break;
-      const int row0 = walk.row0(), kvh = walk.kvh();
-      const int rows = min(FM, walk.q.q_len * p.G - row0);
-      const uint32_t dst = smem_u32(sQ + qb * C::kQBytes);
-      // Spare rows of a softmax warp that has valid ones are zero; the others
-      // are never looked at.
-      const int fill = (rows + 31) / 32 * 32;
-      for (int i = lane; i < fill * (D / 8); i += 32) {
-        const int r = i / (D / 8), ch = i % (D / 8);
-        const bool valid = r < rows;
-        const int g = row0 + (valid ? r : 0);
-        const __nv_bfloat16* src = p.q + (long long)(walk.q.q0 + g / p.G) * p.q_stride +
-                                   (long long)(kvh * p.G + g % p.G) * D + ch * 8;
-        cp_async_16(dst + (ch >> 3) * C::kQChunk + sw_off(r, ch & 7), src, valid);
+  } else if (warp == 11) {
+    // --------------------------------------------------------------- cleaner
+    Unit x;
+    int n = 0, got = 0;
+    bool ok = true;
+    for (int u = 0; ok && take(u, x, false) && x.j0 < x.j1; ++u) {
+      for (int j = x.j0; j < x.j1 && ok; ++j, ++n) {
+        if (!x.template dirty<FN>(j)) continue;
+        const int pos = pos_v(n);
+        ok = __all_sync(0xffffffffu,
+                        mbar_wait(&v_dirty[got & 1], (uint32_t)((got >> 1) & 1), p.err) &&
+                            mbar_wait(&full[pos % NS], (uint32_t)((pos / NS) & 1), p.err));
+        if (!ok) break;
+        uint8_t* sv = sKV + (pos % NS) * C::kTile;
+        const int kbase = x.k_lo + j * FN;
+        constexpr int kU = D / 8;
+        auto zero = [&](int from, int to) {  // rows [from, to)
+          for (int i = from * kU + lane; i < to * kU; i += 32) {
+            const int k = i / kU, c16 = i % kU;
+            *reinterpret_cast<uint4*>(sv + (c16 >> 3) * C::kChunk + sw_off(k, c16 & 7)) =
+                make_uint4(0, 0, 0, 0);
+          }
+        };
+        zero(0, min(FN, x.k_first - kbase));
+        zero(max(0, x.seq_len - kbase), FN);
+        fence_proxy_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&v_clean[got & 1]);
+        ++got;
       }
-      asm volatile("cp.async.wait_all;" ::: "memory");
-      fence_proxy_async_shared();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&q_full[qb]);
-      ++units;
     }
   } else {
     // --------------------------------------------------------------- softmax
-    const int q4 = warp & 3;         // the 32 TMEM lanes this warp may touch
-    const int half = (warp - 2) / 4; // which half of the tile's keys
+    const int q4 = warp & 3;          // the 32 TMEM lanes this warp may touch
+    const int half = (warp - 2) / 4;  // which half of the tile's keys
     const int row = q4 * 32 + lane;
-    const int stid = (int)threadIdx.x - 64;  // 0 .. 255
-    constexpr int HN = FN / 2;               // keys of a half
-    constexpr int HD = D / 2;                // O columns of a half
+    constexpr int HN = FN / 2;        // keys of a half
+    constexpr int HD = D / 2;         // O columns of a half
     const uint32_t lane_base = (uint32_t)(q4 * 32) << 16;
     const float sc = p.scale_log2;
     const uint64_t sc2 = f32x2_pack(sc, sc);
     bool ok = true;
-    int n = 0, units = 0, meets = 0;
+    int n = 0, meets = 0;
     // Both warps of these 32 rows meet (a wait with a limit, like the others:
     // either may have given up).
     auto meet = [&]() -> bool {
@@ -474,33 +568,128 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
       ++meets;
       return __all_sync(0xffffffffu, r);
     };
-    while (ok && walk.next(p)) {
-      const int row0 = walk.row0(), kvh = walk.kvh();
-      const int n_rows = walk.q.q_len * p.G - row0;
-      const bool valid = row < n_rows;
-      const bool warp_on = q4 * 32 < n_rows;
-      const int node = (row0 + (valid ? row : 0)) / p.G;
-      const int head = kvh * p.G + (row0 + (valid ? row : 0)) % p.G;
-      const uint32_t* mrow = p.mask + (long long)(walk.q.q0 + node) * p.mask_words;
-      const int nodes = walk.q.nodes, prefix = walk.q.prefix, seq_len = walk.q.seq_len;
+    // This thread's half of a unit's Q row: to registers, then to TMEM (zero
+    // for spare rows, so that their scores are numbers).
+    uint4 qr[HD / 8];
+    auto load_q = [&](const Unit& x) {
+      const bool on = row < x.rows;
+      const int g = x.row0 + (on ? row : 0), t = g / p.G;
+      const __nv_bfloat16* src = p.q + (long long)(x.q0 + t) * p.q_stride +
+                                 (long long)(x.kvh * p.G + g - t * p.G) * D + half * HD;
+#pragma unroll
+      for (int i = 0; i < HD / 8; ++i) qr[i] = on ? ld_q(src + i * 8) : make_uint4(0, 0, 0, 0);
+    };
+    auto store_q = [&] {
+      const uint32_t dst = tQ + lane_base + half * (HD / 2);
+      if constexpr (HD == 32) {
+        tmem_st_32x32b_x16(dst, *reinterpret_cast<uint32_t(*)[16]>(qr));
+      } else {
+#pragma unroll
+        for (int c = 0; c < HD / 64; ++c)
+          tmem_st_32x32b_x32(dst + c * 32, *reinterpret_cast<uint32_t(*)[32]>(qr + 8 * c));
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+    };
+    // A finished unit's row, until its O is read.
+    struct Done {
+      long long dst;    // element of out, or of part_o for a cut unit
+      long long piece;  // row of part_ml, or -1 for a whole unit
+      float m, l;
+      int head;
+      bool valid, on;
+    } fin{0, -1, 0.f, 0.f, 0, false, false};
+    int finished = 0;
+    auto epilogue = [&]() -> bool {
+      if (!__all_sync(0xffffffffu, mbar_wait(o_full, (uint32_t)(finished & 1), p.err)))
+        return false;
+      ++finished;
+      tc_fence_after();
+      if (fin.on) {
+        const bool whole = fin.piece < 0;
+        float f = 1.f;
+        if (whole) {
+          float den = fin.l;
+          if (p.sinks != nullptr)
+            den = fin.m == -INFINITY
+                      ? 1.f
+                      : den + exp2f(p.sinks[fin.head] * 1.4426950408889634f - fin.m);
+          f = den > 0.f ? 1.f / den : 0.f;
+        } else if (fin.valid && half == 0) {
+          p.part_ml[fin.piece] = make_float2(fin.m, fin.l);
+        }
+#pragma unroll 1
+        for (int c = 0; c < HD / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld_32x32b_x32(tO + lane_base + half * HD + c * 32, o);  // warp-collective
+          tmem_wait_ld();
+          if (!fin.valid) continue;
+          if (whole) {
+            __nv_bfloat16* dst = p.out + fin.dst + c * 32;
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+              uint32_t w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                w[e] = pack_bf16x2(__uint_as_float(o[8 * v + 2 * e]) * f,
+                                   __uint_as_float(o[8 * v + 2 * e + 1]) * f);
+              *reinterpret_cast<uint4*>(dst + v * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          } else {
+            float* dst = p.part_o + fin.dst + c * 32;
+#pragma unroll
+            for (int v = 0; v < 8; ++v)
+              *reinterpret_cast<uint4*>(dst + v * 4) =
+                  make_uint4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(o_free);
+      return true;
+    };
+
+    Unit x, next;
+    ok = take(0, next, false);
+    if (ok && next.j0 < next.j1) {
+      load_q(next);
+      store_q();
+    }
+    for (int u = 0; ok && next.j0 < next.j1; ++u) {
+      x = next;
+      const bool valid = row < x.rows;
+      const bool warp_on = q4 * 32 < x.rows;
+      const int g = x.row0 + (valid ? row : 0), node = g / p.G;
+      const int head = x.kvh * p.G + g - node * p.G;
+      MaskRow mask{p.mask + (long long)(x.q0 + node) * p.mask_words, p.mask_words, x.nodes, 0u, 0u};
+      mask.w0 = ld_word(mask.row);
+      if (p.mask_words > 1) mask.w1 = ld_word(mask.row + 1);
       // First key of the prefix this row sees. A node's position is the
       // prefix plus its depth, the number of its ancestors.
       int key_lo = 0;
       if (p.window > 0 && warp_on) {
         int depth = 0;
-        for (int i = 0; 32 * i < nodes; ++i)
-          depth += __popc(mask_word(mrow, p.mask_words, nodes, i));
-        key_lo = prefix + max(depth - 1, 0) - p.window + 1;
+        for (int i = 0; 32 * i < x.nodes; ++i) depth += __popc(mask.word(i));
+        key_lo = x.prefix + max(depth - 1, 0) - p.window + 1;
       }
       // Exponent reference (log2 units; the same in both halves), this half's sum.
       float m_used = -INFINITY, l = 0.f;
-      for (int j = walk.j0; j < walk.j1; ++j, ++n) {
+      for (int j = x.j0; j < x.j1; ++j, ++n) {
         const int sb = n & 1;
         ok = __all_sync(0xffffffffu, mbar_wait(&s_full[sb], (uint32_t)((n >> 1) & 1), p.err));
         if (!ok) break;
         tc_fence_after();
-        const int kbase = walk.q.k_lo + j * FN;
-        const int kb = kbase + half * HN;
+        // The unit's last S is there: Q may be replaced.
+        bool stage_q = false;
+        if (j == x.j1 - 1) {
+          ok = take(u + 1, next, false);
+          if (!ok) break;
+          stage_q = next.j0 < next.j1;
+          if (stage_q) load_q(next);
+        }
         if (warp_on) {
           // The half row of scores, masked, and its maximum.
           uint32_t r[HN / 32][32];
@@ -508,13 +697,13 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
           for (int w = 0; w < HN / 32; ++w)
             tmem_ld_32x32b_x32(tS + lane_base + sb * FN + half * HN + w * 32, r[w]);
           tmem_wait_ld();
-          if (__any_sync(0xffffffffu, key_lo > kb) || kb + HN > prefix) {
+          const int kb = x.k_lo + j * FN + half * HN;
+          if (__any_sync(0xffffffffu, key_lo > kb) || kb + HN > x.prefix) {
 #pragma unroll
             for (int w = 0; w < HN / 32; ++w) {
               const int k0 = kb + 32 * w;
-              const uint32_t vis = valid ? range_bits(key_lo - k0, prefix - k0) |
-                                               mask_bits(mrow, p.mask_words, nodes, k0 - prefix)
-                                         : 0u;
+              const uint32_t vis =
+                  valid ? range_bits(key_lo - k0, x.prefix - k0) | mask.bits(k0 - x.prefix) : 0u;
 #pragma unroll
               for (int i = 0; i < 32; ++i)
                 if (!((vis >> i) & 1u)) r[w][i] = 0xff800000u;
@@ -538,10 +727,9 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
               l *= alpha;
               m_used = mx;
             }
-            if (j > walk.j0) {
+            if (j > x.j0) {
               // O is final for the tiles before once P V of tile n - 1 is done.
-              ok = __all_sync(0xffffffffu, mbar_wait(&p_free[sb ^ 1],
-                                                     (uint32_t)(((n - 1) >> 1) & 1), p.err));
+              ok = __all_sync(0xffffffffu, mbar_wait(pv_done, (uint32_t)((n - 1) & 1), p.err));
               if (!ok) break;
               tc_fence_after();
 #pragma unroll 1
@@ -575,11 +763,9 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
           float a0, a1;
           f32x2_unpack(f32x2_add(acc[0], acc[1]), a0, a1);
           l += a0 + a1;
-          // This P buffer is free once P V of tile n - 2 has completed.
-          if (n >= 2) ok = mbar_wait(&p_free[sb], (uint32_t)(((n - 2) >> 1) & 1), p.err);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          const uint32_t p_row = tP + lane_base + sb * (FN / 2) + half * (HN / 2);
+          // P goes over the first half of its S buffer: both warps have read
+          // their scores (they met).
+          const uint32_t p_row = tS + lane_base + sb * FN + half * (HN / 2);
           if constexpr (HN == 64)
             tmem_st_32x32b_x32(p_row, *reinterpret_cast<uint32_t(*)[32]>(w));
           else
@@ -588,31 +774,17 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&s_free[sb]);
-        if (kbase + FN > seq_len || kbase < walk.q.k_first) {
-          // V rows that no node sees (past the end, before the window) may
-          // hold anything, and 0 x NaN is not 0: they become zero.
-          const int pos = pos_v(n);
-          ok = __all_sync(0xffffffffu,
-                          mbar_wait(&full[pos % NS], (uint32_t)((pos / NS) & 1), p.err));
-          if (!ok) break;
-          uint8_t* sv = sKV + (pos % NS) * C::kTile;
-          constexpr int kU = D / 8;
-          for (int i = stid; i < FN * kU; i += kSoftmaxWarps * 32) {
-            const int k = i / kU, c16 = i % kU;
-            if (kbase + k >= seq_len || kbase + k < walk.q.k_first)
-              *reinterpret_cast<uint4*>(sv + (c16 >> 3) * C::kChunk + sw_off(k, c16 & 7)) =
-                  make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async_shared();
-          __syncwarp();
-        }
         if (lane == 0) mbar_arrive(&p_full[sb]);
+        if (stage_q) store_q();
+        if (j == x.j0 && u > 0) {
+          ok = epilogue();  // of the unit before
+          if (!ok) break;
+        }
       }
       if (!ok) break;
-      // ---------------------------------------------------- the unit's epilogue
       if (warp_on) {
-        // (The buffer is the next unit's first tile's, hence the second meeting.)
+        // The row's sum: the halves' (in the buffer of the next unit's first
+        // tile, hence the second meeting).
         sh_max[n & 1][half][row] = l;
         ok = meet();
         if (!ok) break;
@@ -620,53 +792,17 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
         ok = meet();
         if (!ok) break;
       }
-      ok = __all_sync(0xffffffffu, mbar_wait(o_full, (uint32_t)(units & 1), p.err));
-      if (!ok) break;
-      ++units;
-      tc_fence_after();
-      if (warp_on) {
-        const bool whole = walk.j0 == 0 && walk.j1 == walk.q.n_tiles;
-        float f = 1.f;
-        if (whole) {
-          float den = l;
-          if (p.sinks != nullptr)
-            den = m_used == -INFINITY ? 1.f
-                                      : l + exp2f(p.sinks[head] * 1.4426950408889634f - m_used);
-          f = den > 0.f ? 1.f / den : 0.f;
-        }
-        __nv_bfloat16* dst = p.out + (long long)(walk.q.q0 + node) * p.o_stride +
-                             (long long)head * D + half * HD;
-        const long long piece = ((long long)blockIdx.x * 2 + (walk.j0 > 0 ? 0 : 1)) * FM + row;
-        float* part = p.part_o + piece * D + half * HD;
-        if (!whole && valid && half == 0) p.part_ml[piece] = make_float2(m_used, l);
-#pragma unroll 1
-        for (int c = 0; c < HD / 32; ++c) {
-          uint32_t o[32];
-          tmem_ld_32x32b_x32(tO + lane_base + half * HD + c * 32, o);  // warp-collective
-          tmem_wait_ld();
-          if (!valid) continue;
-          if (whole) {
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
-              uint32_t w[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                w[e] = pack_bf16x2(__uint_as_float(o[8 * v + 2 * e]) * f,
-                                   __uint_as_float(o[8 * v + 2 * e + 1]) * f);
-              *reinterpret_cast<uint4*>(dst + c * 32 + v * 8) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-          } else {
-#pragma unroll
-            for (int v = 0; v < 8; ++v)
-              *reinterpret_cast<uint4*>(part + c * 32 + v * 4) =
-                  make_uint4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
-          }
-        }
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(o_free);
+      fin.m = m_used;
+      fin.l = l;
+      fin.head = head;
+      fin.valid = valid;
+      fin.on = warp_on;
+      // A cut unit leaves pieces: 0 for one that began before this share.
+      fin.piece = x.whole ? -1 : ((long long)blockIdx.x * 2 + (x.j0 > 0 ? 0 : 1)) * FM + row;
+      fin.dst = (x.whole ? (long long)(x.q0 + node) * p.o_stride + (long long)head * D
+                         : fin.piece * D) + half * HD;
     }
+    if (ok && n > 0) epilogue();
   }
   tc_fence_before();
   __syncthreads();
@@ -676,71 +812,69 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
   }
 }
 
-// Joins the pieces of units that were cut, in share order: one warp a
-// (token, head) row. Rows of whole units return at once.
+// Joins the pieces of units that were cut, in share order. Block (c - 1, y)
+// looks at the edge before share c: if the unit there began in share c - 1, it
+// joins 16 of its rows, a warp a row.
 template <int D_>
 __global__ void __launch_bounds__(128) tree_join_kernel(const Params p) {
   constexpr int D = D_, FN = Cfg<D_>::FN;
   constexpr int V = D >= 128 ? D / 128 : 1;  // float4 of a lane
   pdl_wait();
   pdl_trigger();
-  const long long id = (long long)blockIdx.x * 4 + threadIdx.x / 32;
+  const int c1 = blockIdx.x + 1;
+  const Cut cut = p.cut[c1];
+  if (cut.j0 == 0) return;
+  const int share = (int)*p.share;
+  const Seq q = load_seq<FN>(p, cut.seq);
+  const long long a = (long long)c1 * share - cut.j0;  // the unit's first tile
+  if (cut.j0 > share) return;                          // an earlier edge joins it
+  const int kvh = cut.unit / q.n_rt, row0 = (cut.unit - kvh * q.n_rt) * FM;
+  const int c_last = (int)((a + q.n_tiles - 1) / share);
   const int lane = threadIdx.x % 32;
-  if (id >= p.T * p.Hq) return;
-  const int tok = (int)(id / p.Hq), head = (int)(id % p.Hq);
-  // The token's sequence: the last s with cu_q[s] <= tok.
-  int lo = 0, hi = p.num_seqs - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
-    if (p.cu_q[mid] <= tok) lo = mid;
-    else hi = mid - 1;
-  }
-  const Seq q = load_seq<FN>(p, lo);
-  if (tok < q.q0 || tok >= q.q0 + q.q_len) return;
-  const int g = (tok - q.q0) * p.G + head % p.G;
-  const int unit = head / p.G * q.n_rt + g / FM, row = g % FM;
-  const long long share = p.seq_tile[p.num_seqs + 1];
-  const long long a = p.seq_tile[lo] + (long long)unit * q.n_tiles, b = a + q.n_tiles;
-  const int c0 = (int)(a / share), c1 = (int)((b - 1) / share);
-  if (c0 == c1) return;
-  auto piece = [&](int c) {
-    return ((long long)c * 2 + (a < c * share ? 0 : 1)) * FM + row;
-  };
-  float m = -INFINITY;
-  for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, p.part_ml[piece(c)].x);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  float den = 0.f;
-  float4 acc[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
   const bool on = D >= 128 || lane < D / 4;
-  for (int c = c0; c <= c1; ++c) {
-    const long long pc = piece(c);
-    const float2 ml = p.part_ml[pc];
-    const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m);
-    den += ml.y * f;
-    if (on) {
+  for (int row = blockIdx.y * 16 + threadIdx.x / 32; row < min(FM, (int)blockIdx.y * 16 + 16);
+       row += 4) {
+    const int g = row0 + row;
+    if (g >= q.q_len * p.G) return;
+    const int t = g / p.G, head = kvh * p.G + g - t * p.G;
+    // The first piece is the last of share c1 - 1, the others open theirs.
+    auto piece = [&](int c) { return ((long long)c * 2 + (c < c1 ? 1 : 0)) * FM + row; };
+    float m = -INFINITY;
+    for (int c = c1 - 1 + lane; c <= c_last; c += 32) m = fmaxf(m, p.part_ml[piece(c)].x);
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const float4 o = *reinterpret_cast<const float4*>(p.part_o + pc * D + (v * 32 + lane) * 4);
-        acc[v].x += o.x * f;
-        acc[v].y += o.y * f;
-        acc[v].z += o.z * f;
-        acc[v].w += o.w * f;
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float den = 0.f;
+    float4 acc[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int c = c1 - 1; c <= c_last; ++c) {
+      const long long pc = piece(c);
+      const float2 ml = p.part_ml[pc];
+      const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m);
+      den += ml.y * f;
+      if (on) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const float4 o = *reinterpret_cast<const float4*>(p.part_o + pc * D + (v * 32 + lane) * 4);
+          acc[v].x += o.x * f;
+          acc[v].y += o.y * f;
+          acc[v].z += o.z * f;
+          acc[v].w += o.w * f;
+        }
       }
     }
-  }
-  if (p.sinks != nullptr)
-    den = m == -INFINITY ? 1.f : den + exp2f(p.sinks[head] * 1.4426950408889634f - m);
-  const float inv = den > 0.f ? 1.f / den : 0.f;
-  if (on) {
-    __nv_bfloat16* dst = p.out + (long long)tok * p.o_stride + (long long)head * D;
+    if (p.sinks != nullptr)
+      den = m == -INFINITY ? 1.f : den + exp2f(p.sinks[head] * 1.4426950408889634f - m);
+    const float inv = den > 0.f ? 1.f / den : 0.f;
+    if (on) {
+      __nv_bfloat16* dst = p.out + (long long)(q.q0 + t) * p.o_stride + (long long)head * D;
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-      *reinterpret_cast<uint2*>(dst + (v * 32 + lane) * 4) =
-          make_uint2(pack_bf16x2(acc[v].x * inv, acc[v].y * inv),
-                     pack_bf16x2(acc[v].z * inv, acc[v].w * inv));
+      for (int v = 0; v < V; ++v)
+        *reinterpret_cast<uint2*>(dst + (v * 32 + lane) * 4) =
+            make_uint2(pack_bf16x2(acc[v].x * inv, acc[v].y * inv),
+                       pack_bf16x2(acc[v].z * inv, acc[v].w * inv));
+    }
   }
 }
 
@@ -773,7 +907,8 @@ void launch_d(const TreeAttnArgs& a, cudaStream_t stream) {
   p.sinks = a.sinks;
   p.part_o = a.workspace;
   p.part_ml = reinterpret_cast<float2*>(a.workspace + (size_t)grid * 2 * FM * D);
-  p.seq_tile = reinterpret_cast<long long*>(p.part_ml + (size_t)grid * 2 * FM);
+  p.cut = reinterpret_cast<Cut*>(p.part_ml + (size_t)grid * 2 * FM);
+  p.share = reinterpret_cast<long long*>(p.cut + grid);
   p.num_seqs = a.num_seqs;
   p.Hq = a.Hq;
   p.Hkv = a.Hkv;
@@ -790,14 +925,14 @@ void launch_d(const TreeAttnArgs& a, cudaStream_t stream) {
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.err = device_status_ptr(dev);
   launch_pdl(kernel, dim3(grid), dim3(kThreads), C::kSmem, stream, nullptr, tk, tv, p);
-  launch_pdl(tree_join_kernel<D>, dim3((unsigned)((a.num_tokens * a.Hq + 3) / 4)), dim3(128), 0,
-             stream, nullptr, p);
+  if (grid > 1)
+    launch_pdl(tree_join_kernel<D>, dim3(grid - 1, FM / 16), dim3(128), 0, stream, nullptr, p);
 }
 
 }  // namespace
 
-size_t tree_attention_workspace_bytes(int num_seqs, int head_dim, int num_sm) {
-  return (size_t)num_sm * 2 * FM * (head_dim + 2) * 4 + (size_t)(num_seqs + 2) * 8;
+size_t tree_attention_workspace_bytes(int head_dim, int num_sm) {
+  return (size_t)num_sm * (2 * FM * (head_dim + 2) * 4 + sizeof(Cut)) + 16;
 }
 
 void tree_attention_launch(const TreeAttnArgs& a, cudaStream_t stream) {
@@ -805,6 +940,10 @@ void tree_attention_launch(const TreeAttnArgs& a, cudaStream_t stream) {
     throw std::runtime_error("tree_attention: Hq must be a multiple of Hkv");
   if (a.block_size < 8 || (a.block_size & (a.block_size - 1)) != 0)
     throw std::runtime_error("tree_attention: block_size must be a power of two >= 8");
+  // Tiles of one sequence are counted in 32 bits.
+  const double tiles = ((double)a.max_blocks * a.block_size / 64 + 1) * a.Hkv *
+                       ((double)a.num_tokens * (a.Hq / a.Hkv) / FM + 1);
+  if (tiles > 2e9) throw std::runtime_error("tree_attention: block table too wide for the batch");
   if (a.num_tokens <= 0 || a.num_seqs <= 0) return;
   switch (a.head_dim) {
     case 64: return launch_d<64>(a, stream);

@@ -23,7 +23,7 @@ struct TreeAttnArgs {
   float scale;
 };
 
-size_t tree_attention_workspace_bytes(int num_seqs, int head_dim, int num_sm);
+size_t tree_attention_workspace_bytes(int head_dim, int num_sm);
 void tree_attention_launch(const TreeAttnArgs& a, cudaStream_t stream);
 
 }  // namespace b200

@@ -17,9 +17,8 @@ int sm_count(int dev) {
   return n > 0 ? n : 148;
 }
 
-int64_t tree_attention_workspace(int64_t num_seqs, int64_t head_dim, int64_t device) {
-  return (int64_t)tree_attention_workspace_bytes((int)num_seqs, (int)head_dim,
-                                                 sm_count((int)device));
+int64_t tree_attention_workspace(int64_t head_dim, int64_t device) {
+  return (int64_t)tree_attention_workspace_bytes((int)head_dim, sm_count((int)device));
 }
 
 bool aligned16(const at::Tensor& t) {
@@ -77,7 +76,7 @@ void tree_attention(at::Tensor& out, const at::Tensor& q, const at::Tensor& k_ca
                 what, ": sinks must be fp32 [Hq]");
   if (T == 0 || B == 0) return;
   c10::cuda::CUDAGuard g(q.device());
-  const int64_t need = tree_attention_workspace(B, D, q.get_device());
+  const int64_t need = tree_attention_workspace(D, q.get_device());
   at::Tensor ws;
   if (workspace) {
     ws = *workspace;
@@ -122,7 +121,7 @@ TORCH_LIBRARY_FRAGMENT(_b200_C, m) {
   m.def("tree_attention(Tensor(a!) out, Tensor q, Tensor k_cache, Tensor v_cache, "
         "Tensor block_table, Tensor seq_lens, Tensor cu_q, Tensor tree_mask, float scale, "
         "int window=0, Tensor? sinks=None, Tensor(b!)? workspace=None) -> ()");
-  m.def("tree_attention_workspace(int num_seqs, int head_dim, int device) -> int",
+  m.def("tree_attention_workspace(int head_dim, int device) -> int",
         &b200::tree_attention_workspace);
 }
 

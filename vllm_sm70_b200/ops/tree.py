@@ -98,14 +98,14 @@ def tree_attention_ref(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
     return out
 
 
-def tree_attention_workspace(num_seqs: int, head_dim: int, device) -> torch.Tensor:
-    """A workspace for :func:`tree_attention` calls of up to ``num_seqs``
-    sequences on ``device`` (kept by a caller that captures graphs; calls that
-    may overlap on different streams need one each)."""
+def tree_attention_workspace(head_dim: int, device) -> torch.Tensor:
+    """A workspace for :func:`tree_attention` calls on ``device`` (kept by a
+    caller that captures graphs; calls that may overlap on different streams
+    need one each)."""
     _ext.require()
     dev = torch.device(device)
     index = dev.index if dev.index is not None else torch.cuda.current_device()
-    n = torch.ops._b200_C.tree_attention_workspace(num_seqs, head_dim, index)
+    n = torch.ops._b200_C.tree_attention_workspace(head_dim, index)
     return torch.empty(n, dtype=torch.uint8, device=dev)
 
 
