@@ -29,25 +29,21 @@
 //              ring in the order of use K0 K1 V0 K2 V1 ... Warp 0 also walks
 //              the share and publishes each unit's numbers, one unit ahead, so
 //              that nobody else waits for lengths or divides.
-//   warp 1     TMEM owner and MMA issuer: S = Q K^T into one of two S buffers,
-//              then O += P V of the tile before it. Q and P are TMEM operands,
-//              so shared memory feeds the tensor core with K and V alone.
-//   warps 2-9  softmax: two threads a row, one for each half of the tile's
-//              keys (warps w and w + 4 of the same 32 TMEM lanes), which
-//              exchange their maxima through shared memory. Exponentials in
-//              base 2 with a lazily raised reference (O is rescaled when a
-//              row's max grows by more than 2^8 over it), P as bf16 over the
-//              first half of its S buffer. In a unit's last tile they bring
-//              the next unit's Q rows to TMEM; a unit's epilogue (half of O's
-//              columns each) comes after the next unit's first tile, when the
-//              last P V has long finished.
-//   warp 11    zeroes V rows that no node sees (past the end, before the
+//   warp 1     TMEM owner and MMA issuer: S = Q K^T into one of two S buffers
+//              and O += P V, each in tile order, whichever is ready first (S
+//              at most two tiles ahead)
+//   warps 2-9  softmax: two groups of four warps, a row a thread, on every
+//              other tile, so that one's waits are the other's work. O has one
+//              exponent reference a row (base 2, raised lazily: O is rescaled
+//              when a row's max grows by more than 2^8 over it), which the
+//              groups hand to each other in tile order through shared memory
+//              as soon as a tile's maximum is known. A unit's epilogue (half
+//              of O's columns each) comes after the next unit's first tile,
+//              when the last P V has long finished.
+//   warp 11    loads Q rows (the next unit's while the present one runs) and
+//              zeroes V rows that no node sees (past the end, before the
 //              window): they may hold anything, and 0 x NaN is not 0.
-// TMEM columns: S0 | S1 | O | Q.
-//
-// Bound: HBM for up to 128 rows a key head (a 64 KB key tile takes ~2800 SM
-// cycles to arrive; the softmax, the longest chain, ~2400, of which 1024 are
-// the multi-function unit's), the softmax beyond.
+// TMEM columns: S0 | S1 | O | P0 | P1.
 //
 // Rounding: P is rounded to bf16 for the tensor core (relative 2^-8 a term at
 // most, as the output's own rounding); scores, maxima, sums and O are fp32.
@@ -73,9 +69,9 @@ namespace {
 constexpr int FM = 128;
 constexpr int kThreads = 384;
 constexpr int kSoftmaxWarps = 8;
-constexpr int kBarBytes = 768;  // barriers and published units
+constexpr int kBarBytes = 1024;  // barriers and published units
 constexpr int kUnits = 4;       // published units
-constexpr int kMaxBytes = 2 * 2 * FM * 4;  // [tile parity][half][row] floats
+constexpr int kRowBytes = 3 * FM * 4;  // a reference and two sums a row
 constexpr int kMinShare = 2;  // key tiles of a CTA, at least
 
 template <int D_>
@@ -83,11 +79,14 @@ struct Cfg {
   static constexpr int D = D_;
   static constexpr int FN = D <= 128 ? 128 : 64;  // keys of a tile
   static constexpr int kDC = D / 64;              // 64-column chunks of a row
+  static constexpr int kQChunk = FM * 128;
+  static constexpr int kQBytes = kDC * kQChunk;
+  static constexpr int NQ = D <= 128 ? 2 : 1;     // Q buffers
   static constexpr int kChunk = FN * 128;
   static constexpr int kTile = kDC * kChunk;      // K or V of a tile
-  static constexpr int NS = D == 64 ? 14 : 7;     // ring slots: 224 KB
-  static constexpr int kSmem = NS * kTile + kBarBytes + kMaxBytes;
-  static_assert(2 * FN + D + D / 2 <= 512, "TMEM columns");
+  static constexpr int NS = D == 64 ? 12 : 5;     // ring slots
+  static constexpr int kSmem = NQ * kQBytes + NS * kTile + kBarBytes + kRowBytes;
+  static_assert(3 * FN + D <= 512, "TMEM columns");
   static_assert(kSmem <= 232448, "shared memory");
 };
 
@@ -118,20 +117,29 @@ struct Params {
 __device__ __forceinline__ uint32_t sw_off(int row, int chunk) {
   return (uint32_t)(row * 128 + ((chunk ^ (row & 7)) << 4));
 }
-// (volatile: issued where they stand, ahead of the tile's work)
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool valid) {
+  const int sz = valid ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(sz)
+               : "memory");
+}
+// Whether the phase of the given parity has completed (never waits).
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred P;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 P, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, P;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// (volatile: issued where it stands, ahead of the tile's work)
 __device__ __forceinline__ uint32_t ld_word(const uint32_t* p) {
   uint32_t v;
   asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(v) : "l"(p));
   return v;
 }
-__device__ __forceinline__ uint4 ld_q(const __nv_bfloat16* p) {
-  uint4 v;
-  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
-}
-
 // One sequence's part of the work.
 struct Seq {
   int q0, q_len, seq_len, nodes, prefix, k_first, k_lo, n_tiles, n_rt;
@@ -230,31 +238,36 @@ __global__ void __launch_bounds__(kThreads, 1)
 tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
                  const Params p) {
   using C = Cfg<D_>;
-  constexpr int D = C::D, FN = C::FN, kDC = C::kDC, NS = C::NS;
+  constexpr int D = C::D, FN = C::FN, kDC = C::kDC, NS = C::NS, NQ = C::NQ;
   // The 128-byte swizzle wants 1024-byte aligned tiles: all shared memory is
   // dynamic, and there is no room for a margin.
   extern __shared__ __align__(1024) uint8_t smem[];
-  uint8_t* sKV = smem;
+  uint8_t* sQ = smem;
+  uint8_t* sKV = sQ + NQ * C::kQBytes;
   uint64_t* full = reinterpret_cast<uint64_t*>(sKV + NS * C::kTile);  // [NS]
   uint64_t* empty = full + NS;                                        // [NS]
-  uint64_t* s_full = empty + NS;                                      // [2]
-  uint64_t* p_full = s_full + 2;                                      // [2]
-  uint64_t* pair = p_full + 2;                                        // [4]
-  uint64_t* q_full = pair + 4;
-  uint64_t* pv_done = q_full + 1;
-  uint64_t* o_full = pv_done + 1;
+  uint64_t* q_full = empty + NS;                                      // [2]
+  uint64_t* q_empty = q_full + 2;                                     // [2]
+  uint64_t* s_full = q_empty + 2;                                     // [2]
+  uint64_t* s_free = s_full + 2;                                      // [2]
+  uint64_t* p_full = s_free + 2;                                      // [2]
+  uint64_t* p_free = p_full + 2;                                      // [2]
+  uint64_t* post = p_free + 2;                                        // [2][4]
+  uint64_t* pair = post + 8;                                          // [4]
+  uint64_t* o_full = pair + 4;
   uint64_t* o_free = o_full + 1;
   uint64_t* done = o_free + 1;
   uint64_t* u_full = done + 1;                                        // [kUnits]
   uint64_t* u_empty = u_full + kUnits;                                // [kUnits]
-  uint64_t* v_dirty = u_empty + kUnits;                               // [2]
-  uint64_t* v_clean = v_dirty + 2;                                    // [2]
-  int* share_of = reinterpret_cast<int*>(v_clean + 2);  // sequence, offset, tiles
+  uint64_t* v_dirty = u_empty + kUnits;                               // [4]
+  uint64_t* v_clean = v_dirty + 4;                                    // [4]
+  int* share_of = reinterpret_cast<int*>(v_clean + 4);  // sequence, offset, tiles
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(share_of + 3);
-  static_assert((2 * NS + 8 + 5 + 2 * kUnits + 4) * 8 + 16 + kUnits * (int)sizeof(Unit) <= kBarBytes,
-                "barriers and units");
+  static_assert((2 * NS + 12 + 12 + 3 + 2 * kUnits + 8) * 8 + 16 +
+                    kUnits * (int)sizeof(Unit) <= kBarBytes, "barriers and units");
   Unit* units_sh = reinterpret_cast<Unit*>(sKV + NS * C::kTile + kBarBytes) - kUnits;
-  float(*sh_max)[2][FM] = reinterpret_cast<float(*)[2][FM]>(sKV + NS * C::kTile + kBarBytes);
+  float* sh_ref = reinterpret_cast<float*>(sKV + NS * C::kTile + kBarBytes);  // [FM]
+  float* sh_sum = sh_ref + FM;                                                // [2][FM]
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   pdl_wait();
@@ -264,14 +277,19 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
       mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], kSoftmaxWarps);
+      mbar_init(&s_free[i], 4);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&p_free[i], 1);
+    }
+    for (int i = 0; i < 8; ++i) mbar_init(&post[i], 1);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&pair[i], 2);
       mbar_init(&v_dirty[i], 1);
       mbar_init(&v_clean[i], 1);
     }
-    for (int i = 0; i < 4; ++i) mbar_init(&pair[i], 2);
-    mbar_init(q_full, kSoftmaxWarps);
-    mbar_init(pv_done, 1);
     mbar_init(o_full, 1);
     mbar_init(o_free, kSoftmaxWarps);
     mbar_init(done, 1);
@@ -342,19 +360,20 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
   tc_fence_after();
   if (threadIdx.x == 0) pdl_trigger();
   const uint32_t tmem_base = *tmem_slot;
-  const uint32_t tS = tmem_base, tO = tS + 2 * FN, tQ = tO + D;
+  const uint32_t tS = tmem_base, tO = tS + 2 * FN, tP = tO + D;
   const int N = share_of[2];  // key tiles of this CTA
   // Ring positions.
   auto pos_k = [&](int n) { return n == 0 ? 0 : 2 * n - 1; };
   auto pos_v = [&](int n) { return n == N - 1 ? 2 * N - 1 : 2 * n + 2; };
 
   // Unit u for a reader (a warp, or one thread with `alone`).
-  auto take = [&](int u, Unit& x, bool alone) -> bool {
+  // `keep`: it is read again later.
+  auto take = [&](int u, Unit& x, bool alone, bool keep = false) -> bool {
     const int e = u % kUnits;
     const bool ok = mbar_wait(&u_full[e], (uint32_t)((u / kUnits) & 1), p.err);
     x = units_sh[e];
     if (!alone) __syncwarp();
-    if (alone || lane == 0) mbar_arrive(&u_empty[e]);
+    if (!keep && (alone || lane == 0)) mbar_arrive(&u_empty[e]);
     return alone ? ok : __all_sync(0xffffffffu, ok);
   };
 
@@ -443,90 +462,135 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
     if (lane == 0 && N > 0) {
       constexpr uint32_t idesc_s = umma_idesc_f16(FM, FN, true);
       constexpr uint32_t idesc_pv = umma_idesc_f16(FM, D, true) | (1u << 16);  // B MN-major
-      int units = 0, units_o = 0;  // units whose S / whose P V has begun
+      // Two cursors over the tiles: the next S and the next P V.
+      Unit a, b;
+      bool ok = take(0, a, true, true) && take(0, b, true);
+      int ns = 0, ja = a.j0, ua = 0, np = 0, jb = b.j0, ub = 0;
       int sent = 0, cleaned = 0;  // dirty V tiles given to the cleaner / taken back
-      auto pv = [&](int n, bool first, bool last, bool dirty) -> bool {
-        const int pos = pos_v(n), st = pos % NS, pb = n & 1;
-        if (first) {
-          // O is free once the epilogue of the unit before has read it.
-          if (!mbar_wait(o_free, (uint32_t)((units_o & 1) ^ 1), p.err)) return false;
-          ++units_o;
-        }
-        if (!mbar_wait(&p_full[pb], (uint32_t)((n >> 1) & 1), p.err) ||
-            !mbar_wait(&full[st], (uint32_t)((pos / NS) & 1), p.err))
-          return false;
-        if (dirty) {
-          if (!mbar_wait(&v_clean[cleaned & 1], (uint32_t)((cleaned >> 1) & 1), p.err))
-            return false;
-          ++cleaned;
-        }
-        tc_fence_after();
-        const uint32_t sv = smem_u32(sKV + st * C::kTile);
+      unsigned long long since = 0;
+      uint32_t spins = 0;
+      while (ok && np < N) {
+        bool moved = false;
+        // S of tile ns: its buffer has been read, K is there, and Q.
+        if (ns < N && ns - np < 3) {
+          const int pos = pos_k(ns), st = pos % NS, sb = ns & 1, qb = ua % NQ;
+          if ((ns < 2 || mbar_test(&s_free[sb], (uint32_t)(((ns >> 1) & 1) ^ 1))) &&
+              mbar_test(&full[st], (uint32_t)((pos / NS) & 1)) &&
+              (ja > a.j0 || mbar_test(&q_full[qb], (uint32_t)((ua / NQ) & 1)))) {
+            tc_fence_after();
+            const uint32_t sq = smem_u32(sQ + qb * C::kQBytes);
+            const uint32_t sk = smem_u32(sKV + st * C::kTile);
 #pragma unroll
-        for (int s = 0; s < FN / 16; ++s) {
-          const uint64_t bv = umma_desc_sw128_mn(sv + s * 16 * 128, C::kChunk, 1024u);
-          umma_f16_ts(tO, tS + pb * FN + s * 8, bv, idesc_pv, (!first || s > 0) ? 1u : 0u);
+            for (int kb = 0; kb < kDC; ++kb) {
+              const uint64_t aq = umma_desc_sw128(sq + kb * C::kQChunk);
+              const uint64_t bk = umma_desc_sw128(sk + kb * C::kChunk);
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                umma_f16(tS + sb * FN, aq + (uint64_t)(2 * k), bk + (uint64_t)(2 * k), idesc_s,
+                         (kb > 0 || k > 0) ? 1u : 0u);
+            }
+            umma_commit(&s_full[sb]);
+            umma_commit(&empty[st]);
+            // (S runs at most two tiles ahead: three are out at most, and the
+            // barriers hold four. That tile ns is at work also means that its
+            // V slot is in its present round: the cleaner's wait relies on it.)
+            if (a.template dirty<FN>(ja)) mbar_arrive(&v_dirty[sent++ & 3]);
+            ++ns;
+            if (++ja == a.j1) {
+              umma_commit(&q_empty[qb]);
+              ok = take(++ua, a, true, true);
+              ja = a.j0;
+            }
+            moved = true;
+          }
         }
-        umma_commit(pv_done);
-        umma_commit(&empty[st]);
-        if (last) umma_commit(o_full);
-        return true;
-      };
-      bool ok = true, first_b = false, dirty_b = false;
-      int n = 0;
-      Unit x;
-      while (ok && take(units, x, true) && x.j0 < x.j1) {
-        // The unit before ends first: its epilogue waits for it.
-        if (n > 0) ok = pv(n - 1, first_b, true, dirty_b);
-        ok = ok && mbar_wait(q_full, (uint32_t)(units & 1), p.err);
-        ++units;
-        for (int j = x.j0; j < x.j1 && ok; ++j, ++n) {
-          const int pos = pos_k(n), st = pos % NS, sb = n & 1;
-          // The S buffer is free: P V of tile n - 2, which reads P from it,
-          // was issued before, and MMAs run in order.
-          if (!mbar_wait(&full[st], (uint32_t)((pos / NS) & 1), p.err)) {
+        // P V of tile np: P and V are there, V clean, O free.
+        if (ok && np < ns) {
+          const int pos = pos_v(np), st = pos % NS, pb = np & 1;
+          const bool first = jb == b.j0, last = jb == b.j1 - 1, dirty = b.template dirty<FN>(jb);
+          if (mbar_test(&p_full[pb], (uint32_t)((np >> 1) & 1)) &&
+              mbar_test(&full[st], (uint32_t)((pos / NS) & 1)) &&
+              (!dirty || mbar_test(&v_clean[cleaned & 3], (uint32_t)((cleaned >> 2) & 1))) &&
+              (!first || mbar_test(o_free, (uint32_t)((ub & 1) ^ 1)))) {
+            if (dirty) ++cleaned;
+            tc_fence_after();
+            const uint32_t sv = smem_u32(sKV + st * C::kTile);
+#pragma unroll
+            for (int s = 0; s < FN / 16; ++s) {
+              const uint64_t bv = umma_desc_sw128_mn(sv + s * 16 * 128, C::kChunk, 1024u);
+              umma_f16_ts(tO, tP + pb * (FN / 2) + s * 8, bv, idesc_pv, (!first || s > 0) ? 1u : 0u);
+            }
+            umma_commit(&p_free[pb]);
+            umma_commit(&empty[st]);
+            if (last) umma_commit(o_full);
+            ++np;
+            if (++jb == b.j1) {
+              ok = take(++ub, b, true);
+              jb = b.j0;
+            }
+            moved = true;
+          }
+        }
+        if (moved) {
+          spins = 0;
+        } else if ((++spins & 255u) == 0) {
+          // The limit of every wait in this file.
+          const unsigned long long now = globaltimer();
+          if (spins == 256u) since = now;
+          if (now - since > kWaitTimeoutNs) {
+            if (p.err) atomicCAS(p.err, (unsigned)kErrNone, (unsigned)kErrMbarTimeout);
             ok = false;
-            break;
           }
-          tc_fence_after();
-          const uint32_t sk = smem_u32(sKV + st * C::kTile);
-#pragma unroll
-          for (int kb = 0; kb < kDC; ++kb) {
-            const uint64_t bk = umma_desc_sw128(sk + kb * C::kChunk);
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              umma_f16_ts(tS + sb * FN, tQ + (kb * 4 + k) * 8, bk + (uint64_t)(2 * k), idesc_s,
-                          (kb > 0 || k > 0) ? 1u : 0u);
-          }
-          umma_commit(&s_full[sb]);
-          umma_commit(&empty[st]);
-          const bool dirty = x.template dirty<FN>(j);
-          // (At most two are out at a time: V_n comes back before S of tile
-          // n + 2. That tile n is at work also means that V_n's slot is in its
-          // present round, which is what the cleaner's wait for it relies on.)
-          if (dirty) mbar_arrive(&v_dirty[sent++ & 1]);
-          if (j > x.j0) ok = pv(n - 1, first_b, false, dirty_b);
-          first_b = j == x.j0;
-          dirty_b = dirty;
+          if (p.err && *(volatile unsigned int*)p.err != kErrNone) ok = false;
         }
       }
-      if (ok && n == N) pv(N - 1, first_b, true, dirty_b);
       // Every MMA done before the TMEM goes.
       umma_commit(done);
       mbar_wait(done, 0, p.err);
     }
     __syncwarp();
   } else if (warp == 11) {
-    // --------------------------------------------------------------- cleaner
-    Unit x;
+    // ------------------------------------------------- Q loader, V cleaner
     int n = 0, got = 0;
-    bool ok = true;
-    for (int u = 0; ok && take(u, x, false) && x.j0 < x.j1; ++u) {
+    // Q rows of unit u into its buffer: eight lanes a 128-byte piece of a row,
+    // four rows at a time. Spare rows of a softmax warp that has valid ones
+    // are zero, so that their scores are numbers.
+    auto load_q = [&](int u, const Unit& x) -> bool {
+      const int qb = u % NQ;
+      const bool free = mbar_wait(&q_empty[qb], (uint32_t)(((u / NQ) & 1) ^ 1), p.err);
+      if (!__all_sync(0xffffffffu, free)) return false;
+      const int rows = min(FM, x.rows), fill = (rows + 31) / 32 * 32, sub = lane & 7;
+      const uint32_t dst = smem_u32(sQ + qb * C::kQBytes);
+      int r = lane >> 3;
+      int t = (x.row0 + r) / p.G, hd = x.row0 + r - t * p.G;
+      for (; r < fill; r += 4) {
+        const bool valid = r < rows;
+        const __nv_bfloat16* src =
+            valid ? p.q + (long long)(x.q0 + t) * p.q_stride + (long long)(x.kvh * p.G + hd) * D + sub * 8
+                  : p.q;
+#pragma unroll
+        for (int c = 0; c < kDC; ++c)
+          cp_async_16(dst + c * C::kQChunk + sw_off(r, sub), src + (valid ? c * 64 : 0), valid);
+        for (hd += 4; hd >= p.G; hd -= p.G) ++t;
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      fence_proxy_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full[qb]);
+      return true;
+    };
+    Unit x, next;
+    bool ok = take(0, x, false);
+    if (ok && x.j0 < x.j1) ok = load_q(0, x);
+    for (int u = 0; ok && x.j0 < x.j1; ++u) {
+      ok = take(u + 1, next, false);
+      const bool more = next.j0 < next.j1;
+      if (ok && more && NQ > 1) ok = load_q(u + 1, next);
       for (int j = x.j0; j < x.j1 && ok; ++j, ++n) {
         if (!x.template dirty<FN>(j)) continue;
         const int pos = pos_v(n);
         ok = __all_sync(0xffffffffu,
-                        mbar_wait(&v_dirty[got & 1], (uint32_t)((got >> 1) & 1), p.err) &&
+                        mbar_wait(&v_dirty[got & 3], (uint32_t)((got >> 2) & 1), p.err) &&
                             mbar_wait(&full[pos % NS], (uint32_t)((pos / NS) & 1), p.err));
         if (!ok) break;
         uint8_t* sv = sKV + (pos % NS) * C::kTile;
@@ -543,24 +607,25 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
         zero(max(0, x.seq_len - kbase), FN);
         fence_proxy_async_shared();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&v_clean[got & 1]);
+        if (lane == 0) mbar_arrive(&v_clean[got & 3]);
         ++got;
       }
+      if (ok && more && NQ == 1) ok = load_q(u + 1, next);
+      x = next;
     }
   } else {
     // --------------------------------------------------------------- softmax
-    const int q4 = warp & 3;          // the 32 TMEM lanes this warp may touch
-    const int half = (warp - 2) / 4;  // which half of the tile's keys
+    const int q4 = warp & 3;         // the 32 TMEM lanes this warp may touch
+    const int grp = (warp - 2) / 4;  // tiles n with n % 2 == grp
     const int row = q4 * 32 + lane;
-    constexpr int HN = FN / 2;        // keys of a half
-    constexpr int HD = D / 2;         // O columns of a half
+    constexpr int HD = D / 2;        // O columns of a group in the epilogue
     const uint32_t lane_base = (uint32_t)(q4 * 32) << 16;
     const float sc = p.scale_log2;
     const uint64_t sc2 = f32x2_pack(sc, sc);
     bool ok = true;
     int n = 0, meets = 0;
-    // Both warps of these 32 rows meet (a wait with a limit, like the others:
-    // either may have given up).
+    // The two warps of these 32 rows meet (a wait with a limit, like the
+    // others: either may have given up).
     auto meet = [&]() -> bool {
       __syncwarp();
       if (lane == 0) mbar_arrive(&pair[q4]);
@@ -568,41 +633,32 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
       ++meets;
       return __all_sync(0xffffffffu, r);
     };
-    // This thread's half of a unit's Q row: to registers, then to TMEM (zero
-    // for spare rows, so that their scores are numbers).
-    uint4 qr[HD / 8];
-    auto load_q = [&](const Unit& x) {
-      const bool on = row < x.rows;
-      const int g = x.row0 + (on ? row : 0), t = g / p.G;
-      const __nv_bfloat16* src = p.q + (long long)(x.q0 + t) * p.q_stride +
-                                 (long long)(x.kvh * p.G + g - t * p.G) * D + half * HD;
-#pragma unroll
-      for (int i = 0; i < HD / 8; ++i) qr[i] = on ? ld_q(src + i * 8) : make_uint4(0, 0, 0, 0);
+    // The reference after tile i, as the warp of these rows in tile i's group
+    // left it.
+    auto ref_after = [&](int i, float& m) -> bool {
+      const bool r = mbar_wait(&post[(i & 1) * 4 + q4], (uint32_t)((i >> 1) & 1), p.err);
+      m = sh_ref[row];
+      return __all_sync(0xffffffffu, r);
     };
-    auto store_q = [&] {
-      const uint32_t dst = tQ + lane_base + half * (HD / 2);
-      if constexpr (HD == 32) {
-        tmem_st_32x32b_x16(dst, *reinterpret_cast<uint32_t(*)[16]>(qr));
-      } else {
-#pragma unroll
-        for (int c = 0; c < HD / 64; ++c)
-          tmem_st_32x32b_x32(dst + c * 32, *reinterpret_cast<uint32_t(*)[32]>(qr + 8 * c));
-      }
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(q_full);
-    };
+    // Exponent reference of O (log2 units), this group's sum against m_own.
+    float m_own = -INFINITY, l = 0.f;
     // A finished unit's row, until its O is read.
     struct Done {
-      long long dst;    // element of out, or of part_o for a cut unit
-      long long piece;  // row of part_ml, or -1 for a whole unit
+      long long dst;  // element of out, or of part_o for a cut unit
       float m, l;
+      int piece;      // row of part_ml, or -1 for a whole unit
       int head;
       bool valid, on;
-    } fin{0, -1, 0.f, 0.f, 0, false, false};
+    } fin{0, 0.f, 0.f, -1, 0, false, false};
     int finished = 0;
     auto epilogue = [&]() -> bool {
+      if (fin.on) {
+        // The row's sum: the groups'. (Met twice: the places are used again.)
+        sh_sum[grp * FM + row] = fin.l;
+        if (!meet()) return false;
+        fin.l = sh_sum[row] + sh_sum[FM + row];
+        if (!meet()) return false;
+      }
       if (!__all_sync(0xffffffffu, mbar_wait(o_full, (uint32_t)(finished & 1), p.err)))
         return false;
       ++finished;
@@ -617,19 +673,19 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
                       ? 1.f
                       : den + exp2f(p.sinks[fin.head] * 1.4426950408889634f - fin.m);
           f = den > 0.f ? 1.f / den : 0.f;
-        } else if (fin.valid && half == 0) {
+        } else if (fin.valid && grp == 0) {
           p.part_ml[fin.piece] = make_float2(fin.m, fin.l);
         }
 #pragma unroll 1
-        for (int c = 0; c < HD / 32; ++c) {
-          uint32_t o[32];
-          tmem_ld_32x32b_x32(tO + lane_base + half * HD + c * 32, o);  // warp-collective
+        for (int c = 0; c < HD / 16; ++c) {
+          uint32_t o[16];
+          tmem_ld_32x32b_x16(tO + lane_base + grp * HD + c * 16, o);  // warp-collective
           tmem_wait_ld();
           if (!fin.valid) continue;
           if (whole) {
-            __nv_bfloat16* dst = p.out + fin.dst + c * 32;
+            __nv_bfloat16* dst = p.out + fin.dst + c * 16;
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
+            for (int v = 0; v < 2; ++v) {
               uint32_t w[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e)
@@ -638,9 +694,9 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
               *reinterpret_cast<uint4*>(dst + v * 8) = make_uint4(w[0], w[1], w[2], w[3]);
             }
           } else {
-            float* dst = p.part_o + fin.dst + c * 32;
+            float* dst = p.part_o + fin.dst + c * 16;
 #pragma unroll
-            for (int v = 0; v < 8; ++v)
+            for (int v = 0; v < 4; ++v)
               *reinterpret_cast<uint4*>(dst + v * 4) =
                   make_uint4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
           }
@@ -651,15 +707,16 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
       if (lane == 0) mbar_arrive(o_free);
       return true;
     };
+    // This group's sum against the unit's last reference.
+    auto close = [&](float m) {
+      fin.m = m;
+      fin.l = m_own == -INFINITY ? 0.f : l * exp2f(m_own - m);
+    };
 
-    Unit x, next;
-    ok = take(0, next, false);
-    if (ok && next.j0 < next.j1) {
-      load_q(next);
-      store_q();
-    }
-    for (int u = 0; ok && next.j0 < next.j1; ++u) {
-      x = next;
+    Unit x;
+    for (int u = 0; ok; ++u) {
+      ok = take(u, x, false);
+      if (!ok || x.j0 >= x.j1) break;
       const bool valid = row < x.rows;
       const bool warp_on = q4 * 32 < x.rows;
       const int g = x.row0 + (valid ? row : 0), node = g / p.G;
@@ -675,134 +732,184 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
         for (int i = 0; 32 * i < x.nodes; ++i) depth += __popc(mask.word(i));
         key_lo = x.prefix + max(depth - 1, 0) - p.window + 1;
       }
-      // Exponent reference (log2 units; the same in both halves), this half's sum.
-      float m_used = -INFINITY, l = 0.f;
       for (int j = x.j0; j < x.j1; ++j, ++n) {
-        const int sb = n & 1;
-        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[sb], (uint32_t)((n >> 1) & 1), p.err));
-        if (!ok) break;
-        tc_fence_after();
-        // The unit's last S is there: Q may be replaced.
-        bool stage_q = false;
-        if (j == x.j1 - 1) {
-          ok = take(u + 1, next, false);
+        if ((n & 1) == grp) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&s_full[grp], (uint32_t)((n >> 1) & 1), p.err));
           if (!ok) break;
-          stage_q = next.j0 < next.j1;
-          if (stage_q) load_q(next);
-        }
-        if (warp_on) {
-          // The half row of scores, masked, and its maximum.
-          uint32_t r[HN / 32][32];
-#pragma unroll
-          for (int w = 0; w < HN / 32; ++w)
-            tmem_ld_32x32b_x32(tS + lane_base + sb * FN + half * HN + w * 32, r[w]);
-          tmem_wait_ld();
-          const int kb = x.k_lo + j * FN + half * HN;
-          if (__any_sync(0xffffffffu, key_lo > kb) || kb + HN > x.prefix) {
-#pragma unroll
-            for (int w = 0; w < HN / 32; ++w) {
+          tc_fence_after();
+          const uint32_t s_row = tS + lane_base + grp * FN, p_row = tP + lane_base + grp * (FN / 2);
+          const int kb = x.k_lo + j * FN;
+          if (warp_on && (__any_sync(0xffffffffu, key_lo > kb) || kb + FN > x.prefix)) {
+            // Hidden scores become -inf in TMEM, by a loop of its own: the code
+            // that every tile runs stays short.
+#pragma unroll 1
+            for (int w = 0; w < FN / 32; ++w) {
               const int k0 = kb + 32 * w;
               const uint32_t vis =
                   valid ? range_bits(key_lo - k0, x.prefix - k0) | mask.bits(k0 - x.prefix) : 0u;
+              if (__all_sync(0xffffffffu, vis == 0xffffffffu)) continue;
+              uint32_t t[32];
+              tmem_ld_32x32b_x32(s_row + w * 32, t);
+              tmem_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (!((vis >> i) & 1u)) r[w][i] = 0xff800000u;
+              for (int i = 0; i < 32; ++i) {
+                const uint32_t keep = (uint32_t)((int)(vis << (31 - i)) >> 31);
+                t[i] = (t[i] & keep) | (0xff800000u & ~keep);
+              }
+              tmem_st_32x32b_x32(s_row + w * 32, t);
             }
+            tmem_wait_st();
           }
-          float mxs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          // One pass over the row's scores, 32 at a time (short loops: an SM's
+          // instruction cache misses cost more than what unrolling gains).
+          // WRITE: P = 2^(S scale - mu) as bf16 pairs, their sum to *rs.
+          // Returns the row's maximum in log2 units.
+          auto sweep = [&](auto write_c, float mu, float* rs) -> float {
+            constexpr bool kWrite = decltype(write_c)::value;
+            float mxa = -INFINITY, mxb = -INFINITY;
+            const float mu_eff = mu == -INFINITY ? 0.f : mu;
+            const uint64_t nmu2 = f32x2_pack(-mu_eff, -mu_eff);
+            uint64_t acc[2] = {f32x2_pack(0.f, 0.f), f32x2_pack(0.f, 0.f)};
+#pragma unroll 1
+            for (int c = 0; c < FN / 32; ++c) {
+              uint32_t r[32], w[16];
+              tmem_ld_32x32b_x32(s_row + c * 32, r);
+              tmem_wait_ld();
 #pragma unroll
-          for (int w = 0; w < HN / 32; ++w)
-#pragma unroll
-            for (int i = 0; i < 32; ++i) mxs[i & 3] = fmaxf(mxs[i & 3], __uint_as_float(r[w][i]));
-          const float own = fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3]));
-          sh_max[sb][half][row] = own;
-          ok = meet();
-          if (!ok) break;
-          float mx = fmaxf(own, sh_max[sb][half ^ 1][row]);
-          mx = mx == -INFINITY ? mx : mx * sc;
-          const bool resc = mx > m_used + 8.f || (m_used == -INFINITY && mx != -INFINITY);
-          if (__any_sync(0xffffffffu, resc)) {
-            const float alpha = !resc ? 1.f : m_used == -INFINITY ? 0.f : exp2f(m_used - mx);
-            if (resc) {
-              l *= alpha;
-              m_used = mx;
+              for (int i = 0; i < 16; ++i) {
+                const float va = __uint_as_float(r[2 * i]), vb = __uint_as_float(r[2 * i + 1]);
+                mxa = fmaxf(mxa, va);
+                mxb = fmaxf(mxb, vb);
+                if constexpr (kWrite) {
+                  float ea, eb;
+                  f32x2_unpack(f32x2_fma(f32x2_pack(va, vb), sc2, nmu2), ea, eb);
+                  ea = fast_exp2(ea);
+                  eb = fast_exp2(eb);
+                  acc[i & 1] = f32x2_add(acc[i & 1], f32x2_pack(ea, eb));
+                  w[i] = pack_bf16x2(ea, eb);
+                }
+              }
+              if constexpr (kWrite) tmem_st_32x32b_x16(p_row + c * 16, w);
             }
-            if (j > x.j0) {
-              // O is final for the tiles before once P V of tile n - 1 is done.
-              ok = __all_sync(0xffffffffu, mbar_wait(pv_done, (uint32_t)((n - 1) & 1), p.err));
+            if constexpr (kWrite) {
+              float a0, a1;
+              f32x2_unpack(f32x2_add(acc[0], acc[1]), a0, a1);
+              *rs = a0 + a1;
+            }
+            const float mx = fmaxf(mxa, mxb);
+            return mx == -INFINITY ? mx : mx * sc;
+          };
+          using T_ = std::true_type;
+          using F_ = std::false_type;
+          auto hand_on = [&](float m) {  // the reference, to the tile after
+            sh_ref[row] = m;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&post[grp * 4 + q4]);
+          };
+          // The reference to try: O's, as far as it is known. A group's first
+          // tile of a unit waits for it (it follows the unit's first tile's
+          // maximum at once); later ones take their own last and look at the
+          // other group's after the pass, when that has long been handed on.
+          float m_prev = -INFINITY;
+          if (n > 0 && j <= x.j0 + 1) {
+            ok = ref_after(n - 1, m_prev);
+            if (!ok) break;
+          }
+          if (j == x.j0) {
+            if (u > 0) close(m_prev);  // of the unit before
+            m_prev = m_own = -INFINITY;
+            l = 0.f;
+          }
+          float m = j <= x.j0 + 1 ? m_prev : m_own;
+          if (warp_on && __any_sync(0xffffffffu, m == -INFINITY)) {
+            const float mx = sweep(F_{}, 0.f, nullptr);
+            if (m == -INFINITY) m = mx;
+          }
+          if (j == x.j0) hand_on(m);
+          // This P buffer is free once P V of tile n - 2 has completed (a warp
+          // without rows waits too, or it would be a tile ahead).
+          if (n >= 2) ok = mbar_wait(&p_free[grp], (uint32_t)(((n - 2) >> 1) & 1), p.err);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          float rs = 0.f, mx = -INFINITY;
+          if (warp_on) mx = sweep(T_{}, m, &rs);
+          if (j > x.j0) {
+            if (j > x.j0 + 1) {
+              ok = ref_after(n - 1, m_prev);
+              if (!ok) break;
+            }
+            const bool resc = mx > m_prev + 8.f || (m_prev == -INFINITY && mx != -INFINITY);
+            const float m_new = resc ? mx : m_prev;
+            hand_on(m_new);
+            if (__any_sync(0xffffffffu, resc)) {
+              // O is final for the tiles before once P V of tile n - 1 is done
+              // (its barrier's round before first: the parity tells two apart).
+              ok = __all_sync(
+                  0xffffffffu,
+                  (n < 3 || mbar_wait(&p_free[grp ^ 1], (uint32_t)(((n - 3) >> 1) & 1), p.err)) &&
+                      mbar_wait(&p_free[grp ^ 1], (uint32_t)(((n - 1) >> 1) & 1), p.err));
               if (!ok) break;
               tc_fence_after();
+              const float alpha = !resc ? 1.f : m_prev == -INFINITY ? 0.f : exp2f(m_prev - m_new);
 #pragma unroll 1
-              for (int c = 0; c < HD / 32; ++c) {
-                uint32_t o[32];
-                tmem_ld_32x32b_x32(tO + lane_base + half * HD + c * 32, o);
+              for (int c = 0; c < D / 16; ++c) {
+                uint32_t o[16];
+                tmem_ld_32x32b_x16(tO + lane_base + c * 16, o);
                 tmem_wait_ld();
 #pragma unroll
-                for (int e = 0; e < 32; ++e)
+                for (int e = 0; e < 16; ++e)
                   o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-                tmem_st_32x32b_x32(tO + lane_base + half * HD + c * 32, o);
+                tmem_st_32x32b_x16(tO + lane_base + c * 16, o);
               }
             }
+            if (__any_sync(0xffffffffu, m != m_new)) {
+              m = m_new;
+              tmem_wait_st();
+              sweep(T_{}, m, &rs);  // P once more, against the reference of O
+            }
           }
-          const float mu = m_used == -INFINITY ? 0.f : m_used;
-          const uint64_t nmu2 = f32x2_pack(-mu, -mu);
-          uint64_t acc[2] = {f32x2_pack(0.f, 0.f), f32x2_pack(0.f, 0.f)};
-          uint32_t w[HN / 2];
-#pragma unroll
-          for (int i = 0; i < HN / 2; ++i) {
-            float ea, eb;
-            f32x2_unpack(f32x2_fma(f32x2_pack(__uint_as_float(r[i >> 4][(2 * i) & 31]),
-                                              __uint_as_float(r[i >> 4][(2 * i + 1) & 31])),
-                                   sc2, nmu2),
-                         ea, eb);
-            ea = fast_exp2(ea);
-            eb = fast_exp2(eb);
-            acc[i & 1] = f32x2_add(acc[i & 1], f32x2_pack(ea, eb));
-            w[i] = pack_bf16x2(ea, eb);
+          if (m != m_own) {
+            l = m_own == -INFINITY ? 0.f : l * exp2f(m_own - m);
+            m_own = m;
           }
-          float a0, a1;
-          f32x2_unpack(f32x2_add(acc[0], acc[1]), a0, a1);
-          l += a0 + a1;
-          // P goes over the first half of its S buffer: both warps have read
-          // their scores (they met).
-          const uint32_t p_row = tS + lane_base + sb * FN + half * (HN / 2);
-          if constexpr (HN == 64)
-            tmem_st_32x32b_x32(p_row, *reinterpret_cast<uint32_t(*)[32]>(w));
-          else
-            tmem_st_32x32b_x16(p_row, *reinterpret_cast<uint32_t(*)[16]>(w));
+          l += rs;
           tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&p_full[grp]);
+            mbar_arrive(&s_free[grp]);
+          }
+        } else if (j == x.j0) {
+          // The other group's tile: this one did the last of the unit before.
+          if (u > 0) close(m_own);
+          m_own = -INFINITY;
+          l = 0.f;
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[sb]);
-        if (stage_q) store_q();
         if (j == x.j0 && u > 0) {
           ok = epilogue();  // of the unit before
           if (!ok) break;
         }
+        if (j == x.j0) {
+          fin.head = head;
+          fin.valid = valid;
+          fin.on = warp_on;
+          // A cut unit leaves pieces: 0 for one that began before this share.
+          const int piece = ((int)blockIdx.x * 2 + (x.j0 > 0 ? 0 : 1)) * FM + row;
+          fin.piece = x.whole ? -1 : piece;
+          fin.dst = (x.whole ? (long long)(x.q0 + node) * p.o_stride + (long long)head * D
+                             : (long long)piece * D) + grp * HD;
+        }
       }
-      if (!ok) break;
-      if (warp_on) {
-        // The row's sum: the halves' (in the buffer of the next unit's first
-        // tile, hence the second meeting).
-        sh_max[n & 1][half][row] = l;
-        ok = meet();
-        if (!ok) break;
-        l = sh_max[n & 1][0][row] + sh_max[n & 1][1][row];
-        ok = meet();
-        if (!ok) break;
-      }
-      fin.m = m_used;
-      fin.l = l;
-      fin.head = head;
-      fin.valid = valid;
-      fin.on = warp_on;
-      // A cut unit leaves pieces: 0 for one that began before this share.
-      fin.piece = x.whole ? -1 : ((long long)blockIdx.x * 2 + (x.j0 > 0 ? 0 : 1)) * FM + row;
-      fin.dst = (x.whole ? (long long)(x.q0 + node) * p.o_stride + (long long)head * D
-                         : fin.piece * D) + half * HD;
     }
-    if (ok && n > 0) epilogue();
+    if (ok && n > 0) {
+      float m = m_own;
+      if (((n - 1) & 1) != grp) ok = ref_after(n - 1, m);
+      if (ok) {
+        close(m);
+        epilogue();
+      }
+    }
   }
   tc_fence_before();
   __syncthreads();
