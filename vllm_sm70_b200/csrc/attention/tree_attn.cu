@@ -22,16 +22,14 @@
 // kernel joins in share order; whole units are written directly. The split
 // depends on the lengths only, so results repeat bit for bit.
 //
-// Twelve warps a CTA:
-//   warp 0     K producer, warp 10 V producer: one (cache block, 64-column)
+// Thirteen warps a CTA:
+//   warp 0     K producer, warp 1 V producer: one (cache block, 64-column)
 //              box a lane, one warp-wide bulk-tensor instruction a tile (that
-//              costs its warp ~80 cycles a box, hence two warps), into one
-//              ring in the order of use K0 K1 V0 K2 V1 ... Warp 0 also walks
+//              costs its warp ~80 cycles a box, hence two warps), each into a
+//              ring of its own: one producer and one consumer, so that a
+//              barrier's parity always tells its rounds apart. Warp 0 also walks
 //              the share and publishes each unit's numbers, one unit ahead, so
 //              that nobody else waits for lengths or divides.
-//   warp 1     TMEM owner and MMA issuer: S = Q K^T into one of two S buffers
-//              and O += P V, each in tile order, whichever is ready first (S
-//              at most two tiles ahead)
 //   warps 2-9  softmax: two groups of four warps, a row a thread, on every
 //              other tile, so that one's waits are the other's work. O has one
 //              exponent reference a row (base 2, raised lazily: O is rescaled
@@ -40,7 +38,11 @@
 //              as soon as a tile's maximum is known. A unit's epilogue (half
 //              of O's columns each) comes after the next unit's first tile,
 //              when the last P V has long finished.
-//   warp 11    loads Q rows (the next unit's while the present one runs) and
+//   warp 10    issues S = Q K^T into one of two S buffers, as soon as softmax
+//              has finished with the tile before in it
+//   warp 11    issues O += P V (its own warp: an issuing thread spends longer
+//              on waits and descriptors than the tensor core on a product)
+//   warp 12    loads Q rows (the next unit's while the present one runs) and
 //              zeroes V rows that no node sees (past the end, before the
 //              window): they may hold anything, and 0 x NaN is not 0.
 // TMEM columns: S0 | S1 | O | P0 | P1.
@@ -67,7 +69,7 @@ namespace b200 {
 namespace {
 
 constexpr int FM = 128;
-constexpr int kThreads = 384;
+constexpr int kThreads = 416;
 constexpr int kSoftmaxWarps = 8;
 constexpr int kBarBytes = 1024;  // barriers and published units
 constexpr int kUnits = 4;       // published units
@@ -84,8 +86,9 @@ struct Cfg {
   static constexpr int NQ = D <= 128 ? 2 : 1;     // Q buffers
   static constexpr int kChunk = FN * 128;
   static constexpr int kTile = kDC * kChunk;      // K or V of a tile
-  static constexpr int NS = D == 64 ? 12 : 5;     // ring slots
-  static constexpr int kSmem = NQ * kQBytes + NS * kTile + kBarBytes + kRowBytes;
+  static constexpr int NK = D == 64 ? 6 : 2;      // K ring slots
+  static constexpr int NV = D == 64 ? 6 : 3;      // V: held until P is there, two tiles on
+  static constexpr int kSmem = NQ * kQBytes + (NK + NV) * kTile + kBarBytes + kRowBytes;
   static_assert(3 * FN + D <= 512, "TMEM columns");
   static_assert(kSmem <= 232448, "shared memory");
 };
@@ -121,18 +124,6 @@ __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool 
   const int sz = valid ? 16 : 0;
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(sz)
                : "memory");
-}
-// Whether the phase of the given parity has completed (never waits).
-__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred P;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 P, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, P;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
 }
 // (volatile: issued where it stands, ahead of the tile's work)
 __device__ __forceinline__ uint32_t ld_word(const uint32_t* p) {
@@ -238,19 +229,22 @@ __global__ void __launch_bounds__(kThreads, 1)
 tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
                  const Params p) {
   using C = Cfg<D_>;
-  constexpr int D = C::D, FN = C::FN, kDC = C::kDC, NS = C::NS, NQ = C::NQ;
+  constexpr int D = C::D, FN = C::FN, kDC = C::kDC, NK = C::NK, NV = C::NV, NQ = C::NQ;
   // The 128-byte swizzle wants 1024-byte aligned tiles: all shared memory is
   // dynamic, and there is no room for a margin.
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* sQ = smem;
-  uint8_t* sKV = sQ + NQ * C::kQBytes;
-  uint64_t* full = reinterpret_cast<uint64_t*>(sKV + NS * C::kTile);  // [NS]
-  uint64_t* empty = full + NS;                                        // [NS]
-  uint64_t* q_full = empty + NS;                                      // [2]
+  uint8_t* sK = sQ + NQ * C::kQBytes;
+  uint8_t* sV = sK + NK * C::kTile;
+  uint8_t* sEnd = sV + NV * C::kTile;
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(sEnd);               // [NK]
+  uint64_t* k_empty = k_full + NK;                                    // [NK]
+  uint64_t* v_full = k_empty + NK;                                    // [NV]
+  uint64_t* v_empty = v_full + NV;                                    // [NV]
+  uint64_t* q_full = v_empty + NV;                                    // [2]
   uint64_t* q_empty = q_full + 2;                                     // [2]
   uint64_t* s_full = q_empty + 2;                                     // [2]
-  uint64_t* s_free = s_full + 2;                                      // [2]
-  uint64_t* p_full = s_free + 2;                                      // [2]
+  uint64_t* p_full = s_full + 2;                                      // [2]
   uint64_t* p_free = p_full + 2;                                      // [2]
   uint64_t* post = p_free + 2;                                        // [2][4]
   uint64_t* pair = post + 8;                                          // [4]
@@ -259,53 +253,56 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
   uint64_t* done = o_free + 1;
   uint64_t* u_full = done + 1;                                        // [kUnits]
   uint64_t* u_empty = u_full + kUnits;                                // [kUnits]
-  uint64_t* v_dirty = u_empty + kUnits;                               // [4]
-  uint64_t* v_clean = v_dirty + 4;                                    // [4]
-  int* share_of = reinterpret_cast<int*>(v_clean + 4);  // sequence, offset, tiles
+  uint64_t* v_dirty = u_empty + kUnits;
+  uint64_t* v_clean = v_dirty + 1;
+  int* share_of = reinterpret_cast<int*>(v_clean + 1);  // sequence, offset, tiles
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(share_of + 3);
-  static_assert((2 * NS + 12 + 12 + 3 + 2 * kUnits + 8) * 8 + 16 +
+  static_assert((2 * (NK + NV) + 10 + 12 + 3 + 2 * kUnits + 2) * 8 + 16 +
                     kUnits * (int)sizeof(Unit) <= kBarBytes, "barriers and units");
-  Unit* units_sh = reinterpret_cast<Unit*>(sKV + NS * C::kTile + kBarBytes) - kUnits;
-  float* sh_ref = reinterpret_cast<float*>(sKV + NS * C::kTile + kBarBytes);  // [FM]
+  Unit* units_sh = reinterpret_cast<Unit*>(sEnd + kBarBytes) - kUnits;
+  float* sh_ref = reinterpret_cast<float*>(sEnd + kBarBytes);  // [FM]
   float* sh_sum = sh_ref + FM;                                                // [2][FM]
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   pdl_wait();
   if (threadIdx.x == 0) {
-    for (int i = 0; i < NS; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
+    for (int i = 0; i < NK; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+    }
+    for (int i = 0; i < NV; ++i) {
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 1);
       mbar_init(&s_full[i], 1);
-      mbar_init(&s_free[i], 4);
       mbar_init(&p_full[i], 4);
       mbar_init(&p_free[i], 1);
     }
     for (int i = 0; i < 8; ++i) mbar_init(&post[i], 1);
     for (int i = 0; i < 4; ++i) {
       mbar_init(&pair[i], 2);
-      mbar_init(&v_dirty[i], 1);
-      mbar_init(&v_clean[i], 1);
     }
+    mbar_init(v_dirty, 1);
+    mbar_init(v_clean, 1);
     mbar_init(o_full, 1);
     mbar_init(o_free, kSoftmaxWarps);
-    mbar_init(done, 1);
+    mbar_init(done, 2);
     for (int i = 0; i < kUnits; ++i) {
       mbar_init(&u_full[i], 1);
-      mbar_init(&u_empty[i], kSoftmaxWarps + 3);  // and the MMA, V and cleaning warps
+      mbar_init(&u_empty[i], kSoftmaxWarps + 4);  // and warps 1, 10, 11, 12
     }
     fence_barrier_init();
     tma_prefetch_desc(&tmk);
     tma_prefetch_desc(&tmv);
   }
-  if (warp == 1) {
+  if (warp == 11) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
-  if (warp == 10) {
+  if (warp == 12) {
     // The share: a scan over the sequences, 32 at a time, for the total and
     // then for the sequence in which this CTA's first tile lies.
     long long total = 0, first32 = 0;
@@ -362,25 +359,24 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
   const uint32_t tmem_base = *tmem_slot;
   const uint32_t tS = tmem_base, tO = tS + 2 * FN, tP = tO + D;
   const int N = share_of[2];  // key tiles of this CTA
-  // Ring positions.
-  auto pos_k = [&](int n) { return n == 0 ? 0 : 2 * n - 1; };
-  auto pos_v = [&](int n) { return n == N - 1 ? 2 * N - 1 : 2 * n + 2; };
-
   // Unit u for a reader (a warp, or one thread with `alone`).
-  // `keep`: it is read again later.
-  auto take = [&](int u, Unit& x, bool alone, bool keep = false) -> bool {
+  auto take = [&](int u, Unit& x, bool alone) -> bool {
     const int e = u % kUnits;
     const bool ok = mbar_wait(&u_full[e], (uint32_t)((u / kUnits) & 1), p.err);
     x = units_sh[e];
     if (!alone) __syncwarp();
-    if (!keep && (alone || lane == 0)) mbar_arrive(&u_empty[e]);
+    if (alone || lane == 0) mbar_arrive(&u_empty[e]);
     return alone ? ok : __all_sync(0xffffffffu, ok);
   };
 
-  if (warp == 0 || warp == 10) {
-    // ------------------------------------------------ producers (K: 0, V: 10)
-    const bool is_v = warp == 10;
+  if (warp == 0 || warp == 1) {
+    // ------------------------------------------------- producers (K: 0, V: 1)
+    const bool is_v = warp == 1;
     const CUtensorMap* tm = is_v ? &tmv : &tmk;
+    uint64_t* full = is_v ? v_full : k_full;
+    uint64_t* empty = is_v ? v_empty : k_empty;
+    uint8_t* ring = is_v ? sV : sK;
+    const int slots = is_v ? NV : NK;
     const int BS = p.block_size;
     const int nb = BS >= FN ? 1 : FN / BS;
     const int rows_box = BS >= FN ? FN : BS;
@@ -435,114 +431,68 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
     bool ok = fetch(unit);
     Box cur{0, 0};
     if (ok && unit.j0 < unit.j1) cur = box_of(unit, unit.j0);
-    int n = 0;
+    int st = 0;
+    uint32_t round = 0;  // parity of the ring's round
     while (ok && unit.j0 < unit.j1) {
       ok = fetch(next);
-      for (int j = unit.j0; j < unit.j1 && ok; ++j, ++n) {
+      for (int j = unit.j0; j < unit.j1 && ok; ++j) {
         // Ids one tile ahead of their use.
         Box nxt = cur;
         if (j + 1 < unit.j1) nxt = box_of(unit, j + 1);
         else if (next.j0 < next.j1) nxt = box_of(next, next.j0);
-        const int pos = is_v ? pos_v(n) : pos_k(n), st = pos % NS;
         int go = 1;
         if (lane == 0) {
-          go = mbar_wait(&empty[st], (uint32_t)(((pos / NS) & 1) ^ 1), p.err) ? 1 : 0;
+          go = mbar_wait(&empty[st], round ^ 1u, p.err) ? 1 : 0;
           if (go) mbar_arrive_expect_tx(&full[st], (uint32_t)C::kTile);
         }
         ok = __shfl_sync(0xffffffffu, go, 0);
         if (ok && h < kDC)
-          tma_load_3d(sKV + st * C::kTile + h * C::kChunk + bi * rows_box * 128, tm, &full[st],
+          tma_load_3d(ring + st * C::kTile + h * C::kChunk + bi * rows_box * 128, tm, &full[st],
                       h * 64, cur.y, cur.blk);
+        if (++st == slots) {
+          st = 0;
+          round ^= 1u;
+        }
         cur = nxt;
       }
       unit = next;
     }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer
-    if (lane == 0 && N > 0) {
-      constexpr uint32_t idesc_s = umma_idesc_f16(FM, FN, true);
-      constexpr uint32_t idesc_pv = umma_idesc_f16(FM, D, true) | (1u << 16);  // B MN-major
-      // Two cursors over the tiles: the next S and the next P V.
-      Unit a, b;
-      bool ok = take(0, a, true, true) && take(0, b, true);
-      int ns = 0, ja = a.j0, ua = 0, np = 0, jb = b.j0, ub = 0;
-      int sent = 0, cleaned = 0;  // dirty V tiles given to the cleaner / taken back
-      unsigned long long since = 0;
-      uint32_t spins = 0;
-      while (ok && np < N) {
-        bool moved = false;
-        // S of tile ns: its buffer has been read, K is there, and Q.
-        if (ns < N && ns - np < 3) {
-          const int pos = pos_k(ns), st = pos % NS, sb = ns & 1, qb = ua % NQ;
-          if ((ns < 2 || mbar_test(&s_free[sb], (uint32_t)(((ns >> 1) & 1) ^ 1))) &&
-              mbar_test(&full[st], (uint32_t)((pos / NS) & 1)) &&
-              (ja > a.j0 || mbar_test(&q_full[qb], (uint32_t)((ua / NQ) & 1)))) {
-            tc_fence_after();
-            const uint32_t sq = smem_u32(sQ + qb * C::kQBytes);
-            const uint32_t sk = smem_u32(sKV + st * C::kTile);
+  } else if (warp == 10) {
+    // -------------------------------------------------------------- S issuer
+    if (lane == 0) {
+      constexpr uint32_t idesc = umma_idesc_f16(FM, FN, true);
+      const uint64_t dq0 = umma_desc_sw128(smem_u32(sQ)), dk0 = umma_desc_sw128(smem_u32(sK));
+      Unit x;
+      bool ok = true;
+      int n = 0, st = 0;
+      uint32_t round = 0;
+      for (int u = 0; ok && take(u, x, true) && x.j0 < x.j1; ++u) {
+        const int qb = u % NQ;
+        ok = mbar_wait(&q_full[qb], (uint32_t)((u / NQ) & 1), p.err);
+        for (int j = x.j0; j < x.j1 && ok; ++j, ++n) {
+          const int sb = n & 1;
+          // K is there, and softmax has finished with tile n - 2.
+          ok = mbar_wait(&k_full[st], round, p.err) &&
+               (n < 2 || mbar_wait(&p_full[sb], (uint32_t)(((n >> 1) & 1) ^ 1), p.err));
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t dq = dq0 + (uint64_t)(qb * (C::kQBytes >> 4));
+          const uint64_t dk = dk0 + (uint64_t)(st * (C::kTile >> 4));
 #pragma unroll
-            for (int kb = 0; kb < kDC; ++kb) {
-              const uint64_t aq = umma_desc_sw128(sq + kb * C::kQChunk);
-              const uint64_t bk = umma_desc_sw128(sk + kb * C::kChunk);
+          for (int kb = 0; kb < kDC; ++kb)
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
-                umma_f16(tS + sb * FN, aq + (uint64_t)(2 * k), bk + (uint64_t)(2 * k), idesc_s,
-                         (kb > 0 || k > 0) ? 1u : 0u);
-            }
-            umma_commit(&s_full[sb]);
-            umma_commit(&empty[st]);
-            // (S runs at most two tiles ahead: three are out at most, and the
-            // barriers hold four. That tile ns is at work also means that its
-            // V slot is in its present round: the cleaner's wait relies on it.)
-            if (a.template dirty<FN>(ja)) mbar_arrive(&v_dirty[sent++ & 3]);
-            ++ns;
-            if (++ja == a.j1) {
-              umma_commit(&q_empty[qb]);
-              ok = take(++ua, a, true, true);
-              ja = a.j0;
-            }
-            moved = true;
+            for (int k = 0; k < 4; ++k)
+              umma_f16(tS + sb * FN, dq + (uint64_t)(kb * (C::kQChunk >> 4) + 2 * k),
+                       dk + (uint64_t)(kb * (C::kChunk >> 4) + 2 * k), idesc,
+                       (kb > 0 || k > 0) ? 1u : 0u);
+          umma_commit(&s_full[sb]);
+          umma_commit(&k_empty[st]);
+          if (++st == NK) {
+            st = 0;
+            round ^= 1u;
           }
         }
-        // P V of tile np: P and V are there, V clean, O free.
-        if (ok && np < ns) {
-          const int pos = pos_v(np), st = pos % NS, pb = np & 1;
-          const bool first = jb == b.j0, last = jb == b.j1 - 1, dirty = b.template dirty<FN>(jb);
-          if (mbar_test(&p_full[pb], (uint32_t)((np >> 1) & 1)) &&
-              mbar_test(&full[st], (uint32_t)((pos / NS) & 1)) &&
-              (!dirty || mbar_test(&v_clean[cleaned & 3], (uint32_t)((cleaned >> 2) & 1))) &&
-              (!first || mbar_test(o_free, (uint32_t)((ub & 1) ^ 1)))) {
-            if (dirty) ++cleaned;
-            tc_fence_after();
-            const uint32_t sv = smem_u32(sKV + st * C::kTile);
-#pragma unroll
-            for (int s = 0; s < FN / 16; ++s) {
-              const uint64_t bv = umma_desc_sw128_mn(sv + s * 16 * 128, C::kChunk, 1024u);
-              umma_f16_ts(tO, tP + pb * (FN / 2) + s * 8, bv, idesc_pv, (!first || s > 0) ? 1u : 0u);
-            }
-            umma_commit(&p_free[pb]);
-            umma_commit(&empty[st]);
-            if (last) umma_commit(o_full);
-            ++np;
-            if (++jb == b.j1) {
-              ok = take(++ub, b, true);
-              jb = b.j0;
-            }
-            moved = true;
-          }
-        }
-        if (moved) {
-          spins = 0;
-        } else if ((++spins & 255u) == 0) {
-          // The limit of every wait in this file.
-          const unsigned long long now = globaltimer();
-          if (spins == 256u) since = now;
-          if (now - since > kWaitTimeoutNs) {
-            if (p.err) atomicCAS(p.err, (unsigned)kErrNone, (unsigned)kErrMbarTimeout);
-            ok = false;
-          }
-          if (p.err && *(volatile unsigned int*)p.err != kErrNone) ok = false;
-        }
+        umma_commit(&q_empty[qb]);
       }
       // Every MMA done before the TMEM goes.
       umma_commit(done);
@@ -550,6 +500,47 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
     }
     __syncwarp();
   } else if (warp == 11) {
+    // ------------------------------------------------------------ P V issuer
+    if (lane == 0) {
+      constexpr uint32_t idesc = umma_idesc_f16(FM, D, true) | (1u << 16);  // B MN-major
+      const uint64_t dv0 = umma_desc_sw128_mn(smem_u32(sV), C::kChunk, 1024u);
+      Unit x;
+      bool ok = true;
+      int n = 0, st = 0, cleaned = 0;  // V tiles given to warp 12 and taken back
+      uint32_t round = 0;
+      for (int u = 0; ok && take(u, x, true) && x.j0 < x.j1; ++u) {
+        for (int j = x.j0; j < x.j1 && ok; ++j, ++n) {
+          const int pb = n & 1;
+          const bool dirty = x.template dirty<FN>(j);
+          // V is there, without rows that no node sees; P is; O has been read
+          // by the epilogue of the unit before.
+          ok = mbar_wait(&v_full[st], round, p.err);
+          if (ok && dirty) mbar_arrive(v_dirty);
+          ok = ok && mbar_wait(&p_full[pb], (uint32_t)((n >> 1) & 1), p.err) &&
+               (!dirty || mbar_wait(v_clean, (uint32_t)(cleaned & 1), p.err)) &&
+               (j > x.j0 || mbar_wait(o_free, (uint32_t)((u & 1) ^ 1), p.err));
+          if (!ok) break;
+          if (dirty) ++cleaned;
+          tc_fence_after();
+          const uint64_t dv = dv0 + (uint64_t)(st * (C::kTile >> 4));
+#pragma unroll
+          for (int s = 0; s < FN / 16; ++s)
+            umma_f16_ts(tO, tP + pb * (FN / 2) + s * 8, dv + (uint64_t)(s * (16 * 128 >> 4)), idesc,
+                        (j > x.j0 || s > 0) ? 1u : 0u);
+          umma_commit(&p_free[pb]);
+          umma_commit(&v_empty[st]);
+          if (++st == NV) {
+            st = 0;
+            round ^= 1u;
+          }
+        }
+        umma_commit(o_full);
+      }
+      umma_commit(done);
+      mbar_wait(done, 0, p.err);
+    }
+    __syncwarp();
+  } else if (warp == 12) {
     // ------------------------------------------------- Q loader, V cleaner
     int n = 0, got = 0;
     // Q rows of unit u into its buffer: eight lanes a 128-byte piece of a row,
@@ -588,12 +579,10 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
       if (ok && more && NQ > 1) ok = load_q(u + 1, next);
       for (int j = x.j0; j < x.j1 && ok; ++j, ++n) {
         if (!x.template dirty<FN>(j)) continue;
-        const int pos = pos_v(n);
-        ok = __all_sync(0xffffffffu,
-                        mbar_wait(&v_dirty[got & 3], (uint32_t)((got >> 2) & 1), p.err) &&
-                            mbar_wait(&full[pos % NS], (uint32_t)((pos / NS) & 1), p.err));
+        // (Its V has landed: warp 11 has waited for it.)
+        ok = __all_sync(0xffffffffu, mbar_wait(v_dirty, (uint32_t)(got & 1), p.err));
         if (!ok) break;
-        uint8_t* sv = sKV + (pos % NS) * C::kTile;
+        uint8_t* sv = sV + (n % NV) * C::kTile;
         const int kbase = x.k_lo + j * FN;
         constexpr int kU = D / 8;
         auto zero = [&](int from, int to) {  // rows [from, to)
@@ -607,7 +596,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
         zero(max(0, x.seq_len - kbase), FN);
         fence_proxy_async_shared();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&v_clean[got & 3]);
+        if (lane == 0) mbar_arrive(v_clean);
         ++got;
       }
       if (ok && more && NQ == 1) ok = load_q(u + 1, next);
@@ -876,10 +865,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(&p_full[grp]);
-            mbar_arrive(&s_free[grp]);
-          }
+          if (lane == 0) mbar_arrive(&p_full[grp]);
         } else if (j == x.j0) {
           // The other group's tile: this one did the last of the unit before.
           if (u > 0) close(m_own);
@@ -913,7 +899,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) {
+  if (warp == 11) {
     tc_fence_after();
     tmem_dealloc(tmem_base, 512);
   }
