@@ -76,6 +76,16 @@ def test_window_and_sinks(b200_ops, heads, window):
     _check(*a, sinks=torch.full((heads[0],), -1e30, device="cuda"))
 
 
+@pytest.mark.parametrize("heads", [(16, 2, 128), (16, 2, 256)])
+def test_window_starts_row_by_row(b200_ops, heads):
+    """Long windowed contexts, several units a share: a window starts inside a
+    tile, at another key for each depth, so that the exponent reference of
+    some rows rises in a unit's second tile."""
+    lens = [8000 - 217 * i for i in range(16)]
+    nodes = [24 - i for i in range(16)]
+    _check(*_setup(lens, nodes, heads, 32), window=4096)
+
+
 def test_window_hides_stale_blocks(b200_ops):
     """Cache entries before every node's window may have been given away: what
     they hold (NaN here) does not reach the output."""

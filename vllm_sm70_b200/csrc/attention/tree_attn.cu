@@ -93,9 +93,12 @@ struct Cfg {
   static_assert(kSmem <= 232448, "shared memory");
 };
 
-// The unit in which a CTA's share begins (tree_join_kernel).
-struct Cut {
-  int seq, unit, j0, pad;
+// The cut at the start of a CTA's share, for tree_join_kernel: the unit that
+// began in the share before and goes on in this one (rows 0: none), with its
+// pieces up to the one of CTA `last`.
+struct __align__(16) Cut {
+  int q0, kvh, row0, rows;
+  int last, pad[3];
 };
 
 struct Params {
@@ -109,7 +112,6 @@ struct Params {
   float* part_o;        // [grid][2][FM][D]
   float2* part_ml;      // [grid][2][FM]
   Cut* cut;             // [grid]
-  long long* share;     // key tiles of a CTA
   int num_seqs, Hq, Hkv, G, block_size, block_shift, max_blocks, num_blocks;
   int mask_words, window;
   long long T, q_stride, o_stride;
@@ -124,6 +126,11 @@ __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool 
   const int sz = valid ? 16 : 0;
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(sz)
                : "memory");
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 // (volatile: issued where it stands, ahead of the tile's work)
 __device__ __forceinline__ uint32_t ld_word(const uint32_t* p) {
@@ -153,6 +160,22 @@ __device__ __forceinline__ Seq load_seq(const Params& p, int s) {
   return r;
 }
 
+// Lane l's sequence, to the whole warp.
+__device__ __forceinline__ Seq share_seq(const Seq& q, int l) {
+  Seq r;
+  r.q0 = __shfl_sync(0xffffffffu, q.q0, l);
+  r.q_len = __shfl_sync(0xffffffffu, q.q_len, l);
+  r.seq_len = __shfl_sync(0xffffffffu, q.seq_len, l);
+  r.nodes = __shfl_sync(0xffffffffu, q.nodes, l);
+  r.prefix = __shfl_sync(0xffffffffu, q.prefix, l);
+  r.k_first = __shfl_sync(0xffffffffu, q.k_first, l);
+  r.k_lo = __shfl_sync(0xffffffffu, q.k_lo, l);
+  r.n_tiles = __shfl_sync(0xffffffffu, q.n_tiles, l);
+  r.n_rt = __shfl_sync(0xffffffffu, q.n_rt, l);
+  r.total = __shfl_sync(0xffffffffu, q.total, l);
+  return r;
+}
+
 // The units of a CTA's share, in order: unit = key head * n_rt + row tile,
 // key tiles [j0, j1) of it.
 template <int FN>
@@ -160,10 +183,6 @@ struct Walk {
   int s, unit, j0, j1, kvh, row0;
   int off, left;
   Seq q;
-  __device__ __forceinline__ Walk(const Params& p, int s0, int off0, int n)
-      : s(s0), off(off0), left(n) {
-    if (left > 0) q = load_seq<FN>(p, s);
-  }
   __device__ __forceinline__ bool next(const Params& p) {
     if (left <= 0) return false;
     while (off >= q.total) {
@@ -255,16 +274,14 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
   uint64_t* u_empty = u_full + kUnits;                                // [kUnits]
   uint64_t* v_dirty = u_empty + kUnits;
   uint64_t* v_clean = v_dirty + 1;
-  int* share_of = reinterpret_cast<int*>(v_clean + 1);  // sequence, offset, tiles
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(share_of + 3);
-  static_assert((2 * (NK + NV) + 10 + 12 + 3 + 2 * kUnits + 2) * 8 + 16 +
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_clean + 1);
+  static_assert((2 * (NK + NV) + 10 + 12 + 3 + 2 * kUnits + 2) * 8 + 8 +
                     kUnits * (int)sizeof(Unit) <= kBarBytes, "barriers and units");
   Unit* units_sh = reinterpret_cast<Unit*>(sEnd + kBarBytes) - kUnits;
   float* sh_ref = reinterpret_cast<float*>(sEnd + kBarBytes);  // [FM]
   float* sh_sum = sh_ref + FM;                                                // [2][FM]
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  pdl_wait();
   if (threadIdx.x == 0) {
     for (int i = 0; i < NK; ++i) {
       mbar_init(&k_full[i], 1);
@@ -302,63 +319,13 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
-  if (warp == 12) {
-    // The share: a scan over the sequences, 32 at a time, for the total and
-    // then for the sequence in which this CTA's first tile lies.
-    long long total = 0, first32 = 0;
-    for (int b = 0; b < p.num_seqs; b += 32) {
-      const int s = b + lane;
-      long long n = s < p.num_seqs ? load_seq<FN>(p, s).total : 0;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long up = __shfl_up_sync(0xffffffffu, n, o);
-        if (lane >= o) n += up;
-      }
-      if (b == 0) first32 = n;
-      total += __shfl_sync(0xffffffffu, n, 31);
-    }
-    const long long share =
-        max((long long)kMinShare, (total + gridDim.x - 1) / (long long)gridDim.x);
-    const long long t0 = share * blockIdx.x;
-    const long long n = min(share, total - t0);
-    int seq = 0, off = 0;
-    long long seen = 0;
-    bool found = n <= 0;
-    for (int b = 0; b < p.num_seqs && !found; b += 32) {
-      long long c = first32;  // sums up to and with this lane's sequence
-      if (b > 0) {
-        const int s = b + lane;
-        c = s < p.num_seqs ? load_seq<FN>(p, s).total : 0;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const long long up = __shfl_up_sync(0xffffffffu, c, o);
-          if (lane >= o) c += up;
-        }
-      }
-      const long long before = __shfl_up_sync(0xffffffffu, c, 1);
-      const uint32_t hit = __ballot_sync(0xffffffffu, seen + c > t0);
-      if (hit) {
-        const int l = __ffs(hit) - 1;
-        seq = b + l;
-        off = (int)(t0 - seen - __shfl_sync(0xffffffffu, lane > 0 ? before : 0, l));
-        found = true;
-      }
-      seen += __shfl_sync(0xffffffffu, c, 31);
-    }
-    if (lane == 0) {
-      share_of[0] = seq;
-      share_of[1] = off;
-      share_of[2] = (int)max(0ll, n);
-      if (blockIdx.x == 0) *p.share = share;
-    }
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  pdl_wait();
   if (threadIdx.x == 0) pdl_trigger();
   const uint32_t tmem_base = *tmem_slot;
   const uint32_t tS = tmem_base, tO = tS + 2 * FN, tP = tO + D;
-  const int N = share_of[2];  // key tiles of this CTA
   // Unit u for a reader (a warp, or one thread with `alone`).
   auto take = [&](int u, Unit& x, bool alone) -> bool {
     const int e = u % kUnits;
@@ -381,7 +348,64 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
     const int nb = BS >= FN ? 1 : FN / BS;
     const int rows_box = BS >= FN ? FN : BS;
     const int bi = lane % nb, h = lane / nb;
-    Walk<FN> walk(p, share_of[0], share_of[1], is_v ? 0 : N);
+    // The share (warp 0): a scan over the sequences, 32 at a time, for the
+    // total and then for the sequence in which this CTA's first tile lies.
+    Walk<FN> walk;
+    int share = 0;
+    if (!is_v) {
+      long long total = 0, sums = 0;
+      Seq mine;
+      for (int b = 0; b < p.num_seqs; b += 32) {
+        long long c = 0;
+        if (b + lane < p.num_seqs) {
+          const Seq q = load_seq<FN>(p, b + lane);
+          c = q.total;
+          if (b == 0) mine = q;
+        }
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const long long up = __shfl_up_sync(0xffffffffu, c, o);
+          if (lane >= o) c += up;
+        }
+        if (b == 0) sums = c;
+        total += __shfl_sync(0xffffffffu, c, 31);
+      }
+      const long long per =
+          max((long long)kMinShare, (total + gridDim.x - 1) / (long long)gridDim.x);
+      const long long t0 = per * blockIdx.x, n = min(per, total - t0);
+      share = (int)per;
+      walk.left = (int)max(0ll, n);
+      walk.s = walk.off = 0;
+      long long seen = 0;
+      bool found = n <= 0;
+      for (int b = 0; b < p.num_seqs && !found; b += 32) {
+        long long c = sums;  // sums up to and with this lane's sequence
+        if (b > 0) {
+          c = 0;
+          if (b + lane < p.num_seqs) {
+            mine = load_seq<FN>(p, b + lane);
+            c = mine.total;
+          }
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const long long up = __shfl_up_sync(0xffffffffu, c, o);
+            if (lane >= o) c += up;
+          }
+        }
+        const long long before = __shfl_up_sync(0xffffffffu, c, 1);
+        const uint32_t hit = __ballot_sync(0xffffffffu, seen + c > t0);
+        if (hit) {
+          const int l = __ffs(hit) - 1;
+          walk.s = b + l;
+          walk.off = (int)(t0 - seen - __shfl_sync(0xffffffffu, lane > 0 ? before : 0, l));
+          walk.q = share_seq(mine, l);
+          found = true;
+        }
+        seen += __shfl_sync(0xffffffffu, c, 31);
+      }
+    } else {
+      walk.left = 0;
+    }
     int published = 0;
     auto publish = [&](Unit& x) -> bool {  // the next unit, to the others and to x
       const int e = published % kUnits;
@@ -406,7 +430,13 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
       if (ok && lane == 0) {
         units_sh[e] = x;
         mbar_arrive(&u_full[e]);
-        if (published == 0) p.cut[blockIdx.x] = Cut{x.seq, more ? walk.unit : 0, x.j0, 0};
+        if (published == 0) {
+          // Tiles of the unit from its first on; an earlier edge than this
+          // one joins a unit that began more than a share before.
+          const bool mine = more && x.j0 > 0 && x.j0 <= share;
+          const int last = (int)blockIdx.x + (walk.q.n_tiles - x.j0 - 1) / max(share, 1);
+          p.cut[blockIdx.x] = Cut{x.q0, x.kvh, x.row0, mine ? min(FM, x.rows) : 0, last, {0, 0, 0}};
+        }
       }
       ++published;
       return ok != 0;
@@ -767,8 +797,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
 #pragma unroll
               for (int i = 0; i < 16; ++i) {
                 const float va = __uint_as_float(r[2 * i]), vb = __uint_as_float(r[2 * i + 1]);
-                mxa = fmaxf(mxa, va);
-                mxb = fmaxf(mxb, vb);
+                if (i & 1) mxa = max3(mxa, va, vb);
+                else mxb = max3(mxb, va, vb);
                 if constexpr (kWrite) {
                   float ea, eb;
                   f32x2_unpack(f32x2_fma(f32x2_pack(va, vb), sc2, nmu2), ea, eb);
@@ -831,12 +861,12 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
             const float m_new = resc ? mx : m_prev;
             hand_on(m_new);
             if (__any_sync(0xffffffffu, resc)) {
-              // O is final for the tiles before once P V of tile n - 1 is done
-              // (its barrier's round before first: the parity tells two apart).
-              ok = __all_sync(
-                  0xffffffffu,
-                  (n < 3 || mbar_wait(&p_free[grp ^ 1], (uint32_t)(((n - 3) >> 1) & 1), p.err)) &&
-                      mbar_wait(&p_free[grp ^ 1], (uint32_t)(((n - 1) >> 1) & 1), p.err));
+              // O is final for the tiles before once P V of tile n - 1 is done.
+              // (P V of tile n - 2 is, by the wait above, so that of tile n - 3,
+              // the round before in this barrier, is too; and that of tile
+              // n + 1 cannot be.)
+              ok = __all_sync(0xffffffffu, mbar_wait(&p_free[grp ^ 1],
+                                                     (uint32_t)(((n - 1) >> 1) & 1), p.err));
               if (!ok) break;
               tc_fence_after();
               const float alpha = !resc ? 1.f : m_prev == -INFINITY ? 0.f : exp2f(m_prev - m_new);
@@ -905,69 +935,78 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
   }
 }
 
-// Joins the pieces of units that were cut, in share order. Block (c - 1, y)
-// looks at the edge before share c: if the unit there began in share c - 1, it
-// joins 16 of its rows, a warp a row.
+// Joins the pieces of units that were cut, in share order: a warp a row, one
+// block for eight rows of the unit that is cut where share blockIdx.x + 1
+// begins.
+constexpr int kJoinRows = 8;
 template <int D_>
-__global__ void __launch_bounds__(128) tree_join_kernel(const Params p) {
-  constexpr int D = D_, FN = Cfg<D_>::FN;
+__global__ void __launch_bounds__(kJoinRows * 32) tree_join_kernel(const Params p) {
+  constexpr int D = D_;
   constexpr int V = D >= 128 ? D / 128 : 1;  // float4 of a lane
+  constexpr int kAhead = 8;                  // pieces in flight
   pdl_wait();
   pdl_trigger();
   const int c1 = blockIdx.x + 1;
   const Cut cut = p.cut[c1];
-  if (cut.j0 == 0) return;
-  const int share = (int)*p.share;
-  const Seq q = load_seq<FN>(p, cut.seq);
-  const long long a = (long long)c1 * share - cut.j0;  // the unit's first tile
-  if (cut.j0 > share) return;                          // an earlier edge joins it
-  const int kvh = cut.unit / q.n_rt, row0 = (cut.unit - kvh * q.n_rt) * FM;
-  const int c_last = (int)((a + q.n_tiles - 1) / share);
-  const int lane = threadIdx.x % 32;
+  const int row = blockIdx.y * kJoinRows + threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (row >= cut.rows) return;
+  const int g = cut.row0 + row, t = g / p.G, head = cut.kvh * p.G + g - t * p.G;
   const bool on = D >= 128 || lane < D / 4;
-  for (int row = blockIdx.y * 16 + threadIdx.x / 32; row < min(FM, (int)blockIdx.y * 16 + 16);
-       row += 4) {
-    const int g = row0 + row;
-    if (g >= q.q_len * p.G) return;
-    const int t = g / p.G, head = kvh * p.G + g - t * p.G;
-    // The first piece is the last of share c1 - 1, the others open theirs.
-    auto piece = [&](int c) { return ((long long)c * 2 + (c < c1 ? 1 : 0)) * FM + row; };
-    float m = -INFINITY;
-    for (int c = c1 - 1 + lane; c <= c_last; c += 32) m = fmaxf(m, p.part_ml[piece(c)].x);
+  const int n = cut.last - c1 + 2;
+  // Piece i: the first is the last of share c1 - 1, the others open theirs.
+  auto piece = [&](int i) { return ((long long)(c1 - 1 + i) * 2 + (i == 0 ? 1 : 0)) * FM + row; };
+  float m = -INFINITY;
+  for (int i = lane; i < n; i += 32) m = fmaxf(m, p.part_ml[piece(i)].x);
+  float den = 0.f;
+  float4 acc[V];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float den = 0.f;
-    float4 acc[V];
+  for (int v = 0; v < V; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = 0; i0 < n; i0 += kAhead) {
+    float4 o[kAhead][V];
+    float2 ml[kAhead];
 #pragma unroll
-    for (int v = 0; v < V; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int c = c1 - 1; c <= c_last; ++c) {
-      const long long pc = piece(c);
-      const float2 ml = p.part_ml[pc];
-      const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m);
-      den += ml.y * f;
-      if (on) {
+    for (int k = 0; k < kAhead; ++k) {
+      ml[k] = make_float2(-INFINITY, 0.f);
+      if (i0 + k < n) {
+        const long long pc = piece(i0 + k);
+        ml[k] = p.part_ml[pc];
+        if (on) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const float4 o = *reinterpret_cast<const float4*>(p.part_o + pc * D + (v * 32 + lane) * 4);
-          acc[v].x += o.x * f;
-          acc[v].y += o.y * f;
-          acc[v].z += o.z * f;
-          acc[v].w += o.w * f;
+          for (int v = 0; v < V; ++v)
+            o[k][v] = *reinterpret_cast<const float4*>(p.part_o + pc * D + (v * 32 + lane) * 4);
         }
       }
     }
-    if (p.sinks != nullptr)
-      den = m == -INFINITY ? 1.f : den + exp2f(p.sinks[head] * 1.4426950408889634f - m);
-    const float inv = den > 0.f ? 1.f / den : 0.f;
-    if (on) {
-      __nv_bfloat16* dst = p.out + (long long)(q.q0 + t) * p.o_stride + (long long)head * D;
+    if (i0 == 0) {
 #pragma unroll
-      for (int v = 0; v < V; ++v)
-        *reinterpret_cast<uint2*>(dst + (v * 32 + lane) * 4) =
-            make_uint2(pack_bf16x2(acc[v].x * inv, acc[v].y * inv),
-                       pack_bf16x2(acc[v].z * inv, acc[v].w * inv));
+      for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
     }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (i0 + k >= n) break;
+      const float f = ml[k].x == -INFINITY ? 0.f : exp2f(ml[k].x - m);
+      den += ml[k].y * f;
+      if (on) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          acc[v].x += o[k][v].x * f;
+          acc[v].y += o[k][v].y * f;
+          acc[v].z += o[k][v].z * f;
+          acc[v].w += o[k][v].w * f;
+        }
+      }
+    }
+  }
+  if (p.sinks != nullptr)
+    den = m == -INFINITY ? 1.f : den + exp2f(p.sinks[head] * 1.4426950408889634f - m);
+  const float inv = den > 0.f ? 1.f / den : 0.f;
+  if (on) {
+    __nv_bfloat16* dst = p.out + (long long)(cut.q0 + t) * p.o_stride + (long long)head * D;
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      *reinterpret_cast<uint2*>(dst + (v * 32 + lane) * 4) =
+          make_uint2(pack_bf16x2(acc[v].x * inv, acc[v].y * inv),
+                     pack_bf16x2(acc[v].z * inv, acc[v].w * inv));
   }
 }
 
@@ -1001,7 +1040,6 @@ void launch_d(const TreeAttnArgs& a, cudaStream_t stream) {
   p.part_o = a.workspace;
   p.part_ml = reinterpret_cast<float2*>(a.workspace + (size_t)grid * 2 * FM * D);
   p.cut = reinterpret_cast<Cut*>(p.part_ml + (size_t)grid * 2 * FM);
-  p.share = reinterpret_cast<long long*>(p.cut + grid);
   p.num_seqs = a.num_seqs;
   p.Hq = a.Hq;
   p.Hkv = a.Hkv;
@@ -1019,13 +1057,14 @@ void launch_d(const TreeAttnArgs& a, cudaStream_t stream) {
   p.err = device_status_ptr(dev);
   launch_pdl(kernel, dim3(grid), dim3(kThreads), C::kSmem, stream, nullptr, tk, tv, p);
   if (grid > 1)
-    launch_pdl(tree_join_kernel<D>, dim3(grid - 1, FM / 16), dim3(128), 0, stream, nullptr, p);
+    launch_pdl(tree_join_kernel<D>, dim3(grid - 1, FM / kJoinRows), dim3(kJoinRows * 32), 0, stream,
+               nullptr, p);
 }
 
 }  // namespace
 
 size_t tree_attention_workspace_bytes(int head_dim, int num_sm) {
-  return (size_t)num_sm * (2 * FM * (head_dim + 2) * 4 + sizeof(Cut)) + 16;
+  return (size_t)num_sm * (2 * FM * (head_dim + 2) * 4 + sizeof(Cut));
 }
 
 void tree_attention_launch(const TreeAttnArgs& a, cudaStream_t stream) {
