@@ -35,17 +35,18 @@
 //              exponent reference a row (base 2, raised lazily: O is rescaled
 //              when a row's max grows by more than 2^8 over it), which the
 //              groups hand to each other in tile order through shared memory
-//              as soon as a tile's maximum is known. A unit's epilogue (half
-//              of O's columns each) comes after the next unit's first tile,
-//              when the last P V has long finished.
-//   warp 10    issues S = Q K^T into one of two S buffers, as soon as softmax
-//              has finished with the tile before in it
+//              as soon as a tile's maximum is known. P (bf16) goes over the
+//              first half of its scores. A unit's epilogue (half of O's
+//              columns each) comes after the next unit's first tile, when the
+//              last P V has long finished.
+//   warp 10    issues S = Q K^T into one of three buffers, as soon as P V of
+//              the tile before in it is done
 //   warp 11    issues O += P V (its own warp: an issuing thread spends longer
 //              on waits and descriptors than the tensor core on a product)
 //   warp 12    loads Q rows (the next unit's while the present one runs) and
 //              zeroes V rows that no node sees (past the end, before the
 //              window): they may hold anything, and 0 x NaN is not 0.
-// TMEM columns: S0 | S1 | O | P0 | P1.
+// TMEM columns: S0 | S1 | S2 | O.
 //
 // Rounding: P is rounded to bf16 for the tensor core (relative 2^-8 a term at
 // most, as the output's own rounding); scores, maxima, sums and O are fp32.
@@ -262,10 +263,12 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
   uint64_t* v_empty = v_full + NV;                                    // [NV]
   uint64_t* q_full = v_empty + NV;                                    // [2]
   uint64_t* q_empty = q_full + 2;                                     // [2]
-  uint64_t* s_full = q_empty + 2;                                     // [2]
-  uint64_t* p_full = s_full + 2;                                      // [2]
-  uint64_t* p_free = p_full + 2;                                      // [2]
-  uint64_t* post = p_free + 2;                                        // [2][4]
+  // A tile's S and P are announced by barrier n % 4: a group's tiles n and
+  // n + 2 may both be on their way, n + 4 only when all have seen n.
+  uint64_t* s_full = q_empty + 2;                                     // [4]
+  uint64_t* p_full = s_full + 4;                                      // [4]
+  uint64_t* s_free = p_full + 4;                                      // [3], by buffer
+  uint64_t* post = s_free + 3;                                        // [2][4]
   uint64_t* pair = post + 8;                                          // [4]
   uint64_t* o_full = pair + 4;
   uint64_t* o_free = o_full + 1;
@@ -275,7 +278,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
   uint64_t* v_dirty = u_empty + kUnits;
   uint64_t* v_clean = v_dirty + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_clean + 1);
-  static_assert((2 * (NK + NV) + 10 + 12 + 3 + 2 * kUnits + 2) * 8 + 8 +
+  static_assert((2 * (NK + NV) + 4 + 11 + 12 + 3 + 2 * kUnits + 2) * 8 + 8 +
                     kUnits * (int)sizeof(Unit) <= kBarBytes, "barriers and units");
   Unit* units_sh = reinterpret_cast<Unit*>(sEnd + kBarBytes) - kUnits;
   float* sh_ref = reinterpret_cast<float*>(sEnd + kBarBytes);  // [FM]
@@ -294,12 +297,12 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 1);
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
-      mbar_init(&p_free[i], 1);
     }
+    for (int i = 0; i < 3; ++i) mbar_init(&s_free[i], 1);
     for (int i = 0; i < 8; ++i) mbar_init(&post[i], 1);
     for (int i = 0; i < 4; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
       mbar_init(&pair[i], 2);
     }
     mbar_init(v_dirty, 1);
@@ -325,7 +328,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
   pdl_wait();
   if (threadIdx.x == 0) pdl_trigger();
   const uint32_t tmem_base = *tmem_slot;
-  const uint32_t tS = tmem_base, tO = tS + 2 * FN, tP = tO + D;
+  const uint32_t tS = tmem_base, tO = tS + 3 * FN;
   // Unit u for a reader (a warp, or one thread with `alone`).
   auto take = [&](int u, Unit& x, bool alone) -> bool {
     const int e = u % kUnits;
@@ -500,10 +503,10 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
         const int qb = u % NQ;
         ok = mbar_wait(&q_full[qb], (uint32_t)((u / NQ) & 1), p.err);
         for (int j = x.j0; j < x.j1 && ok; ++j, ++n) {
-          const int sb = n & 1;
-          // K is there, and softmax has finished with tile n - 2.
+          const int sb = n % 3;
+          // K is there, and P V of tile n - 3 done with the buffer.
           ok = mbar_wait(&k_full[st], round, p.err) &&
-               (n < 2 || mbar_wait(&p_full[sb], (uint32_t)(((n >> 1) & 1) ^ 1), p.err));
+               mbar_wait(&s_free[sb], (uint32_t)(((n / 3) & 1) ^ 1), p.err);
           if (!ok) break;
           tc_fence_after();
           const uint64_t dq = dq0 + (uint64_t)(qb * (C::kQBytes >> 4));
@@ -515,7 +518,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
               umma_f16(tS + sb * FN, dq + (uint64_t)(kb * (C::kQChunk >> 4) + 2 * k),
                        dk + (uint64_t)(kb * (C::kChunk >> 4) + 2 * k), idesc,
                        (kb > 0 || k > 0) ? 1u : 0u);
-          umma_commit(&s_full[sb]);
+          umma_commit(&s_full[n & 3]);
           umma_commit(&k_empty[st]);
           if (++st == NK) {
             st = 0;
@@ -540,13 +543,13 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
       uint32_t round = 0;
       for (int u = 0; ok && take(u, x, true) && x.j0 < x.j1; ++u) {
         for (int j = x.j0; j < x.j1 && ok; ++j, ++n) {
-          const int pb = n & 1;
+          const int pb = n % 3;
           const bool dirty = x.template dirty<FN>(j);
           // V is there, without rows that no node sees; P is; O has been read
           // by the epilogue of the unit before.
           ok = mbar_wait(&v_full[st], round, p.err);
           if (ok && dirty) mbar_arrive(v_dirty);
-          ok = ok && mbar_wait(&p_full[pb], (uint32_t)((n >> 1) & 1), p.err) &&
+          ok = ok && mbar_wait(&p_full[n & 3], (uint32_t)((n >> 2) & 1), p.err) &&
                (!dirty || mbar_wait(v_clean, (uint32_t)(cleaned & 1), p.err)) &&
                (j > x.j0 || mbar_wait(o_free, (uint32_t)((u & 1) ^ 1), p.err));
           if (!ok) break;
@@ -555,9 +558,9 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
           const uint64_t dv = dv0 + (uint64_t)(st * (C::kTile >> 4));
 #pragma unroll
           for (int s = 0; s < FN / 16; ++s)
-            umma_f16_ts(tO, tP + pb * (FN / 2) + s * 8, dv + (uint64_t)(s * (16 * 128 >> 4)), idesc,
+            umma_f16_ts(tO, tS + pb * FN + s * 8, dv + (uint64_t)(s * (16 * 128 >> 4)), idesc,
                         (j > x.j0 || s > 0) ? 1u : 0u);
-          umma_commit(&p_free[pb]);
+          umma_commit(&s_free[pb]);
           umma_commit(&v_empty[st]);
           if (++st == NV) {
             st = 0;
@@ -753,10 +756,10 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
       }
       for (int j = x.j0; j < x.j1; ++j, ++n) {
         if ((n & 1) == grp) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&s_full[grp], (uint32_t)((n >> 1) & 1), p.err));
+          ok = __all_sync(0xffffffffu, mbar_wait(&s_full[n & 3], (uint32_t)((n >> 2) & 1), p.err));
           if (!ok) break;
           tc_fence_after();
-          const uint32_t s_row = tS + lane_base + grp * FN, p_row = tP + lane_base + grp * (FN / 2);
+          const uint32_t s_row = tS + lane_base + n % 3 * FN;
           const int kb = x.k_lo + j * FN;
           if (warp_on && (__any_sync(0xffffffffu, key_lo > kb) || kb + FN > x.prefix)) {
             // Hidden scores become -inf in TMEM, by a loop of its own: the code
@@ -779,58 +782,28 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
             }
             tmem_wait_st();
           }
-          // One pass over the row's scores, 32 at a time (short loops: an SM's
-          // instruction cache misses cost more than what unrolling gains).
-          // WRITE: P = 2^(S scale - mu) as bf16 pairs, their sum to *rs.
-          // Returns the row's maximum in log2 units.
-          auto sweep = [&](auto write_c, float mu, float* rs) -> float {
-            constexpr bool kWrite = decltype(write_c)::value;
+          // The row's maximum (log2 units), 32 scores at a time. (Short loops:
+          // an SM's instruction cache misses cost more than unrolling gains.)
+          float own = -INFINITY;
+          if (warp_on) {
             float mxa = -INFINITY, mxb = -INFINITY;
-            const float mu_eff = mu == -INFINITY ? 0.f : mu;
-            const uint64_t nmu2 = f32x2_pack(-mu_eff, -mu_eff);
-            uint64_t acc[2] = {f32x2_pack(0.f, 0.f), f32x2_pack(0.f, 0.f)};
 #pragma unroll 1
             for (int c = 0; c < FN / 32; ++c) {
-              uint32_t r[32], w[16];
+              uint32_t r[32];
               tmem_ld_32x32b_x32(s_row + c * 32, r);
               tmem_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const float va = __uint_as_float(r[2 * i]), vb = __uint_as_float(r[2 * i + 1]);
-                if (i & 1) mxa = max3(mxa, va, vb);
-                else mxb = max3(mxb, va, vb);
-                if constexpr (kWrite) {
-                  float ea, eb;
-                  f32x2_unpack(f32x2_fma(f32x2_pack(va, vb), sc2, nmu2), ea, eb);
-                  ea = fast_exp2(ea);
-                  eb = fast_exp2(eb);
-                  acc[i & 1] = f32x2_add(acc[i & 1], f32x2_pack(ea, eb));
-                  w[i] = pack_bf16x2(ea, eb);
-                }
+              for (int i = 0; i < 16; i += 2) {
+                mxa = max3(mxa, __uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+                mxb = max3(mxb, __uint_as_float(r[2 * i + 2]), __uint_as_float(r[2 * i + 3]));
               }
-              if constexpr (kWrite) tmem_st_32x32b_x16(p_row + c * 16, w);
             }
-            if constexpr (kWrite) {
-              float a0, a1;
-              f32x2_unpack(f32x2_add(acc[0], acc[1]), a0, a1);
-              *rs = a0 + a1;
-            }
-            const float mx = fmaxf(mxa, mxb);
-            return mx == -INFINITY ? mx : mx * sc;
-          };
-          using T_ = std::true_type;
-          using F_ = std::false_type;
-          auto hand_on = [&](float m) {  // the reference, to the tile after
-            sh_ref[row] = m;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&post[grp * 4 + q4]);
-          };
-          // The reference to try: O's, as far as it is known. A group's first
-          // tile of a unit waits for it (it follows the unit's first tile's
-          // maximum at once); later ones take their own last and look at the
-          // other group's after the pass, when that has long been handed on.
+            own = fmaxf(mxa, mxb);
+            own = own == -INFINITY ? own : own * sc;
+          }
+          // The reference from the tile before, to the tile after.
           float m_prev = -INFINITY;
-          if (n > 0 && j <= x.j0 + 1) {
+          if (n > 0) {
             ok = ref_after(n - 1, m_prev);
             if (!ok) break;
           }
@@ -839,37 +812,22 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
             m_prev = m_own = -INFINITY;
             l = 0.f;
           }
-          float m = j <= x.j0 + 1 ? m_prev : m_own;
-          if (warp_on && __any_sync(0xffffffffu, m == -INFINITY)) {
-            const float mx = sweep(F_{}, 0.f, nullptr);
-            if (m == -INFINITY) m = mx;
-          }
-          if (j == x.j0) hand_on(m);
-          // This P buffer is free once P V of tile n - 2 has completed (a warp
-          // without rows waits too, or it would be a tile ahead).
-          if (n >= 2) ok = mbar_wait(&p_free[grp], (uint32_t)(((n - 2) >> 1) & 1), p.err);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          float rs = 0.f, mx = -INFINITY;
-          if (warp_on) mx = sweep(T_{}, m, &rs);
-          if (j > x.j0) {
-            if (j > x.j0 + 1) {
-              ok = ref_after(n - 1, m_prev);
-              if (!ok) break;
-            }
-            const bool resc = mx > m_prev + 8.f || (m_prev == -INFINITY && mx != -INFINITY);
-            const float m_new = resc ? mx : m_prev;
-            hand_on(m_new);
-            if (__any_sync(0xffffffffu, resc)) {
+          const bool resc = own > m_prev + 8.f || (m_prev == -INFINITY && own != -INFINITY);
+          const float m = resc ? own : m_prev;
+          sh_ref[row] = m;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&post[grp * 4 + q4]);
+          if (warp_on) {
+            if (j > x.j0 && __any_sync(0xffffffffu, resc)) {
               // O is final for the tiles before once P V of tile n - 1 is done.
-              // (P V of tile n - 2 is, by the wait above, so that of tile n - 3,
-              // the round before in this barrier, is too; and that of tile
-              // n + 1 cannot be.)
-              ok = __all_sync(0xffffffffu, mbar_wait(&p_free[grp ^ 1],
-                                                     (uint32_t)(((n - 1) >> 1) & 1), p.err));
+              // (Its buffer's barrier is in that round: S of tile n - 1 went
+              // there after the round before, and P V of tile n + 2 comes
+              // after this tile's.)
+              ok = __all_sync(0xffffffffu, mbar_wait(&s_free[(n - 1) % 3],
+                                                     (uint32_t)(((n - 1) / 3) & 1), p.err));
               if (!ok) break;
               tc_fence_after();
-              const float alpha = !resc ? 1.f : m_prev == -INFINITY ? 0.f : exp2f(m_prev - m_new);
+              const float alpha = !resc ? 1.f : m_prev == -INFINITY ? 0.f : exp2f(m_prev - m);
 #pragma unroll 1
               for (int c = 0; c < D / 16; ++c) {
                 uint32_t o[16];
@@ -881,21 +839,40 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
                 tmem_st_32x32b_x16(tO + lane_base + c * 16, o);
               }
             }
-            if (__any_sync(0xffffffffu, m != m_new)) {
-              m = m_new;
-              tmem_wait_st();
-              sweep(T_{}, m, &rs);  // P once more, against the reference of O
+            if (m != m_own) {
+              l = m_own == -INFINITY ? 0.f : l * exp2f(m_own - m);
+              m_own = m;
             }
+            // P = 2^(S scale - m) as bf16 pairs, over scores already read.
+            const float mu = m == -INFINITY ? 0.f : m;
+            const uint64_t nmu2 = f32x2_pack(-mu, -mu);
+            uint64_t acc[2] = {f32x2_pack(0.f, 0.f), f32x2_pack(0.f, 0.f)};
+#pragma unroll 1
+            for (int c = 0; c < FN / 32; ++c) {
+              uint32_t r[32], w[16];
+              tmem_ld_32x32b_x32(s_row + c * 32, r);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                float ea, eb;
+                f32x2_unpack(f32x2_fma(f32x2_pack(__uint_as_float(r[2 * i]),
+                                                  __uint_as_float(r[2 * i + 1])), sc2, nmu2),
+                             ea, eb);
+                ea = fast_exp2(ea);
+                eb = fast_exp2(eb);
+                acc[i & 1] = f32x2_add(acc[i & 1], f32x2_pack(ea, eb));
+                w[i] = pack_bf16x2(ea, eb);
+              }
+              tmem_st_32x32b_x16(s_row + c * 16, w);
+            }
+            float a0, a1;
+            f32x2_unpack(f32x2_add(acc[0], acc[1]), a0, a1);
+            l += a0 + a1;
           }
-          if (m != m_own) {
-            l = m_own == -INFINITY ? 0.f : l * exp2f(m_own - m);
-            m_own = m;
-          }
-          l += rs;
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[grp]);
+          if (lane == 0) mbar_arrive(&p_full[n & 3]);
         } else if (j == x.j0) {
           // The other group's tile: this one did the last of the unit before.
           if (u > 0) close(m_own);
