@@ -40,7 +40,8 @@ def _check_scores(x, y, n, t=1.0):
     assert torch.equal(r.top_ids, e.top_ids)
     for a, b in ((r.logprobs, e.logprobs), (r.entropy, e.entropy), (r.lse, e.lse),
                  (r.top_logprobs, e.top_logprobs)):
-        torch.testing.assert_close(a.double(), b, atol=TOL, rtol=TOL, equal_nan=True)
+        # (rounded to the output's type: 64 bits hold log-probs that fp32 has as -inf)
+        torch.testing.assert_close(a, b.float(), atol=TOL, rtol=TOL, equal_nan=True)
 
 
 SHAPES = [(1, 1), (3, 7), (5, 1000), (2, 32003), (17, 4099), (9, 151936), (700, 1031),
@@ -97,6 +98,24 @@ def test_scores_masks_and_ties(b200_ops, dtype, rows):
         _check_scores(x, y, n)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_scores_far_out_and_forbidden(b200_ops, dtype):
+    """Rows whose maximum lies far below or above, and given tokens whose own
+    logit is -inf, in rows at every alignment."""
+    x = _rows(40, 4099, dtype, 3, pad=2, offset=3)
+    x[0], x[1, :] = -3e37, 2e37
+    x[1, 7] = 2.5e37
+    x[2] = -5e29
+    x[2, 9:12] = -4e29
+    x[3, ::2] = -2e30
+    x[4, 1:] = -INF
+    x[4, 0] = torch.finfo(dtype).min
+    x[5:] = torch.where(torch.rand(35, 4099, device="cuda") < 0.5, -INF, x[5:].float()).to(dtype)
+    x[5:, 2000] = -INF
+    _check_scores(x, torch.full((40,), 2000, device="cuda"), 20)
+    _check_scores(x, torch.arange(40, device="cuda") % 9, 5, 0.01)
+
+
 def test_scores_clustered_top(b200_ops):
     """More than 512 elements of few threads above every other thread's: the
     bound is raised to the exact one."""
@@ -109,6 +128,25 @@ def test_scores_clustered_top(b200_ops):
     y = torch.randint(0, V, (330,), device="cuda", generator=g)
     _check_scores(xf.bfloat16(), y, 64)
     _check_scores(xf.view(330, V), y, 64)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_scores_largest_vocabulary(b200_ops, dtype):
+    """Where a thread has more groups of vectors than places for their maxima."""
+    x = _rows(2, 2 ** 22 - 3, dtype, 6, pad=3, offset=1)
+    _check_scores(x, torch.tensor([2 ** 22 - 4, 0], device="cuda"), 64)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows", [3, 600])
+def test_scores_top_in_every_warp(b200_ops, dtype, rows):
+    """Some 1500 elements above every other, in few groups of every warp."""
+    x = torch.full((rows, 65536), -3.0, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x.view(rows, 1024, 64)[:, ::2, :3] = torch.randn(rows, 512, 3, device="cuda", generator=g) + 10
+    y = torch.randint(0, 65536, (rows,), device="cuda", generator=g)
+    _check_scores(x.to(dtype), y, 64)
+    _check_scores(x.to(dtype), y, 9)
 
 
 def test_scores_nan_inf_and_no_token(b200_ops):

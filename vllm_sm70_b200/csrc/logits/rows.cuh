@@ -32,6 +32,18 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Where a sum needs x (x - m) finite, elements below this count as this: their
+// exponentials are zero all the same unless the whole row lies down there
+// (rows whose maximum does are summed element by element, slow_sums).
+constexpr float kFloor = -1e30f;
+constexpr float kSlowBelow = -1e29f, kSlowAbove = 1e30f;
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
 __device__ __forceinline__ uint4 ldg_stream(const void* p) {
   uint4 v;
   asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
@@ -58,7 +70,6 @@ template <>
 struct Traits<__nv_bfloat16> {
   static constexpr int E = 8;                        // elements of a 16-byte vector
   static constexpr uint32_t kNegInf = 0xff80ff80u;   // one word of -inf elements
-  static constexpr int kKeyLowBit = 16;              // key bits below are constant per sign
   __device__ static __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
   // Elements 2i and 2i + 1 of a vector.
   __device__ static __forceinline__ void pair(const uint4& v, int i, float& a, float& b) {
@@ -66,13 +77,32 @@ struct Traits<__nv_bfloat16> {
     a = bf16_bits_lo(w);
     b = bf16_bits_hi(w);
   }
-  __device__ static __forceinline__ float max_of(const uint4& v) {
+  // A vector's maximum, kept packed; NaN elements do not count.
+  using Max = __nv_bfloat162;
+  __device__ static __forceinline__ Max vmax(const uint4& v) {
     const __nv_bfloat162 a = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&v.x),
                                      *reinterpret_cast<const __nv_bfloat162*>(&v.y));
     const __nv_bfloat162 b = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&v.z),
                                      *reinterpret_cast<const __nv_bfloat162*>(&v.w));
-    const __nv_bfloat162 c = __hmax2(a, b);
-    return fmaxf(__low2float(c), __high2float(c));
+    return __hmax2(a, b);
+  }
+  __device__ static __forceinline__ Max vmax(Max a, Max b) { return __hmax2(a, b); }
+  __device__ static __forceinline__ float value(Max m) {
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+  __device__ static __forceinline__ float max_of(const uint4& v) { return value(vmax(v)); }
+  // Is every element below y (an element's value)?
+  __device__ static __forceinline__ bool all_below(Max m, float y) {
+    return __hblt2(m, __float2bfloat162_rn(y));
+  }
+  // Elements 2i and 2i + 1, not below kFloor.
+  __device__ static __forceinline__ void pair_floor(const uint4& v, int i, float& a, float& b) {
+    const uint32_t w = i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+    const __nv_bfloat162 f = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&w),
+                                         __float2bfloat162_rn(kFloor));
+    const uint32_t u = *reinterpret_cast<const uint32_t*>(&f);
+    a = bf16_bits_lo(u);
+    b = bf16_bits_hi(u);
   }
   // Packed counter of elements above (or, GE, at or above) a value: adds one
   // 16-bit all-ones mask a hit. n = lo + hi with sum = 65536 (lo - hi) - lo.
@@ -112,15 +142,24 @@ template <>
 struct Traits<float> {
   static constexpr int E = 4;
   static constexpr uint32_t kNegInf = 0xff800000u;
-  static constexpr int kKeyLowBit = 0;
   __device__ static __forceinline__ float to_f(float v) { return v; }
   __device__ static __forceinline__ void pair(const uint4& v, int i, float& a, float& b) {
     a = __uint_as_float(i == 0 ? v.x : v.z);
     b = __uint_as_float(i == 0 ? v.y : v.w);
   }
-  __device__ static __forceinline__ float max_of(const uint4& v) {
+  using Max = float;
+  __device__ static __forceinline__ Max vmax(const uint4& v) {
     return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)),
                  fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+  }
+  __device__ static __forceinline__ Max vmax(Max a, Max b) { return fmaxf(a, b); }
+  __device__ static __forceinline__ float value(Max m) { return m; }
+  __device__ static __forceinline__ float max_of(const uint4& v) { return vmax(v); }
+  __device__ static __forceinline__ bool all_below(Max m, float y) { return m < y; }
+  __device__ static __forceinline__ void pair_floor(const uint4& v, int i, float& a, float& b) {
+    pair(v, i, a, b);
+    a = max_nan(a, kFloor);
+    b = max_nan(b, kFloor);
   }
   template <bool GE>
   __device__ static __forceinline__ void count(const uint4& v, float y, uint32_t& acc) {
@@ -184,6 +223,78 @@ struct Row {
   }
 };
 
+// Part `part` of `parts` of a row's vectors: [lo, hi), of which [a, b) are
+// full; the row's first and last vector, where they are partial and here (-1
+// otherwise), belong to threads 0 and 1.
+struct Slice {
+  int lo, hi, a, b, head, tail;
+  template <typename T>
+  __device__ __forceinline__ Slice(const Row<T>& row, int part, int parts) {
+    const int per = (row.n_vec + parts - 1) / parts;
+    lo = min(part * per, row.n_vec);
+    hi = min(lo + per, row.n_vec);
+    const int full_hi = row.full_lo + (int)row.n_full;
+    a = max(lo, row.full_lo);
+    b = max(a, min(hi, full_hi));
+    head = lo == 0 && hi > 0 && row.full_lo > 0 ? 0 : -1;
+    tail = hi == row.n_vec && hi > lo && hi > full_hi && hi - 1 != head ? hi - 1 : -1;
+  }
+};
+
+// Calls f(v, u0, it) for groups it = 0 .. of U vectors of this thread, those of
+// vectors u0 + k NT; vectors past the end are -inf. The partial vectors make a
+// last group, of warp 0 alone. The next group's loads are out while one is
+// worked on. Full groups run without checks: at the rate HBM
+// delivers, an SM has some ten issue slots an element.
+template <int NT, int U, typename T, typename F>
+__device__ __forceinline__ void for_groups(const Row<T>& row, const Slice& s, F&& f) {
+  const uint4 none = make_uint4(Traits<T>::kNegInf, Traits<T>::kNegInf, Traits<T>::kNegInf,
+                                Traits<T>::kNegInf);
+  const int tid = threadIdx.x, n = s.b - s.a;
+  const uint4* p = reinterpret_cast<const uint4*>(row.x - row.pad) + s.a + tid;
+  uint4 v[U];
+  int left = n, u = s.a + tid, it = 0;
+  if (left >= U * NT) {
+#pragma unroll
+    for (int k = 0; k < U; ++k) v[k] = ldg_stream(p + k * NT);
+#pragma unroll 2
+    while (left >= 2 * U * NT) {
+      uint4 w[U];
+      p += U * NT;
+#pragma unroll
+      for (int k = 0; k < U; ++k) w[k] = ldg_stream(p + k * NT);
+      f(v, u, it++);
+      u += U * NT;
+      left -= U * NT;
+#pragma unroll
+      for (int k = 0; k < U; ++k) v[k] = w[k];
+    }
+    p += U * NT;
+    left -= U * NT;
+    if (left > 0) {
+      uint4 w[U];
+#pragma unroll
+      for (int k = 0; k < U; ++k) w[k] = tid + k * NT < left ? ldg_stream(p + k * NT) : none;
+      f(v, u, it++);
+#pragma unroll
+      for (int k = 0; k < U; ++k) v[k] = w[k];
+      u += U * NT;
+    }
+    f(v, u, it++);
+  } else if (left > 0) {
+#pragma unroll
+    for (int k = 0; k < U; ++k) v[k] = tid + k * NT < left ? ldg_stream(p + k * NT) : none;
+    f(v, u, it++);
+  }
+  if ((s.head >= 0 || s.tail >= 0) && tid < 32) {
+    const int e = tid == 0 ? s.head : tid == 1 ? s.tail : -1;
+#pragma unroll
+    for (int k = 0; k < U; ++k) v[k] = none;
+    if (e >= 0) v[0] = row.load(e);
+    f(v, e >= 0 ? e : row.n_vec, it);
+  }
+}
+
 __device__ __forceinline__ int64_t load_id(const void* ids, bool ids64, int64_t row) {
   return ids64 ? reinterpret_cast<const int64_t*>(ids)[row]
                : (int64_t) reinterpret_cast<const int*>(ids)[row];
@@ -196,7 +307,7 @@ __device__ __forceinline__ uint64_t f32x2_mul(uint64_t a, uint64_t b) {
 }
 
 // Running sums of a thread, a CTA or a cluster: m = max x, s = sum 2^((x - m) c),
-// t = sum 2^((x - m) c) (x - m). Empty: m = -inf, s = t = 0.
+// t = sum 2^((x - m) c) (x - m) c. Empty: m = -inf, s = t = 0.
 struct Acc {
   float m, s, t;
 };
@@ -206,8 +317,8 @@ __device__ __forceinline__ float shift_of(float m) { return m == -INFINITY ? 0.f
 __device__ __forceinline__ void rebase(Acc& a, float m, float c) {
   if (a.m == m) return;
   if (a.m != -INFINITY) {
-    const float d = a.m - m;
-    const float f = ex2(d * c);
+    const float d = (a.m - m) * c;
+    const float f = ex2(d);
     a.t = f == 0.f ? 0.f : f * (a.t + d * a.s);
     a.s *= f;
   }

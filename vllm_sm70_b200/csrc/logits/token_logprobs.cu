@@ -12,11 +12,14 @@
 // One pass. A CTA (or a cluster of 2 to 8 when there are few rows) streams a
 // row once and keeps per thread: the maximum, the two base-2 sums of rows.cuh
 // and the count of elements before y. The alternatives need no second pass
-// over the row: the n-th largest of the THREADS' maxima, tau, is a lower bound
-// of the row's n-th largest value (n threads hold an element that large), so
-// every alternative is an element >= tau of a thread whose maximum is >= tau.
-// About n threads qualify; only their elements are read again (from L2), and
-// the few above tau are ranked by counting. Elements equal to tau enter by
+// over the row: a value tau that the maxima of n THREADS reach is a lower
+// bound of the row's n-th largest value, so every alternative is an element
+// >= tau of a thread whose maximum is >= tau. With j = ceil(n / warps), tau is
+// the ceil(n / j)-th largest of the warps' j-th largest maxima: each warp
+// finds its own with j warp reductions, no bisection over the whole CTA. A
+// thread also leaves the maximum of each of its groups of vectors in shared
+// memory: the some n to 2 n groups that reach tau are all that is read again
+// (from L2), and the few elements above tau are ranked by counting. Elements equal to tau enter by
 // lowest id. Rows where too many elements pass (values that cluster in few
 // threads) raise tau to the exact n-th largest value by bisection first.
 #include <cuda_bf16.h>
@@ -36,11 +39,13 @@ namespace {
 
 using namespace rows;
 
-constexpr int NT = 512;
+constexpr int NT = 256;
 constexpr int kWarps = NT / 32;
-constexpr int U = 4;          // vectors of a thread in flight
+constexpr int U = 4;          // vectors of a thread worked on at a time
 constexpr int kCand = 512;    // elements above tau kept before tau is raised
 constexpr int kEq = 256;      // elements equal to tau kept before they are found in id order
+constexpr int kHits = 512;    // groups read again by themselves; more: the whole slice
+constexpr int kSlots = 64;    // maxima of groups kept a thread
 constexpr int kMaxCluster = 8;
 
 struct FwdParams {
@@ -49,6 +54,7 @@ struct FwdParams {
   int64_t ld;
   int V, top_n;
   bool ids64;
+  int shift;       // groups of a slot, as a power of two
   float c, inv_t;  // log2(e) / T, 1 / T
   float* logprob;
   int* rank;
@@ -60,16 +66,14 @@ struct FwdParams {
 };
 
 struct Smem {
-  float red[kWarps];
   Acc acc[kWarps];
   int cnt[kWarps];
-  uint32_t tmax[NT];           // key of each thread's maximum
-  int qual[NT];                // threads with elements >= tau
+  uint32_t jth[kWarps];        // each warp's j-th largest maximum
+  int hit[kHits];              // slot * NT + thread of groups that reach tau
   unsigned long long cand[kCand + kEq];
   int eq[kEq];
   int scan[kWarps];
-  int n_qual, n_gt, n_eq, n_hit;
-  uint32_t tau;
+  int n_hit, n_gt, n_eq, n_at;
   float m, log2_s;
   // filled by the CTAs of the cluster in rank 0's copy
   Acc part[kMaxCluster];
@@ -82,44 +86,34 @@ __device__ __forceinline__ unsigned long long entry(uint32_t key, int id) {
   return ((unsigned long long)key << 32) | (uint32_t)~(uint32_t)id;
 }
 
-// Largest key k with at least n of the CTA's thread maxima >= k (n <= NT).
-// Warp 0 bisects over the key's bits with 16 maxima a lane in registers.
-template <typename T>
-__device__ void find_tau(Smem& sm, int n) {
-  if (threadIdx.x < 32) {
-    uint32_t k[kWarps];
+// The key that n of the CTA's thread maxima reach (see the head of this file),
+// from the warps' j-th largest in sm.jth.
+__device__ __forceinline__ uint32_t find_tau(const Smem& sm, int n) {
+  const int j = (n + kWarps - 1) / kWarps, need = (n + j - 1) / j;
+  const uint32_t k = sm.jth[threadIdx.x % kWarps];
+  int reach = 0;
 #pragma unroll
-    for (int i = 0; i < kWarps; ++i) k[i] = sm.tmax[i * 32 + threadIdx.x];
-    uint32_t tau = 0;
-    for (int b = 31; b >= Traits<T>::kKeyLowBit; --b) {
-      const uint32_t cand = tau | (1u << b);
-      int c = 0;
-#pragma unroll
-      for (int i = 0; i < kWarps; ++i) c += k[i] >= cand ? 1 : 0;
-      c = __reduce_add_sync(0xffffffffu, c);
-      if (c >= n) tau = cand;
-      if (c == n) break;  // any bound that n maxima reach will do
-    }
-    // The bound as a key that an element can have: the smallest maximum
-    // above it, so that "equal to tau" means something.
-    uint32_t low = 0xffffffffu;
-#pragma unroll
-    for (int i = 0; i < kWarps; ++i)
-      if (k[i] >= tau) low = min(low, k[i]);
-    low = __reduce_min_sync(0xffffffffu, low);
-    if (threadIdx.x == 0) sm.tau = low;
-  }
-  __syncthreads();
+  for (int i = 0; i < kWarps; ++i) reach += sm.jth[i] >= k ? 1 : 0;
+  return __reduce_max_sync(0xffffffffu, reach >= need ? k : 0u);
 }
 
-// Calls f(key, id) for every element of the qualified threads' vectors.
+// Calls f(key, id) for every element of the groups in sm.hit.
 template <typename T, typename F>
-__device__ __forceinline__ void visit_qualified(const Smem& sm, const Row<T>& row, int u_lo,
-                                                int u_hi, F f) {
-  const int per = (u_hi - u_lo + NT - 1) / NT;  // vectors of a thread, at most
-  for (int w = threadIdx.x; w < sm.n_qual * per; w += NT) {
-    const int u = u_lo + sm.qual[w / per] + (w % per) * NT;
-    if (u >= u_hi) continue;
+__device__ __forceinline__ void visit(const Smem& sm, const Row<T>& row, const Slice& sl,
+                                      int shift, F f) {
+  const int n_groups = (sl.b - sl.a + U * NT - 1) / (U * NT);
+  const bool all = sm.n_hit > kHits;
+  const int n = all ? sl.hi - sl.lo : (sm.n_hit * U) << shift;
+  for (int w = threadIdx.x; w < n; w += NT) {
+    int u = sl.lo + w;
+    if (!all) {
+      const int h = sm.hit[(w / U) >> shift];
+      const int it = ((h / NT) << shift) + ((w / U) & ((1 << shift) - 1)), k = w % U, t = h % NT;
+      u = sl.a + (it * U + k) * NT + t;
+      if (it == n_groups) u = k > 0 ? -1 : t == 0 ? sl.head : t == 1 ? sl.tail : -1;
+      else if (u >= sl.b) u = -1;
+      if (u < 0) continue;
+    }
     const uint4 v = row.load(u);
 #pragma unroll
     for (int i = 0; i < Traits<T>::E / 2; ++i) {
@@ -136,14 +130,9 @@ __device__ __forceinline__ void visit_qualified(const Smem& sm, const Row<T>& ro
 // the ids of those equal to it into sm.eq (up to kEq; sm.n_eq counts them).
 // The order in which they arrive does not matter: the lists are ranked.
 template <typename T>
-__device__ void collect(Smem& sm, const Row<T>& row, int u_lo, int u_hi) {
-  const uint32_t tau = sm.tau;
-  __syncthreads();
-  if (threadIdx.x == 0) sm.n_qual = sm.n_gt = sm.n_eq = 0;
-  __syncthreads();
-  if (sm.tmax[threadIdx.x] >= tau) sm.qual[atomicAdd(&sm.n_qual, 1)] = threadIdx.x;
-  __syncthreads();
-  visit_qualified(sm, row, u_lo, u_hi, [&](uint32_t k, int id) {
+__device__ __forceinline__ void collect(Smem& sm, const Row<T>& row, const Slice& sl, int shift,
+                                        uint32_t tau) {
+  visit(sm, row, sl, shift, [&](uint32_t k, int id) {
     if (k > tau) {
       const int at = atomicAdd(&sm.n_gt, 1);
       if (at < kCand) sm.cand[at] = entry(k, id);
@@ -155,26 +144,26 @@ __device__ void collect(Smem& sm, const Row<T>& row, int u_lo, int u_hi) {
   __syncthreads();
 }
 
-// Exact n-th largest key among the qualified threads' elements (more than n
-// of them lie above the present tau).
+// Exact n-th largest key among the elements of the groups in sm.hit (more
+// than n of them lie above the present tau).
 template <typename T>
-__device__ void raise_tau(Smem& sm, const Row<T>& row, int u_lo, int u_hi, int n) {
+__device__ __noinline__ uint32_t raise_tau(Smem& sm, Row<T> row, Slice sl, int shift, int n) {
   uint32_t tau = 0;
   for (int b = 31; b >= 0; --b) {
     const uint32_t cand = tau | (1u << b);
     __syncthreads();
-    if (threadIdx.x == 0) sm.n_hit = 0;
+    if (threadIdx.x == 0) sm.n_at = 0;
     __syncthreads();
     int c = 0;
-    visit_qualified(sm, row, u_lo, u_hi, [&](uint32_t k, int) { c += k >= cand ? 1 : 0; });
+    visit(sm, row, sl, shift, [&](uint32_t k, int) { c += k >= cand ? 1 : 0; });
     c = __reduce_add_sync(0xffffffffu, c);
-    if (threadIdx.x % 32 == 0 && c) atomicAdd(&sm.n_hit, c);
+    if (threadIdx.x % 32 == 0 && c) atomicAdd(&sm.n_at, c);
     __syncthreads();
-    if (sm.n_hit >= n) tau = cand;
+    if (sm.n_at >= n) tau = cand;
   }
+  if (threadIdx.x == 0) sm.n_gt = sm.n_eq = 0;
   __syncthreads();
-  if (threadIdx.x == 0) sm.tau = tau;
-  __syncthreads();
+  return tau;
 }
 
 // The lowest ids whose key is tau, up to `need` (<= kEq), into sm.eq[0 ..
@@ -182,14 +171,13 @@ __device__ void raise_tau(Smem& sm, const Row<T>& row, int u_lo, int u_hi, int n
 // rows where very many elements tie (a mask leaves fewer than n): there the
 // first vectors hold enough.
 template <typename T>
-__device__ void collect_equal(Smem& sm, const Row<T>& row, int u_lo, int u_hi, int need) {
-  const uint32_t tau = sm.tau;
+__device__ __noinline__ void collect_equal(Smem& sm, Row<T> row, Slice sl, uint32_t tau, int need) {
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   int found = 0;  // uniform
-  for (int u0 = u_lo; u0 < u_hi && found < need; u0 += NT) {
+  for (int u0 = sl.lo; u0 < sl.hi && found < need; u0 += NT) {
     const int u = u0 + threadIdx.x;
     uint32_t mask = 0;  // bit e: element e of my vector equals tau
-    if (u < u_hi) {
+    if (u < sl.hi) {
       const uint4 v = row.load(u);
 #pragma unroll
       for (int i = 0; i < Traits<T>::E / 2; ++i) {
@@ -228,9 +216,45 @@ __device__ void collect_equal(Smem& sm, const Row<T>& row, int u_lo, int u_hi, i
   __syncthreads();
 }
 
+// This thread's sums of a row whose maximum lies so far out that x c or the
+// floor would not do: element by element against its own maximum.
+template <typename T>
+__device__ __noinline__ Acc slow_sums(Row<T> row, int lo, int hi, float c) {
+  Acc a{-INFINITY, 0.f, 0.f};
+  for (int u = lo + threadIdx.x; u < hi; u += NT) {
+    const uint4 v = row.load(u);
+    const float mx = Traits<T>::max_of(v);
+    if (mx > a.m) rebase(a, mx, c);
+    const float m = shift_of(a.m);
+#pragma unroll
+    for (int i = 0; i < Traits<T>::E / 2; ++i) {
+      float x[2];
+      Traits<T>::pair(v, i, x[0], x[1]);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const float d = (x[k] - m) * c, e = ex2(d);
+        a.s += e;
+        a.t += e == 0.f ? 0.f : e * d;
+      }
+    }
+  }
+  return a;
+}
+
+// How many of list[0 .. n) are larger than e, for groups of 4 threads that
+// share an e; all of them get it.
+__device__ __forceinline__ int rank_of(const unsigned long long* list, int n,
+                                       unsigned long long e) {
+  int before = 0;
+  for (int j = threadIdx.x % 4; j < n; j += 4) before += list[j] > e ? 1 : 0;
+  before += __shfl_xor_sync(0xffffffffu, before, 1);
+  before += __shfl_xor_sync(0xffffffffu, before, 2);
+  return before;
+}
+
 // CL CTAs a row. TOP: alternatives wanted.
 template <typename T, int CL, bool TOP>
-__global__ void __launch_bounds__(NT, 2) token_logprobs_kernel(const FwdParams p) {
+__global__ void __launch_bounds__(NT, 4) token_logprobs_kernel(const FwdParams p) {
   using Tr = Traits<T>;
   constexpr int E = Tr::E;
   __shared__ Smem sm;
@@ -239,64 +263,94 @@ __global__ void __launch_bounds__(NT, 2) token_logprobs_kernel(const FwdParams p
   const int64_t r = blockIdx.x / CL;
   const int part = blockIdx.x % CL;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  const int n = p.top_n;
+  if (TOP && tid == 0) sm.n_hit = sm.n_gt = sm.n_eq = 0;
   // Every CTA of the cluster has started before its memory is written to.
   if constexpr (CL > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
 
   const Row<T> row(p.x, r, p.ld, p.V);
-  const int per = (row.n_vec + CL - 1) / CL;
-  const int u_lo = min(part * per, row.n_vec), u_hi = min(u_lo + per, row.n_vec);
+  const Slice sl(row, part, CL);
   const int64_t y = load_id(p.ids, p.ids64, r);
   const bool has_y = y >= 0 && y < p.V;
   const float xy = has_y ? Tr::to_f(row.x[y]) : NAN;
   const int uy = has_y ? ((int)y + row.pad) / E : 0x7fffffff;
   const float c = p.c;
 
-  Acc a{-INFINITY, 0.f, 0.f};
+  // Sums against r = the rounded m c of the thread's maximum m so far: one
+  // fused product an element. (rows.cuh's form follows at the end: r's own
+  // rounding is taken out of s and t.)
+  float m = -INFINITY, r0 = 0.f, s = 0.f, t = 0.f;
   uint32_t cnt = 0;
-  for (int u = u_lo + tid; u < u_hi; u += U * NT) {
-    uint4 v[U];
+  const uint64_t c2 = f32x2_pack(c, c);
+  // A given token at -inf ties with everything that is masked: those before
+  // it are counted on their own.
+  const bool y_masked = xy == -INFINITY;
+  extern __shared__ uint16_t slots[];
+  const int shift = p.shift;
+  float slot_max = -INFINITY;
+  int n_slots = 0;
+  for_groups<NT, U>(row, sl, [&](const uint4(&v)[U], int u, int it) {
+    typename Tr::Max vm[U];
 #pragma unroll
-    for (int k = 0; k < U; ++k) {
-      const int uk = u + k * NT;
-      v[k] = uk < u_hi ? row.load(uk)
-                       : make_uint4(Tr::kNegInf, Tr::kNegInf, Tr::kNegInf, Tr::kNegInf);
+    for (int k = 0; k < U; ++k) vm[k] = Tr::vmax(v[k]);
+    static_assert(U == 4, "tree of maxima");
+    const float mx = Tr::value(Tr::vmax(Tr::vmax(vm[0], vm[1]), Tr::vmax(vm[2], vm[3])));
+    if constexpr (TOP) {
+      // The upper half of the float keeps the order.
+      slot_max = (it & ((1 << shift) - 1)) == 0 ? mx : fmaxf(slot_max, mx);
+      slots[(it >> shift) * NT + tid] = (uint16_t)(__float_as_uint(slot_max) >> 16);
+      n_slots = (it >> shift) + 1;
     }
-    float mx = Tr::max_of(v[0]);
-#pragma unroll
-    for (int k = 1; k < U; ++k) mx = fmaxf(mx, Tr::max_of(v[k]));
-    if (mx > a.m) rebase(a, mx, c);
-    const float m = shift_of(a.m);
-    const uint64_t c2 = f32x2_pack(c, c), nm2 = f32x2_pack(-m, -m);
+    if (mx > m) {
+      const float rn = __fmul_rn(fmaxf(mx, kFloor), c), d = r0 - rn;
+      const float f = m == -INFINITY ? 0.f : ex2(d);
+      t = f == 0.f ? 0.f : f * (t + d * s);
+      s = f == 0.f ? 0.f * s : f * s;
+      m = mx;
+      r0 = rn;
+    }
+    const uint64_t nr2 = f32x2_pack(-r0, -r0);
     uint64_t s2 = f32x2_pack(0.f, 0.f), t2 = s2;
 #pragma unroll
     for (int k = 0; k < U; ++k) {
 #pragma unroll
       for (int i = 0; i < E / 2; ++i) {
-        float xa, xb, da, db, ea, eb;
-        Tr::pair(v[k], i, xa, xb);
-        const uint64_t d2 = f32x2_add(f32x2_pack(xa, xb), nm2);
-        f32x2_unpack(f32x2_mul(d2, c2), ea, eb);
-        const uint64_t e2 = f32x2_pack(ex2(ea), ex2(eb));
-        s2 = f32x2_add(s2, e2);
-        // -inf times a zero exponential is zero here
+        float xa, xb, da, db;
+        Tr::pair_floor(v[k], i, xa, xb);
+        const uint64_t d2 = f32x2_fma(f32x2_pack(xa, xb), c2, nr2);
         f32x2_unpack(d2, da, db);
-        t2 = f32x2_fma(e2, f32x2_pack(fmaxf(da, -1e30f), fmaxf(db, -1e30f)), t2);
+        const uint64_t e2 = f32x2_pack(ex2(da), ex2(db));
+        s2 = f32x2_add(s2, e2);
+        t2 = f32x2_fma(e2, d2, t2);
       }
+      // Elements before y: most vectors hold none above it.
       const int uk = u + k * NT;
-      if (uk < uy) {
-        Tr::template count<true>(v[k], xy, cnt);
-      } else if (uk > uy) {
-        Tr::template count<false>(v[k], xy, cnt);
+      if (!Tr::all_below(vm[k], xy)) {
+        if (uk < uy && !y_masked)
+          Tr::template count<true>(v[k], xy, cnt);
+        else if (uk != uy)
+          Tr::template count<false>(v[k], xy, cnt);
       }
     }
     float s0, s1, t0, t1;
     f32x2_unpack(s2, s0, s1);
     f32x2_unpack(t2, t0, t1);
-    a.s += s0 + s1;
-    a.t += t0 + t1;
-  }
+    s += s0 + s1;
+    t += t0 + t1;
+  });
   int n_before = Tr::counted(cnt);
-  if (has_y && uy >= u_lo && uy < u_hi && (uy - u_lo) % NT == tid) {
+  if (y_masked)
+    for (int u = sl.lo + tid; u < min(sl.hi, uy); u += NT) {
+      const uint4 v = row.load(u);
+      for (int i = 0; i < E / 2; ++i) {
+        float xa, xb;
+        Tr::pair(v, i, xa, xb);
+        const int id = row.index(u, 2 * i);
+        n_before += id >= 0 && id < p.V && xa == -INFINITY;
+        n_before += id + 1 >= 0 && id + 1 < p.V && xb == -INFINITY;
+      }
+    }
+  if (has_y && uy >= sl.lo && uy < sl.hi && (uy - sl.lo) % NT == tid) {
     // The vector that holds y, element by element.
     const uint4 v = row.load(uy);
     for (int i = 0; i < E / 2; ++i) {
@@ -308,11 +362,25 @@ __global__ void __launch_bounds__(NT, 2) token_logprobs_kernel(const FwdParams p
     }
   }
 
-  // The CTA's sums, in a fixed order.
-  const float own_max = a.m;
-  if constexpr (TOP) sm.tmax[tid] = key_of(own_max);
-  const float m = block_max<NT>(own_max, sm.red);
-  rebase(a, m, c);
+  // A warp's sums against its own maximum, in a fixed order.
+  const uint32_t key = key_of(m);
+  const uint32_t key_w = __reduce_max_sync(0xffffffffu, key);
+  const float m_w = value_of(key_w);
+  Acc a{m, s, t};
+  if (m_w >= kSlowBelow && m_w <= kSlowAbove) {
+    const float e = fmaf(m, c, -r0);  // what r lacks of m c
+    if (m >= kSlowBelow) {
+      a.t = (t - e * s) * ex2(-e);
+      a.s = s * ex2(-e);
+    } else {
+      a = Acc{-INFINITY, s != s ? s : 0.f, 0.f};  // nothing against the warp's maximum
+    }
+  } else if (m_w == -INFINITY) {
+    a = Acc{-INFINITY, s != s ? s : 0.f, 0.f};
+  } else {
+    a = slow_sums(row, sl.lo, sl.hi, c);
+  }
+  rebase(a, m_w, c);
   a.s = warp_sum(a.s);
   a.t = warp_sum(a.t);
   n_before = __reduce_add_sync(0xffffffffu, n_before);
@@ -320,95 +388,22 @@ __global__ void __launch_bounds__(NT, 2) token_logprobs_kernel(const FwdParams p
     sm.acc[warp] = a;
     sm.cnt[warp] = n_before;
   }
+  if constexpr (TOP) {
+    uint32_t left = key, jth = key_w;
+    for (int j = (n + kWarps - 1) / kWarps; j > 1; --j) {
+      if (lane == __ffs(__ballot_sync(0xffffffffu, left == jth)) - 1) left = 0u;
+      jth = __reduce_max_sync(0xffffffffu, left);
+    }
+    if (lane == 0) sm.jth[warp] = jth;
+  }
   __syncthreads();
 
-  // The CTA's first n elements: `n_local` entries of sm.cand.
-  int n_local = 0;
-  const int n = p.top_n;
-  if constexpr (TOP) {
-    find_tau<T>(sm, n);
-    collect(sm, row, u_lo, u_hi);
-    if (sm.n_gt > kCand) {
-      raise_tau(sm, row, u_lo, u_hi, n);
-      collect(sm, row, u_lo, u_hi);
-    }
-    const int n_gt = min(sm.n_gt, kCand);
-    const int need = max(0, n - n_gt);
-    if (need > 0) {
-      if (sm.n_eq > kEq) collect_equal(sm, row, u_lo, u_hi, need);
-      if (tid < sm.n_eq) sm.cand[n_gt + tid] = entry(sm.tau, sm.eq[tid]);
-      __syncthreads();
-    }
-    n_local = n_gt + (need > 0 ? sm.n_eq : 0);
-  }
-
-  unsigned long long* list = sm.cand;
-  int n_list = n_local;
-  if constexpr (CL > 1) {
-    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
-    if (tid == 0) {
-      Acc q = sm.acc[0];
-      int k = sm.cnt[0];
-      for (int w = 1; w < kWarps; ++w) {
-        q.s += sm.acc[w].s;
-        q.t += sm.acc[w].t;
-        k += sm.cnt[w];
-      }
-      const uint32_t dst = mapa_shared(smem_u32(&sm.part[part]), 0);
-      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(q.m) : "memory");
-      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + 4), "f"(q.s) : "memory");
-      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + 8), "f"(q.t) : "memory");
-      asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(
-                       mapa_shared(smem_u32(&sm.part_cnt[part]), 0)),
-                   "r"(k)
-                   : "memory");
-    }
-    if constexpr (TOP) {
-      // Its first n, by rank, into rank 0's list; empty places hold 0.
-      const uint32_t dst = mapa_shared(smem_u32(&sm.merged[part * kMaxTopN]), 0);
-      if (tid < n && tid >= n_local)
-        asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(dst + tid * 8), "l"(0ull) : "memory");
-      for (int i = tid; i < n_local; i += NT) {
-        const unsigned long long e = sm.cand[i];
-        int before = 0;
-        for (int j = 0; j < n_local; ++j) before += sm.cand[j] > e ? 1 : 0;
-        if (before < n)
-          asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(dst + before * 8), "l"(e)
-                       : "memory");
-      }
-    }
-    cluster_sync_all();
-    if (part != 0) return;
-  }
-
-  if (tid == 0) {
-    Acc q;
-    int k;
-    if constexpr (CL > 1) {
-      float mm = sm.part[0].m;
-      for (int i = 1; i < CL; ++i) mm = fmaxf(mm, sm.part[i].m);
-      q = Acc{mm, 0.f, 0.f};
-      k = 0;
-      for (int i = 0; i < CL; ++i) {
-        Acc b = sm.part[i];
-        rebase(b, mm, c);
-        q.s += b.s;
-        q.t += b.t;
-        k += sm.part_cnt[i];
-      }
-    } else {
-      q = sm.acc[0];
-      k = sm.cnt[0];
-      for (int w = 1; w < kWarps; ++w) {
-        q.s += sm.acc[w].s;
-        q.t += sm.acc[w].t;
-        k += sm.cnt[w];
-      }
-    }
+  // Warp 0 adds the warps up, and where the row is one CTA's, finishes it.
+  auto finish = [&](const Acc& q, int k) {
     const bool empty = q.m == -INFINITY && q.s == 0.f;  // nothing above -inf, no NaN
     const float m0 = shift_of(q.m);
     const float l2 = log2f(q.s);  // -inf for an empty row
-    const float ent = empty ? 0.f : (l2 - q.t / q.s * c) * kLn2;
+    const float ent = empty ? 0.f : (l2 - q.t / q.s) * kLn2;
     p.entropy[r] = ent;
     p.lse[r] = fmaf(m0, p.inv_t, l2 * kLn2);
     const float lp = empty ? -INFINITY : fmaf(xy - m0, p.inv_t, -l2 * kLn2);
@@ -418,43 +413,112 @@ __global__ void __launch_bounds__(NT, 2) token_logprobs_kernel(const FwdParams p
     p.stats[r] = make_float4(m0, inv, empty ? 0.f : l2, ent);
     sm.m = m0;
     sm.log2_s = empty ? INFINITY : l2;
+  };
+  if (warp == 0) {
+    Acc q = lane < kWarps ? sm.acc[lane] : Acc{-INFINITY, 0.f, 0.f};
+    rebase(q, value_of(__reduce_max_sync(0xffffffffu, key_of(q.m))), c);
+    q.s = warp_sum(q.s);
+    q.t = warp_sum(q.t);
+    const int k = __reduce_add_sync(0xffffffffu, lane < kWarps ? sm.cnt[lane] : 0);
+    if constexpr (CL == 1) {
+      if (lane == 0) finish(q, k);
+    } else {
+      asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+      if (lane == 0) {
+        const uint32_t dst = mapa_shared(smem_u32(&sm.part[part]), 0);
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(q.m) : "memory");
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + 4), "f"(q.s) : "memory");
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + 8), "f"(q.t) : "memory");
+        asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(
+                         mapa_shared(smem_u32(&sm.part_cnt[part]), 0)),
+                     "r"(k)
+                     : "memory");
+      }
+    }
+  } else if constexpr (CL > 1) {
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
   }
+
+  // The CTA's first n elements: `n_list` entries of sm.cand, those among them.
+  int n_list = 0;
   if constexpr (TOP) {
-    if constexpr (CL > 1) {
-      // Rank 0's list: CL runs of kMaxTopN places, n used in each.
-      list = sm.merged;
-      n_list = CL * kMaxTopN;
+    uint32_t tau = find_tau(sm, n);
+    if (key >= tau) {
+      const uint32_t tau_up = key_of(__uint_as_float(__float_as_uint(value_of(tau)) & 0xffff0000u));
+#pragma unroll 4
+      for (int i = 0; i < n_slots; ++i)
+        if (key_of(__uint_as_float((uint32_t)slots[i * NT + tid] << 16)) >= tau_up) {
+          const int at = atomicAdd(&sm.n_hit, 1);
+          if (at < kHits) sm.hit[at] = i * NT + tid;
+        }
     }
     __syncthreads();
-    const float m0 = sm.m, l2 = sm.log2_s;
-    // Places that no element fills (fewer than n numbers in the row).
-    if (tid < n) {
-      int have = n_list;
-      if constexpr (CL > 1) {
-        have = 0;
-        for (int q = 0; q < CL; ++q)
-          for (int j = 0; j < n; ++j) have += list[q * kMaxTopN + j] != 0 ? 1 : 0;
-      }
-      if (tid >= have) {
-        p.top_ids[r * n + tid] = -1;
-        p.top_lp[r * n + tid] = -INFINITY;
+    collect(sm, row, sl, shift, tau);
+    if (sm.n_gt > kCand) {
+      tau = raise_tau(sm, row, sl, shift, n);
+      collect(sm, row, sl, shift, tau);
+    }
+    const int n_gt = min(sm.n_gt, kCand);
+    n_list = n_gt;
+    if (n_gt < n) {
+      if (sm.n_eq > kEq) collect_equal(sm, row, sl, tau, n - n_gt);
+      const int n_eq = sm.n_eq;
+      if (tid < n_eq) sm.cand[n_gt + tid] = entry(tau, sm.eq[tid]);
+      n_list += n_eq;
+      __syncthreads();
+    }
+  }
+
+  if constexpr (CL > 1) {
+    if constexpr (TOP) {
+      // Its first n, by rank, into rank 0's list; empty places hold 0.
+      const uint32_t dst = mapa_shared(smem_u32(&sm.merged[part * kMaxTopN]), 0);
+      if (tid < n && tid >= n_list)
+        asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(dst + tid * 8), "l"(0ull) : "memory");
+      for (int i0 = 0; i0 < n_list; i0 += NT / 4) {
+        const int i = i0 + tid / 4;
+        const unsigned long long e = i < n_list ? sm.cand[i] : 0ull;
+        const int before = rank_of(sm.cand, n_list, e);
+        if (i < n_list && before < n && tid % 4 == 0)
+          asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(dst + before * 8), "l"(e)
+                       : "memory");
       }
     }
-    for (int i = tid; i < n_list; i += NT) {
-      if (CL > 1 && i % kMaxTopN >= n) continue;
-      const unsigned long long e = list[i];
-      if (CL > 1 && e == 0) continue;
-      int before = 0;
-      if constexpr (CL > 1) {
-        for (int q = 0; q < CL; ++q)
-          for (int j = 0; j < n; ++j) before += list[q * kMaxTopN + j] > e ? 1 : 0;
-      } else {
-        for (int j = 0; j < n_list; ++j) before += list[j] > e ? 1 : 0;
-      }
-      if (before < n) {
+    cluster_sync_all();
+    if (part != 0) return;
+    if (warp == 0) {
+      Acc q = lane < CL ? sm.part[lane] : Acc{-INFINITY, 0.f, 0.f};
+      rebase(q, value_of(__reduce_max_sync(0xffffffffu, key_of(q.m))), c);
+      q.s = warp_sum(q.s);
+      q.t = warp_sum(q.t);
+      const int k = __reduce_add_sync(0xffffffffu, lane < CL ? sm.part_cnt[lane] : 0);
+      if (lane == 0) finish(q, k);
+    }
+    if constexpr (TOP) {
+      // The CTAs' lists, closed up.
+      const int i = tid;
+      for (int j = i; j < CL * n; j += NT) sm.cand[j] = sm.merged[j / n * kMaxTopN + j % n];
+      n_list = CL * n;
+      __syncthreads();
+    }
+  }
+  if constexpr (TOP) {
+    // sm.m and sm.log2_s: written before the last barrier.
+    const float m0 = sm.m, l2 = sm.log2_s;
+    for (int i0 = 0; i0 < n_list; i0 += NT / 4) {
+      const int i = i0 + tid / 4;
+      const unsigned long long e = i < n_list ? sm.cand[i] : 0ull;
+      const int before = rank_of(sm.cand, n_list, e);
+      if (e != 0 && before < n && tid % 4 == 0) {
         p.top_ids[r * n + before] = (int)~(uint32_t)e;
         p.top_lp[r * n + before] = fmaf(value_of((uint32_t)(e >> 32)) - m0, p.inv_t, -l2 * kLn2);
       }
+    }
+    // Places that no element fills (fewer than n numbers in the row).
+    const int have = rank_of(sm.cand, n_list, 0ull);
+    if (tid < n && tid >= have) {
+      p.top_ids[r * n + tid] = -1;
+      p.top_lp[r * n + tid] = -INFINITY;
     }
   }
 }
@@ -546,24 +610,28 @@ __global__ void __launch_bounds__(NT) token_logprobs_bwd_kernel(const BwdParams 
 }
 
 template <typename T, int CL>
-void launch_fwd(const FwdParams& p, int64_t rows, cudaStream_t stream) {
+void launch_fwd(FwdParams p, int64_t rows, cudaStream_t stream) {
   cudaLaunchAttribute cl;
   cl.id = cudaLaunchAttributeClusterDimension;
   cl.val.clusterDim.x = CL;
   cl.val.clusterDim.y = cl.val.clusterDim.z = 1;
   const dim3 grid((unsigned)(rows * CL));
   const cudaLaunchAttribute* extra = CL > 1 ? &cl : nullptr;
-  if (p.top_n > 0)
-    launch_pdl(token_logprobs_kernel<T, CL, true>, grid, dim3(NT), 0, stream, extra, p);
-  else
-    launch_pdl(token_logprobs_kernel<T, CL, false>, grid, dim3(NT), 0, stream, extra, p);
+  auto kernel = p.top_n > 0 ? token_logprobs_kernel<T, CL, true> : token_logprobs_kernel<T, CL, false>;
+  // Groups of a thread, a last one for the partial vectors among them.
+  const int n_vec = (p.V + 2 * Traits<T>::E - 2) / Traits<T>::E;
+  const int groups = ((n_vec + CL - 1) / CL + U * NT - 1) / (U * NT) + 1;
+  p.shift = 0;
+  while ((groups - 1) >> p.shift >= kSlots) ++p.shift;
+  const int smem = p.top_n > 0 ? (((groups - 1) >> p.shift) + 1) * NT * 2 : 0;
+  launch_pdl(kernel, grid, dim3(NT), smem, stream, extra, p);
 }
 
 template <typename T>
 void launch_fwd_t(const FwdParams& p, int64_t rows, cudaStream_t stream) {
   int dev = 0;
   cudaGetDevice(&dev);
-  switch (row_split(rows, p.V / Traits<T>::E, num_sms(dev), NT)) {
+  switch (row_split(rows, p.V / Traits<T>::E, 2 * num_sms(dev), NT)) {
     case 1: return launch_fwd<T, 1>(p, rows, stream);
     case 2: return launch_fwd<T, 2>(p, rows, stream);
     case 4: return launch_fwd<T, 4>(p, rows, stream);
@@ -585,7 +653,7 @@ void token_logprobs_launch(const TokenLogprobsArgs& a, cudaStream_t stream) {
     throw std::runtime_error("token_logprobs: top_n must be in [0, min(64, vocabulary)]");
   if (a.in.rows <= 0) return;
   FwdParams p{a.in.x,  a.ids,       a.in.ld,    a.in.V,
-              a.top_n, a.ids64,     (float)(1.4426950408889634 / a.temperature), (float)(1.0 / a.temperature),
+              a.top_n, a.ids64,     0, (float)(1.4426950408889634 / a.temperature), (float)(1.0 / a.temperature),
               a.logprob, a.rank,    a.entropy,  a.lse,
               a.top_ids, a.top_lp,  reinterpret_cast<float4*>(a.stats)};
   if (a.in.bf16)
