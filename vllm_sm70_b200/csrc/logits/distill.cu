@@ -9,39 +9,49 @@
 //                                       over repeated ids), M = sum p_k + p_t
 //           = (M - p_t / q_t) q_j       other j
 // q_t is the sum over the other j themselves (never 1 - sum q_k, which would
-// cancel for a student that agrees with its teacher): a bitmap of the row's
-// teacher ids in shared memory leaves them out of the streamed sum, and their
-// K exponentials are added on their own.
+// cancel for a student that agrees with its teacher): the row's teacher ids
+// are left out of the sum, and their K exponentials are added on their own.
 //
 // A row with weight 0 has loss 0 and gradient 0 whatever it holds, and is not
 // read. Ids outside [0, V) are absent: their mass joins the tail.
 //
-// Bound: bytes. The training form computes loss and gradient in one kernel: a
-// cluster of CTAs shares a row, each streams its slice once for the sums and
-// keeps as much of it as fits in shared memory; after one exchange of the
-// sums within the cluster the gradient is written from there.
+// Bound: bytes. The training form computes loss and gradient in one kernel:
+// the logits are read once, the gradient written once.
+//   * A cluster of 1 to 8 CTAs holds a row in shared memory, at most 64 KB a
+//     CTA so that three share an SM (at 8 CTAs a row as much as an SM has).
+//     A warp copies its own part of the row with asynchronous copies, takes
+//     out the teacher's elements (they read as -inf from then on), and sums
+//     the rest; the warps of the whole cluster exchange (max, sums) through
+//     each other's shared memory at the row's only barrier. Then each warp
+//     writes its part of the gradient, and as it is done with a vector starts
+//     the copy of the next row's into its place: the clusters are persistent
+//     and memory is read while they work.
+//   * Rows too long for that (more than 8 CTAs' shared memory) and calls
+//     without gradient stream the row; a bitmap of the teacher's ids leaves
+//     them out of the sum.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
 #include <stdexcept>
 #include <string>
+#include <type_traits>
 
 #include "common/launch.h"
 #include "common/tmap.h"
 #include "logits/logits_api.h"
 #include "logits/rows.cuh"
+#include "ops_api.h"
 
 namespace b200 {
 namespace {
 
 using namespace rows;
 
-constexpr int NT = 512;
+constexpr int NT = 256;
 constexpr int kWarps = NT / 32;
 constexpr int U = 4;
 constexpr int kMaxCluster = 8;
-constexpr int K_ = kMaxTeacherK;
 
 struct Params {
   const void* x;
@@ -49,105 +59,562 @@ struct Params {
   const float* t_lp;
   const float* weights;
   int64_t ld;
-  int V, K, keep;  // keep: vectors of a thread held in shared memory
+  int V, K;
+  int64_t rows;
   bool tail;
   float c, inv_t, gscale;  // log2(e) / T; 1 / T; upstream gradient / T of a row of weight 1
   float* row_loss;
   float4* stats;
   void* grad;
+  unsigned int* err;
 };
 
-struct Smem {
-  float red[kWarps];
-  float2 sum[kWarps];
-  int id[K_];        // teacher ids, -1 absent
-  float p[K_];       // teacher probabilities
-  float lp[K_];
-  float xk[K_];      // student logits at the ids
-  int dup;           // some id of this slice is there twice
-  float4 row;        // m, M / s, outside coefficient, 1 (0: empty row)
-  float4 part[kMaxCluster];  // a slice's max, sum outside, sum at the ids
-};
+constexpr int kIds = kMaxTeacherK / 32;  // teacher entries a lane holds
 
-// The teacher's side of a row into shared memory: threads 0 .. K - 1.
-// Returns nothing; ends with a __syncthreads.
-__device__ void load_teacher(Smem& sm, const Params& p, int64_t r) {
-  const int k = threadIdx.x;
-  if (k < p.K) {
-    const int id = p.t_ids[r * p.K + k];
-    sm.id[k] = id >= 0 && id < p.V ? id : -1;
-    sm.lp[k] = p.t_lp[r * p.K + k];
-  }
-  __syncthreads();
-  if (!p.tail) {
-    // renormalise over the ids that are present
-    float mx = -INFINITY, z = 0.f;
-    for (int j = 0; j < p.K; ++j)
-      if (sm.id[j] >= 0) mx = fmaxf(mx, sm.lp[j]);
-    for (int j = 0; j < p.K; ++j)
-      if (sm.id[j] >= 0) z += expf(sm.lp[j] - mx);
-    __syncthreads();
-    if (k < p.K) sm.lp[k] = sm.lp[k] - mx - logf(z);
-  }
-  if (k < p.K) sm.p[k] = sm.id[k] >= 0 ? expf(sm.lp[k]) : 0.f;
-  __syncthreads();
-}
+// A row's teacher: entry lane + 32 i in every warp's registers.
+struct Teacher {
+  int id[kIds];      // -1: absent
+  float lp[kIds], p[kIds];
+  float norm, sum_p;  // subtracted from the given log-probs; sum of p
 
-// Whether teacher entry k is the first with its id, and P there: the p of
-// every entry with that id.
-__device__ __forceinline__ bool first_of_id(const Smem& sm, int K, int k, float& mass) {
-  mass = sm.p[k];
-  if (!sm.dup) return true;
-  const int id = sm.id[k];
-  float m = 0.f;
-  for (int j = 0; j < K; ++j)
-    if (sm.id[j] == id) {
-      if (j < k) return false;
-      m += sm.p[j];
+  __device__ __forceinline__ void load(const int* ids, const float* lps, int K) {
+#pragma unroll
+    for (int i = 0; i < kIds; ++i) {
+      const int k = threadIdx.x % 32 + 32 * i;
+      id[i] = k < K ? ids[k] : -1;
+      lp[i] = k < K ? lps[k] : -INFINITY;
     }
-  mass = m;
-  return true;
+  }
+  // Ids outside the vocabulary are absent; without a tail the rest is
+  // renormalised.
+  __device__ __forceinline__ void prepare(const Params& q) {
+    norm = sum_p = 0.f;
+#pragma unroll
+    for (int i = 0; i < kIds; ++i)
+      if (id[i] >= q.V) id[i] = -1;
+    if (!q.tail) {
+      float mx = -INFINITY, z = 0.f;
+#pragma unroll
+      for (int i = 0; i < kIds; ++i)
+        if (id[i] >= 0) mx = fmaxf(mx, lp[i]);
+      mx = warp_max(mx);
+#pragma unroll
+      for (int i = 0; i < kIds; ++i)
+        if (32 * i < q.K && id[i] >= 0) z += expf(lp[i] - mx);
+      norm = mx + logf(warp_sum(z));
+    }
+#pragma unroll
+    for (int i = 0; i < kIds; ++i) {
+      p[i] = 0.f;
+      if (32 * i < q.K) {
+        if (id[i] >= 0) p[i] = expf(lp[i] -= norm);
+        sum_p += p[i];
+      }
+    }
+    sum_p = warp_sum(sum_p);
+  }
+  // The p of all entries with entry (lane, i)'s id; -1 at those that are not
+  // the first of theirs. For all lanes of a warp.
+  __device__ __forceinline__ void masses(int K, float (&mass)[kIds]) const {
+    const int lane = threadIdx.x % 32;
+#pragma unroll
+    for (int i = 0; i < kIds; ++i) mass[i] = 0.f;
+    for (int k = 0; k < K; ++k) {
+      int idk = -1;
+      float pk = 0.f;
+#pragma unroll
+      for (int i = 0; i < kIds; ++i)
+        if (k / 32 == i) {
+          idk = __shfl_sync(0xffffffffu, id[i], k % 32);
+          pk = __shfl_sync(0xffffffffu, p[i], k % 32);
+        }
+#pragma unroll
+      for (int i = 0; i < kIds; ++i)
+        if (id[i] == idk && mass[i] != -1.f) {
+          if (k < lane + 32 * i)
+            mass[i] = -1.f;
+          else
+            mass[i] += pk;
+        }
+    }
+  }
+};
+
+// Which of a lane's entries (bit i: entry lane + 32 i) are the first of their
+// id, with kDup set.
+constexpr uint32_t kDup = 1u << 31;
+__device__ __noinline__ uint32_t first_of_ids(uint32_t own, const int* ids, int K) {
+  for (int i = 0; i < kIds; ++i)
+    if ((own >> i) & 1u)
+      for (int k = 0; k < (int)threadIdx.x % 32 + 32 * i; ++k)
+        if (ids[k] == ids[threadIdx.x % 32 + 32 * i]) own &= ~(1u << i);
+  return own | kDup;
+}
+// The p of all entries with this id.
+__device__ __noinline__ float mass_of_id(int id, const int* ids, const float* p, int K) {
+  float m = 0.f;
+  for (int k = 0; k < K; ++k)
+    if (ids[k] == id) m += p[k];
+  return m;
 }
 
-// Gradient of the elements of one vector, all taken as outside ones: g =
-// coef * 2^((x - m) c). coef 0 leaves exact zeros (-inf logits included).
-template <typename T>
-__device__ __forceinline__ uint4 grad_vec(const uint4& v, float c, float m, float coef) {
+// The slices' or warps' sums (max, sum outside, sum at the ids), two a lane,
+// against the largest max.
+__device__ __forceinline__ float3 join(const float4& a, const float4& b, float c) {
+  const float m = warp_max(fmaxf(a.x, b.x));
+  // a part without any element above -inf has no sums to rebase
+  const float fa = a.x == -INFINITY || a.x == m ? 1.f : ex2((a.x - m) * c);
+  const float fb = b.x == -INFINITY || b.x == m ? 1.f : ex2((b.x - m) * c);
+  return make_float3(m, warp_sum(a.y * fa + b.y * fb), warp_sum(a.z * fa + b.z * fb));
+}
+
+// The row's numbers: m, M / s, the coefficient of the elements outside, the
+// teacher's normaliser. M / s is 0 for a row without a distribution.
+__device__ __forceinline__ float4 row_numbers(float norm, float sum_p, bool tail, float3 q) {
+  const float s = q.y + q.z, p_t = tail ? fmaxf(0.f, 1.f - sum_p) : 0.f;
+  const float mass = sum_p + p_t, inv = s == 0.f ? 0.f : 1.f / s;
+  // A student with no mass outside has q_j = 0 there.
+  const float ratio = p_t > 0.f && q.y != 0.f ? p_t * s / q.y : 0.f;
+  return make_float4(shift_of(q.x), mass * inv, q.y == 0.f ? 0.f : (mass - ratio) * inv, norm);
+}
+
+// The row's loss, on a whole warp; xk: the student's logits at the ids.
+__device__ __forceinline__ float row_loss(const Teacher& t, const Params& p, float3 q,
+                                          const float (&xk)[kIds]) {
+  const float s = q.y + q.z, m0 = shift_of(q.x);
+  // An empty row: every log q is -inf, the loss inf where the teacher has mass.
+  const float l2 = s == 0.f ? 0.f : log2f(s);
+  float loss = 0.f;
+#pragma unroll
+  for (int i = 0; i < kIds; ++i) {
+    const float pk = t.p[i];
+    if (pk > 0.f)
+      loss += pk * (t.lp[i] - fmaf(xk[i] - m0, p.inv_t, -l2 * kLn2));
+    else if (pk != pk)
+      loss = pk;
+  }
+  loss = warp_sum(loss);
+  const float p_t = p.tail ? fmaxf(0.f, 1.f - t.sum_p) : 0.f;
+  if (p_t > 0.f) loss += p_t * (logf(p_t) - (log2f(q.y) - l2) * kLn2);
+  return loss;
+}
+
+// 2^((x - m) c) of a vector, times coef, for the gradient. kSlow: (x - m)
+// rounded by itself; otherwise one fused product against r = the rounded m c,
+// whose rounding the caller has put into coef (see rows.cuh).
+template <typename T, bool kSlow>
+__device__ __forceinline__ uint4 grad_vec(const uint4& v, float c, float m_or_r, float coef) {
   using Tr = Traits<T>;
   float g[Tr::E];
-  const uint64_t c2 = f32x2_pack(c, c), nm2 = f32x2_pack(-m, -m);
+  const uint64_t c2 = f32x2_pack(c, c), n2 = f32x2_pack(-m_or_r, -m_or_r),
+                 k2 = f32x2_pack(coef, coef);
 #pragma unroll
   for (int i = 0; i < Tr::E / 2; ++i) {
     float a, b, da, db;
     Tr::pair(v, i, a, b);
-    f32x2_unpack(f32x2_mul(f32x2_add(f32x2_pack(a, b), nm2), c2), da, db);
-    g[2 * i] = ex2(da) * coef;
-    g[2 * i + 1] = ex2(db) * coef;
+    const uint64_t x2 = f32x2_pack(a, b);
+    f32x2_unpack(kSlow ? f32x2_mul(f32x2_add(x2, n2), c2) : f32x2_fma(x2, c2, n2), da, db);
+    f32x2_unpack(f32x2_mul(f32x2_pack(ex2(da), ex2(db)), k2), g[2 * i], g[2 * i + 1]);
   }
   return Tr::pack(g);
 }
 
+// Whether m c can be taken apart from x c.
+__device__ __forceinline__ bool slow_range(float m) { return !(m >= kSlowBelow && m <= kSlowAbove); }
+
+// The elements of vector u that the row has, one by one.
 template <typename T>
-__device__ __forceinline__ void store_vec(T* out, const Row<T>& row, int u, const uint4& v) {
+__device__ __forceinline__ void store_part(T* out, const Row<T>& row, int u, const uint4& v) {
   constexpr int E = Traits<T>::E;
   const int id0 = row.index(u, 0);
-  T* dst = out + id0;
-  if (row.full(u) && (reinterpret_cast<uintptr_t>(dst) & 15u) == 0) {
-    *reinterpret_cast<uint4*>(dst) = v;
-  } else {
-    const T* e = reinterpret_cast<const T*>(&v);
+  const T* e = reinterpret_cast<const T*>(&v);
 #pragma unroll
-    for (int i = 0; i < E; ++i)
-      if (id0 + i >= 0 && id0 + i < row.V) dst[i] = e[i];
+  for (int i = 0; i < E; ++i)
+    if (id0 + i >= 0 && id0 + i < row.V) out[id0 + i] = e[i];
+}
+template <typename T>
+__device__ __forceinline__ void store_vec(T* out, const Row<T>& row, int u, const uint4& v) {
+  T* dst = out + row.index(u, 0);
+  if (row.full(u) && (reinterpret_cast<uintptr_t>(dst) & 15u) == 0)
+    *reinterpret_cast<uint4*>(dst) = v;
+  else
+    store_part(out, row, u, v);
+}
+
+// This thread's part of a streamed slice's sum, against m, element by element.
+template <typename T>
+__device__ __noinline__ float slow_sum(Row<T> row, Slice sl, const uint8_t* bitmap, float m,
+                                       float c) {
+  float s = 0.f;
+  for (int u = sl.lo + threadIdx.x; u < sl.hi; u += NT) {
+    uint4 v = row.load(u);
+    Traits<T>::blank(v, bitmap[u - sl.lo]);
+    for (int i = 0; i < Traits<T>::E / 2; ++i) {
+      float a, b;
+      Traits<T>::pair(v, i, a, b);
+      s += ex2((a - m) * c) + ex2((b - m) * c);
+    }
+  }
+  return s;
+}
+
+// A value and the number of the exchange that it belongs to, as one 8-byte
+// word: who sees the number sees the value, so no fence is needed (one would
+// wait for the gradient's stores).
+__device__ __forceinline__ unsigned long long word_of(float v, uint32_t seq) {
+  return ((unsigned long long)seq << 32) | __float_as_uint(v);
+}
+template <int CL>
+__device__ __forceinline__ void send(unsigned long long* to, int rank, float v, uint32_t seq) {
+  if constexpr (CL == 1)
+    *reinterpret_cast<volatile unsigned long long*>(to) = word_of(v, seq);
+  else
+    asm volatile("st.relaxed.cluster.shared::cluster.b64 [%0], %1;" ::"r"(
+                     mapa_shared(smem_u32(to), rank)),
+                 "l"(word_of(v, seq))
+                 : "memory");
+}
+// Waits for the word of exchange `seq` (2 s at most, see mbar_wait); false
+// where it does not come.
+__device__ __forceinline__ bool receive(unsigned long long* from, uint32_t seq, float& v,
+                                        unsigned int* err) {
+  unsigned long long t0 = 0;
+  for (uint32_t spins = 0;; ++spins) {
+    unsigned long long q;
+    asm volatile("ld.relaxed.cluster.shared::cta.b64 %0, [%1];" : "=l"(q) : "r"(smem_u32(from)) : "memory");
+    v = __uint_as_float((uint32_t)q);
+    if ((uint32_t)(q >> 32) == seq) return true;
+    if ((spins & 63u) == 63u) {
+      if (t0 == 0) t0 = globaltimer();
+      if (globaltimer() - t0 > kWaitTimeoutNs) {
+        atomicCAS(err, kErrNone, kErrMbarTimeout);
+        return false;
+      }
+      if (*(volatile unsigned int*)err != kErrNone) return false;
+    }
   }
 }
 
+// Vectors of a warp, of `per` a CTA: whole steps of 32 lanes.
+__host__ __device__ __forceinline__ int warp_vectors(int per) {
+  return (per + 32 * kWarps - 1) / (32 * kWarps) * 32;
+}
+
+// Loss and gradient of rows held in shared memory: CL CTAs a row, cluster
+// blockIdx.x / CL takes rows blockIdx.x / CL + i * gridDim.x / CL.
+template <typename T, int CL>
+__global__ void __launch_bounds__(NT, 3) distill_fused_kernel(const Params p) {
+  using Tr = Traits<T>;
+  using Tag = std::conditional_t<sizeof(T) == 2, uint16_t, uint32_t>;
+  constexpr int E = Tr::E;
+  // What the warps send one another, and a row's teacher: every warp writes
+  // the same there, so none waits for another to read it. Two rows' worth: a
+  // warp that has the sums of a row knows that all others are done with the
+  // row before, and only then writes over that.
+  __shared__ unsigned long long parts[2][3][CL * kWarps];
+  __shared__ unsigned long long xks[2][kMaxTeacherK];  // in the cluster's first CTA
+  __shared__ uint64_t bar[2];
+  __shared__ int t_id[2][kMaxTeacherK];  // as given
+  __shared__ float t_lp[2][kMaxTeacherK];
+  __shared__ float t_p[2][kMaxTeacherK], t_x[2][kMaxTeacherK];
+  extern __shared__ __align__(16) uint8_t dyn[];
+  uint4* kept = reinterpret_cast<uint4*>(dyn);
+  const int part = blockIdx.x % CL, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  if (threadIdx.x == 0) {
+    mbar_init(&bar[0], CL * kWarps);
+    mbar_init(&bar[1], CL * kWarps);
+    fence_barrier_init();
+  }
+  for (int i = threadIdx.x; i < 6 * CL * kWarps; i += NT) (&parts[0][0][0])[i] = 0ull;
+  for (int i = threadIdx.x; i < 2 * kMaxTeacherK; i += NT) (&xks[0][0])[i] = 0ull;
+  if constexpr (CL > 1)
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  else
+    __syncthreads();
+  pdl_wait();
+  pdl_trigger();
+  const int64_t stride = gridDim.x / CL;
+  // My warp's vectors of any row: [first, first + cap), those that exist.
+  const int per = ((p.V + 2 * E - 2) / E + CL - 1) / CL, cap = warp_vectors(per);
+  const int first = part * per + warp * cap, last = min(first + cap, (part + 1) * per);
+  uint4* mine = kept + warp * cap - first;  // indexed by the vector
+  T* elem = reinterpret_cast<T*>(mine);
+  const float c = p.c;
+
+  auto weight = [&](int64_t r) { return r >= p.rows ? 0.f : p.weights ? p.weights[r] : 1.f; };
+  auto fetch = [&](const Row<T>& row, int u) {
+    if (row.full(u)) {
+      cp_async_16(smem_u32(mine + u), row.x + ((int64_t)u * E - row.pad));
+    } else {
+      mine[u] = make_uint4(Tr::kNegInf, Tr::kNegInf, Tr::kNegInf, Tr::kNegInf);
+#pragma unroll 1
+      for (int e = max(0, row.pad - u * E); e < min(E, row.pad + p.V - u * E); ++e)
+        elem[u * E + e] = row.x[row.index(u, e)];
+    }
+  };
+  auto fetch_teacher = [&](int64_t r, int buf) {
+#pragma unroll 1
+    for (int k = lane; k < p.K; k += 32) {
+      cp_async_4(smem_u32(&t_id[buf][k]), p.t_ids + r * p.K + k);
+      cp_async_4(smem_u32(&t_lp[buf][k]), p.t_lp + r * p.K + k);
+    }
+  };
+
+  int64_t r = blockIdx.x / CL;
+  float w = weight(r);
+  Row<T> row(p.x, min(r, p.rows - 1), p.ld, p.V);
+  if (w != 0.f) {
+    const int end = min(last, row.n_vec);
+    for (int u = first + lane; u < end; u += 32) fetch(row, u);
+    fetch_teacher(r, 0);
+  }
+  if constexpr (CL > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+
+  for (uint32_t n = 0; r < p.rows;) {  // n: rows that counted
+    const int64_t r_next = r + stride;
+    const float w_next = weight(r_next);
+    const Row<T> next(p.x, min(r_next, p.rows - 1), p.ld, p.V);
+    const int end = min(last, row.n_vec), end_next = w_next != 0.f ? min(last, next.n_vec) : first;
+    T* out = reinterpret_cast<T*>(p.grad) + r * p.V;
+    if (w == 0.f) {  // uniform over the cluster
+      for (int u = first + lane; u < end; u += 32)
+        store_vec(out, row, u, make_uint4(0u, 0u, 0u, 0u));
+      if (part == 0 && threadIdx.x == 0) {
+        p.row_loss[r] = 0.f;
+        p.stats[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      for (int u = first + lane; u < end_next; u += 32) fetch(next, u);
+      if (w_next != 0.f) fetch_teacher(r_next, n & 1);
+      r = r_next, w = w_next, row = next;
+      continue;
+    }
+    const int buf = n & 1;
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncwarp();
+    float norm, sum_p;
+    {
+      Teacher t;
+      t.load(t_id[buf], t_lp[buf], p.K);
+      t.prepare(p);
+      norm = t.norm, sum_p = t.sum_p;
+#pragma unroll
+      for (int i = 0; i < kIds; ++i)
+        if (lane + 32 * i < p.K) t_p[buf][lane + 32 * i] = t.p[i];
+    }
+
+    // The teacher's elements of my part out of the row: value, then a tag of
+    // the entry (repeated ids overwrite one another's), then -inf.
+    uint32_t own = 0;  // entries lane + 32 i here, the first of their id
+    float m_k = -INFINITY;
+#pragma unroll 1
+    for (int i = 0; 32 * i < p.K; ++i) {
+      const int k = lane + 32 * i;
+      if (k >= p.K) break;
+      const int id = t_id[buf][k], at = id + row.pad;
+      if (id >= 0 && id < p.V && at / E >= first && at / E < end) {
+        const float x = Tr::to_f(elem[at]);
+        t_x[buf][k] = x;
+        m_k = fmaxf(m_k, x);
+        own |= 1u << i;
+        send<CL>(&xks[buf][k], 0, x, n + 1);
+      }
+    }
+    if (__any_sync(0xffffffffu, own != 0)) {
+      __syncwarp();
+#pragma unroll 1
+      for (int i = 0; i < kIds; ++i)
+        if ((own >> i) & 1u)
+          reinterpret_cast<Tag*>(elem)[t_id[buf][lane + 32 * i] + row.pad] = (Tag)(lane + 32 * i);
+      __syncwarp();
+      bool dup = false;
+#pragma unroll 1
+      for (int i = 0; i < kIds; ++i)
+        if ((own >> i) & 1u)
+          dup |= reinterpret_cast<const Tag*>(elem)[t_id[buf][lane + 32 * i] + row.pad] !=
+                 (Tag)(lane + 32 * i);
+      __syncwarp();
+#pragma unroll 1
+      for (int i = 0; i < kIds; ++i)
+        if ((own >> i) & 1u)
+          reinterpret_cast<Tag*>(elem)[t_id[buf][lane + 32 * i] + row.pad] = (Tag)Tr::kNegInf;
+      if (__any_sync(0xffffffffu, dup)) own = first_of_ids(own, t_id[buf], p.K);
+      __syncwarp();
+    }
+
+    // The rest: maximum, then sum.
+    const int n4 = end > first ? (end - first) / 128 * 128 : 0, tail = first + n4;
+    typename Tr::Max vm = Tr::vmax(make_uint4(Tr::kNegInf, Tr::kNegInf, Tr::kNegInf, Tr::kNegInf));
+#pragma unroll 1
+    for (int u = first + lane; u < tail; u += 128) {
+      typename Tr::Max q[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) q[k] = Tr::vmax(mine[u + 32 * k]);
+      vm = Tr::vmax(vm, Tr::vmax(Tr::vmax(q[0], q[1]), Tr::vmax(q[2], q[3])));
+    }
+#pragma unroll 1
+    for (int u = tail + lane; u < end; u += 32) vm = Tr::vmax(vm, Tr::vmax(mine[u]));
+    const float m_w = warp_max(fmaxf(Tr::value(vm), m_k));
+    float s = 0.f;
+    if (!slow_range(m_w)) {
+      const float rw = __fmul_rn(m_w, c);
+      const uint64_t c2 = f32x2_pack(c, c), nr2 = f32x2_pack(-rw, -rw);
+      uint64_t s2[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s2[k] = f32x2_pack(0.f, 0.f);
+      auto add = [&](const uint4& v, uint64_t& sum) {
+#pragma unroll
+        for (int i = 0; i < E / 2; ++i) {
+          float a, b;
+          Tr::pair(v, i, a, b);
+          f32x2_unpack(f32x2_fma(f32x2_pack(a, b), c2, nr2), a, b);
+          sum = f32x2_add(sum, f32x2_pack(ex2(a), ex2(b)));
+        }
+      };
+#pragma unroll 1
+      for (int u = first + lane; u < tail; u += 128) {
+        uint4 v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = mine[u + 32 * k];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) add(v[k], s2[k]);
+      }
+#pragma unroll 1
+      for (int u = tail + lane; u < end; u += 32) add(mine[u], s2[0]);
+      float a, b;
+      f32x2_unpack(f32x2_add(f32x2_add(s2[0], s2[1]), f32x2_add(s2[2], s2[3])), a, b);
+      s = (a + b) * ex2(-fmaf(m_w, c, -rw));  // what rw lacks of m c
+    } else {
+      const float m = shift_of(m_w);
+#pragma unroll 1
+      for (int u = first + lane; u < end; u += 32)
+#pragma unroll 1
+        for (int e = 0; e < E; ++e) s += ex2((Tr::to_f(elem[u * E + e]) - m) * c);
+    }
+    float s_in = 0.f;
+#pragma unroll
+    for (int i = 0; i < kIds; ++i)
+      if ((own >> i) & 1u) s_in += ex2((t_x[buf][lane + 32 * i] - shift_of(m_w)) * c);
+    s = warp_sum(s);
+    s_in = warp_sum(s_in);
+    // To every CTA of the cluster; each warp hears from every other.
+    if (lane < CL) {
+      send<CL>(&parts[buf][0][part * kWarps + warp], lane, m_w, n + 1);
+      send<CL>(&parts[buf][1][part * kWarps + warp], lane, s, n + 1);
+      send<CL>(&parts[buf][2][part * kWarps + warp], lane, s_in, n + 1);
+      // (The barrier is where a warp sleeps until all have sent; what it then
+      // reads carries its own proof.)
+      if constexpr (CL == 1)
+        mbar_arrive(&bar[buf]);
+      else
+        mbar_arrive_cluster_relaxed(mapa_shared(smem_u32(&bar[buf]), lane));
+    }
+    bool met = mbar_wait(&bar[buf], (n >> 1) & 1u, p.err);
+    float4 got[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      got[i] = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+      const int from = lane + 32 * i;
+      if (from < CL * kWarps) {
+        met &= receive(&parts[buf][0][from], n + 1, got[i].x, p.err);
+        met &= receive(&parts[buf][1][from], n + 1, got[i].y, p.err);
+        met &= receive(&parts[buf][2][from], n + 1, got[i].z, p.err);
+      }
+    }
+    __syncwarp();
+
+    if (w_next != 0.f) fetch_teacher(r_next, buf ^ 1);
+
+    // Every warp finishes the row's numbers (the same in all of them).
+    const float3 q = join(got[0], got[1], c);
+    const float4 st = row_numbers(norm, sum_p, p.tail, q);
+    if (part == 0 && warp == 0) {
+      Teacher t;
+      t.load(t_id[buf], t_lp[buf], p.K);
+      float xk[kIds];
+#pragma unroll
+      for (int i = 0; i < kIds; ++i) {
+        t.p[i] = xk[i] = 0.f;
+        t.lp[i] -= norm;
+        if (lane + 32 * i < p.K) {
+          t.p[i] = t_p[buf][lane + 32 * i];
+          if (t.id[i] >= 0 && t.id[i] < p.V) met &= receive(&xks[buf][lane + 32 * i], n + 1, xk[i], p.err);
+        }
+      }
+      t.sum_p = sum_p;
+      const float loss = row_loss(t, p, q, xk);
+      met = __all_sync(0xffffffffu, met);
+      if (lane == 0) {
+        p.row_loss[r] = met ? loss * w : NAN;
+        p.stats[r] = st;
+      }
+    }
+    // The gradient: every element as an outside one (the teacher's are -inf by
+    // now), then the teacher's over it. The next row's vectors follow.
+    const float up = w * p.gscale;
+    const bool slow = slow_range(st.x);
+    const float rm = __fmul_rn(st.x, c), coef = st.z * up * (slow ? 1.f : ex2(-fmaf(st.x, c, -rm)));
+    // Whole steps of 128 full vectors without checks.
+    uint4* dst = reinterpret_cast<uint4*>(out - row.pad);
+    const uint4* src = reinterpret_cast<const uint4*>(next.x - next.pad);
+    const bool aligned = (reinterpret_cast<uintptr_t>(dst) & 15u) == 0;
+    const int fa = aligned && !slow ? row.full_lo : p.V, fb = row.full_lo + (int)row.n_full;
+    const int next_fa = next.full_lo, next_fb = next.full_lo + (int)next.n_full;
+#pragma unroll 1
+    for (int u0 = first; u0 < end || u0 < end_next; u0 += 128) {
+      const int u = u0 + lane;
+      if (u0 >= fa && u0 + 128 <= min(fb, end)) {
+        uint4 v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = mine[u + 32 * k];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) dst[u + 32 * k] = grad_vec<T, false>(v[k], c, rm, coef);
+        if (u0 >= next_fa && u0 + 128 <= min(next_fb, end_next)) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            cp_async_16(smem_u32(mine + u + 32 * k), src + u + 32 * k);
+          continue;
+        }
+      } else {
+#pragma unroll 1
+        for (int v = u; v < min(u0 + 128, end); v += 32)
+          store_vec(out, row, v,
+                    slow ? grad_vec<T, true>(mine[v], c, st.x, coef)
+                         : grad_vec<T, false>(mine[v], c, rm, coef));
+      }
+#pragma unroll 1
+      for (int v = u; v < min(u0 + 128, end_next); v += 32) fetch(next, v);
+    }
+    __syncwarp();
+#pragma unroll 1
+    for (int i = 0; i < kIds; ++i)
+      if ((own >> i) & 1u) {
+        const int k = lane + 32 * i, id = t_id[buf][k];
+        float mass = t_p[buf][k];
+        if (own & kDup) mass = mass_of_id(id, t_id[buf], t_p[buf], p.K);
+        const float qk = ex2((t_x[buf][k] - st.x) * c) * st.y;
+        out[id] = Tr::from_f((qk - (st.y == 0.f ? 0.f : mass)) * up);
+      }
+    ++n;
+    r = r_next, w = w_next, row = next;
+  }
+  // (No CTA leaves while another's exchange may still reach it.)
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  if constexpr (CL > 1) cluster_sync_all();
+}
+
+struct Smem {
+  Acc acc[kWarps];
+  int dup;                   // some id of this slice is there twice
+  float4 part[kMaxCluster];  // a slice's max, sum outside, sum at the ids
+};
+
+// Loss, and with GRAD the gradient, of rows that are streamed: CL CTAs a row.
 template <typename T, int CL, bool GRAD>
-__global__ void __launch_bounds__(NT, 2) distill_kernel(const Params p) {
+__global__ void __launch_bounds__(NT, 4) distill_stream_kernel(const Params p) {
   using Tr = Traits<T>;
   constexpr int E = Tr::E;
   __shared__ Smem sm;
-  extern __shared__ __align__(16) uint8_t dyn[];  // kept vectors, then the bitmap
+  extern __shared__ __align__(16) uint8_t dyn[];  // the bitmap: a byte a vector
   pdl_wait();
   pdl_trigger();
   const int64_t r = blockIdx.x / CL;
@@ -156,13 +623,12 @@ __global__ void __launch_bounds__(NT, 2) distill_kernel(const Params p) {
   if constexpr (CL > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
 
   const Row<T> row(p.x, r, p.ld, p.V);
-  const int per = (row.n_vec + CL - 1) / CL;
-  const int u_lo = min(part * per, row.n_vec), u_hi = min(u_lo + per, row.n_vec);
+  const Slice sl(row, part, CL);
   T* out = GRAD ? reinterpret_cast<T*>(p.grad) + r * p.V : nullptr;
   const float w = p.weights ? p.weights[r] : 1.f;
   if (w == 0.f) {  // uniform over the cluster
     if constexpr (GRAD)
-      for (int u = u_lo + tid; u < u_hi; u += NT)
+      for (int u = sl.lo + tid; u < sl.hi; u += NT)
         store_vec(out, row, u, make_uint4(0u, 0u, 0u, 0u));
     if (part == 0 && tid == 0) {
       p.row_loss[r] = 0.f;
@@ -172,154 +638,166 @@ __global__ void __launch_bounds__(NT, 2) distill_kernel(const Params p) {
     return;
   }
 
-  uint4* kept = reinterpret_cast<uint4*>(dyn);
-  uint8_t* bitmap = dyn + (size_t)p.keep * NT * 16;  // E bits (a byte or half) a vector
-  for (int i = tid; i < (per + 15) / 16; i += NT)
+  uint8_t* bitmap = dyn;
+  for (int i = tid; i < (sl.hi - sl.lo + 15) / 16; i += NT)
     reinterpret_cast<uint4*>(bitmap)[i] = make_uint4(0u, 0u, 0u, 0u);
   if (tid == 0) sm.dup = 0;
-  load_teacher(sm, p, r);
-  // The ids of this slice: owned by thread k.
-  bool mine = false;
-  float xk = -INFINITY;
-  if (tid < p.K && sm.id[tid] >= 0) {
-    const int id = sm.id[tid], u = (id + row.pad) / E, e = (id + row.pad) % E;
-    xk = Tr::to_f(row.x[id]);
-    sm.xk[tid] = xk;
-    mine = u >= u_lo && u < u_hi;
-    if (mine) {
-      const int at = u - u_lo;
-      const uint32_t bit = 1u << (8 * (at % 4) + e);
-      if (atomicOr(reinterpret_cast<uint32_t*>(bitmap) + at / 4, bit) & bit) sm.dup = 1;
+  Teacher t;
+  t.load(p.t_ids + r * p.K, p.t_lp + r * p.K, p.K);
+  __syncthreads();
+  // Warp 0 marks the ids of this slice.
+  float xk[kIds];
+  uint32_t own = 0;
+  if (warp == 0) {
+#pragma unroll
+    for (int i = 0; i < kIds; ++i) {
+      xk[i] = -INFINITY;
+      if (t.id[i] >= 0 && t.id[i] < p.V) {
+        const int u = (t.id[i] + row.pad) / E, e = (t.id[i] + row.pad) % E, at = u - sl.lo;
+        xk[i] = Tr::to_f(row.x[t.id[i]]);
+        if (u >= sl.lo && u < sl.hi) {
+          const uint32_t bit = 1u << (8 * (at % 4) + e);
+          own |= 1u << i;
+          if (atomicOr(reinterpret_cast<uint32_t*>(bitmap) + at / 4, bit) & bit) sm.dup = 1;
+        }
+      }
     }
   }
   __syncthreads();
-  float mass_k = 0.f;
-  const bool own = mine && first_of_id(sm, p.K, tid, mass_k);
 
   // The slice's sum over the elements that are not the teacher's.
   const float c = p.c;
   const uint64_t c2 = f32x2_pack(c, c);
-  Acc a{-INFINITY, 0.f, 0.f};
-  for (int u = u_lo + tid, it = 0; u < u_hi; u += U * NT, it += U) {
+  float m = -INFINITY, r0 = 0.f, s = 0.f;
+  for_groups<NT, U>(row, sl, [&](const uint4(&x)[U], int u, int) {
     uint4 v[U];
+    typename Tr::Max vm[U];
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       const int uk = u + k * NT;
-      v[k] = uk < u_hi ? row.load(uk) : make_uint4(Tr::kNegInf, Tr::kNegInf, Tr::kNegInf, Tr::kNegInf);
-    }
-    float mx = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < U; ++k) {
-      const int uk = u + k * NT;
-      if (GRAD && it + k < p.keep) kept[(it + k) * NT + tid] = v[k];
-      const uint32_t in = uk < u_hi ? bitmap[uk - u_lo] : 0u;
+      v[k] = x[k];
+      const uint32_t in = uk < sl.hi ? bitmap[uk - sl.lo] : 0u;
       if (in) Tr::blank(v[k], in);
-      mx = fmaxf(mx, Tr::max_of(v[k]));
+      vm[k] = Tr::vmax(v[k]);
     }
-    if (mx > a.m) rebase(a, mx, c);
-    const float m = shift_of(a.m);
-    const uint64_t nm2 = f32x2_pack(-m, -m);
+    static_assert(U == 4, "tree of maxima");
+    const float mx = Tr::value(Tr::vmax(Tr::vmax(vm[0], vm[1]), Tr::vmax(vm[2], vm[3])));
+    if (mx > m) {
+      const float rn = __fmul_rn(fmaxf(mx, kFloor), c);
+      s *= m == -INFINITY ? (s != s ? s : 0.f) : ex2(r0 - rn);
+      m = mx;
+      r0 = rn;
+    }
+    const uint64_t nr2 = f32x2_pack(-r0, -r0);
     uint64_t s2 = f32x2_pack(0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < U; ++k) {
 #pragma unroll
       for (int i = 0; i < E / 2; ++i) {
-        float xa, xb, da, db;
-        Tr::pair(v[k], i, xa, xb);
-        f32x2_unpack(f32x2_mul(f32x2_add(f32x2_pack(xa, xb), nm2), c2), da, db);
-        s2 = f32x2_add(s2, f32x2_pack(ex2(da), ex2(db)));
+        float a, b;
+        Tr::pair(v[k], i, a, b);
+        f32x2_unpack(f32x2_fma(f32x2_pack(a, b), c2, nr2), a, b);
+        s2 = f32x2_add(s2, f32x2_pack(ex2(a), ex2(b)));
       }
     }
-    float s0, s1;
-    f32x2_unpack(s2, s0, s1);
-    a.s += s0 + s1;
+    float a, b;
+    f32x2_unpack(s2, a, b);
+    s += a + b;
+  });
+  // A warp's sums against its own maximum, in a fixed order.
+  const float m_w = warp_max(m);
+  if (slow_range(m_w) && m_w != -INFINITY) {
+    s = slow_sum(row, sl, bitmap, m_w, c);
+  } else {
+    const float e = fmaf(m, c, -r0);  // what r0 lacks of m c
+    if (m >= kSlowBelow)
+      s *= ex2(-e) * (m == m_w ? 1.f : ex2((m - m_w) * c));
+    else
+      s = s != s ? s : 0.f;  // nothing against the warp's maximum
   }
-  const float m = block_max<NT>(own ? fmaxf(a.m, xk) : a.m, sm.red);
-  rebase(a, m, c);
-  const float s_out_w = warp_sum(a.s);
-  const float s_in_w = warp_sum(own ? ex2((xk - shift_of(m)) * c) : 0.f);
-  if (lane == 0) sm.sum[warp] = make_float2(s_out_w, s_in_w);
+  s = warp_sum(s);
+  if (lane == 0) sm.acc[warp] = Acc{m_w, s, 0.f};
   __syncthreads();
+
+  // Warp 0 adds the warps up, with the ids' own exponentials.
+  float3 q;
+  float mass[kIds];
   if (warp == 0) {
-    // Every CTA of the cluster gets every slice's sums.
-    float s_out = 0.f, s_in = 0.f;
-    for (int i = 0; i < kWarps; ++i) {
-      s_out += sm.sum[i].x;
-      s_in += sm.sum[i].y;
+    t.prepare(p);
+#pragma unroll
+    for (int i = 0; i < kIds; ++i) mass[i] = t.p[i];
+    if (sm.dup) {
+      t.masses(p.K, mass);
+#pragma unroll
+      for (int i = 0; i < kIds; ++i)
+        if (mass[i] == -1.f) own &= ~(1u << i);
     }
+    Acc a = lane < kWarps ? sm.acc[lane] : Acc{-INFINITY, 0.f, 0.f};
+    float m_all = a.m;
+#pragma unroll
+    for (int i = 0; i < kIds; ++i)
+      if ((own >> i) & 1u) m_all = fmaxf(m_all, xk[i]);
+    m_all = warp_max(m_all);
+    rebase(a, m_all, c);
+    float s_in = 0.f;
+#pragma unroll
+    for (int i = 0; i < kIds; ++i)
+      if ((own >> i) & 1u) s_in += ex2((xk[i] - shift_of(m_all)) * c);
+    q = make_float3(m_all, warp_sum(a.s), warp_sum(s_in));
     if constexpr (CL > 1) {
       asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+      // Every CTA of the cluster gets every slice's sums.
       if (lane < CL)
-        st_dsmem_f4(mapa_shared(smem_u32(&sm.part[part]), lane), make_float4(m, s_out, s_in, 0.f));
-    } else if (lane == 0) {
-      sm.part[0] = make_float4(m, s_out, s_in, 0.f);
+        st_dsmem_f4(mapa_shared(smem_u32(&sm.part[part]), lane), make_float4(q.x, q.y, q.z, 0.f));
     }
   } else if constexpr (CL > 1) {
     asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
   }
-  if constexpr (CL > 1)
-    cluster_sync_all();
-  else
-    __syncthreads();
-
-  // Warp 0 finishes the row's numbers (the same in every CTA of the cluster).
+  if constexpr (CL > 1) cluster_sync_all();
+  __shared__ float4 numbers;
   if (warp == 0) {
-    float mm = -INFINITY;
-    for (int i = 0; i < CL; ++i) mm = fmaxf(mm, sm.part[i].x);
-    const float m0 = shift_of(mm);
-    float s_out = 0.f, s_in = 0.f;
-    for (int i = 0; i < CL; ++i) {
-      const float4 q = sm.part[i];
-      // a slice without any element above -inf has no sums to rebase
-      const float f = q.x == -INFINITY || q.x == mm ? 1.f : ex2((q.x - mm) * c);
-      s_out += q.y * f;
-      s_in += q.z * f;
-    }
-    float sum_p = 0.f;
-    for (int k = lane; k < p.K; k += 32) sum_p += sm.p[k];
-    sum_p = warp_sum(sum_p);
-    const float s = s_out + s_in;
-    // An empty row: every log q is -inf, the loss inf where the teacher has mass.
-    const float l2 = s == 0.f ? 0.f : log2f(s);
-    float loss = 0.f;
-    for (int k = lane; k < p.K; k += 32) {
-      const float pk = sm.p[k];
-      if (pk > 0.f)
-        loss += pk * (sm.lp[k] - fmaf(sm.xk[k] - m0, p.inv_t, -l2 * kLn2));
-      else if (pk != pk)
-        loss = pk;
-    }
-    loss = warp_sum(loss);
-    const float p_t = p.tail ? fmaxf(0.f, 1.f - sum_p) : 0.f;
-    if (p_t > 0.f) loss += p_t * (logf(p_t) - (log2f(s_out) - l2) * kLn2);
-    if (lane == 0) {
-      const float mass = sum_p + p_t;
-      const float inv = s == 0.f ? 0.f : 1.f / s;
-      // A student with no mass outside has q_j = 0 there.
-      const float ratio = p_t > 0.f && s_out != 0.f ? p_t * s / s_out : 0.f;
-      sm.row = make_float4(m0, mass * inv, s_out == 0.f ? 0.f : (mass - ratio) * inv,
-                           s == 0.f ? 0.f : 1.f);
-      if (part == 0) {
+    if constexpr (CL > 1)
+      q = join(lane < CL ? sm.part[lane] : make_float4(-INFINITY, 0.f, 0.f, 0.f),
+               make_float4(-INFINITY, 0.f, 0.f, 0.f), c);
+    const float4 st = row_numbers(t.norm, t.sum_p, p.tail, q);
+    if (part == 0) {
+      const float loss = row_loss(t, p, q, xk);
+      if (lane == 0) {
         p.row_loss[r] = loss * w;
-        p.stats[r] = sm.row;
+        p.stats[r] = st;
       }
     }
+    if (lane == 0) numbers = st;
   }
   if constexpr (!GRAD) return;
   __syncthreads();
 
   // The gradient: every element as an outside one, then the teacher's ids of
   // this slice over it (same CTA, after the barrier).
-  const float4 st = sm.row;
+  const float4 st = numbers;
   const float up = w * p.gscale;
-  for (int u = u_lo + tid, it = 0; u < u_hi; u += NT, ++it) {
-    const uint4 v = it < p.keep ? kept[it * NT + tid] : row.load(u);
-    store_vec(out, row, u, grad_vec<T>(v, c, st.x, st.z * up));
+  if (!slow_range(st.x)) {
+    const float rm = __fmul_rn(st.x, c), coef = st.z * up * ex2(-fmaf(st.x, c, -rm));
+    for_groups<NT, U>(row, sl, [&](const uint4(&v)[U], int u, int) {
+#pragma unroll
+      for (int k = 0; k < U; ++k)
+        if (u + k * NT >= sl.a && u + k * NT < sl.b)
+          store_vec(out, row, u + k * NT, grad_vec<T, false>(v[k], c, rm, coef));
+    });
+    const int e = tid == 0 ? sl.head : tid == 1 ? sl.tail : -1;
+    if (e >= 0) store_part(out, row, e, grad_vec<T, false>(row.load(e), c, rm, coef));
+  } else {
+    for (int u = sl.lo + tid; u < sl.hi; u += NT)
+      store_vec(out, row, u, grad_vec<T, true>(row.load(u), c, st.x, st.z * up));
   }
   __syncthreads();
-  if (own) {
-    const float q = ex2((xk - st.x) * c) * st.y;
-    out[sm.id[tid]] = Tr::from_f((q - mass_k * st.w) * up);
+  if (warp == 0) {
+#pragma unroll
+    for (int i = 0; i < kIds; ++i)
+      if ((own >> i) & 1u) {
+        const float qk = ex2((xk[i] - st.x) * c) * st.y;
+        out[t.id[i]] = Tr::from_f((qk - (st.y == 0.f ? 0.f : mass[i])) * up);
+      }
   }
 }
 
@@ -335,7 +813,9 @@ template <typename T>
 __global__ void __launch_bounds__(NT) distill_bwd_kernel(const BwdParams b) {
   using Tr = Traits<T>;
   constexpr int E = Tr::E;
-  __shared__ Smem sm;
+  constexpr int kBits = NT * U * E;  // elements of the chunk
+  __shared__ uint32_t seen[kBits / 32];
+  __shared__ int dup;
   pdl_wait();
   pdl_trigger();
   const Params& p = b.f;
@@ -347,33 +827,51 @@ __global__ void __launch_bounds__(NT) distill_bwd_kernel(const BwdParams b) {
   T* out = reinterpret_cast<T*>(p.grad) + r * p.V;
   const float w = p.weights ? p.weights[r] : 1.f;
   const float up = w == 0.f ? 0.f : w * p.gscale * b.g[r * b.g_stride];
-  const float4 st = p.stats[r];
-  const bool none = up == 0.f;
+  if (up == 0.f) {
+    for (int u = u_lo + tid; u < u_hi; u += NT) store_vec(out, row, u, make_uint4(0u, 0u, 0u, 0u));
+    return;
+  }
   uint4 v[U];
 #pragma unroll
   for (int k = 0; k < U; ++k) {
     const int u = u_lo + tid + k * NT;
-    v[k] = u < u_hi && !none ? row.load(u) : make_uint4(0u, 0u, 0u, 0u);
+    v[k] = u < u_hi ? row.load(u) : make_uint4(0u, 0u, 0u, 0u);
   }
-  if (tid == 0) sm.dup = 1;  // no bitmap here: repeats are looked for
-  if (!none) load_teacher(sm, p, r);
-#pragma unroll
-  for (int k = 0; k < U; ++k) {
-    const int u = u_lo + tid + k * NT;
-    if (u < u_hi)
-      store_vec(out, row, u,
-                none ? make_uint4(0u, 0u, 0u, 0u) : grad_vec<T>(v[k], p.c, st.x, st.z * up));
-  }
-  if (none) return;
+  // Thread k's teacher entry, if it is of this chunk, and whether an id of
+  // the chunk is there twice.
+  const int id = tid < p.K ? p.t_ids[r * p.K + tid] : -1;
+  const int at = id + row.pad - u_lo * E;
+  const bool mine = id >= 0 && id < p.V && at >= 0 && at / E < u_hi - u_lo;
+  const float4 st = p.stats[r];
+  const float xk = mine ? Tr::to_f(row.x[id]) : 0.f;
+  float mass = mine ? expf(p.t_lp[r * p.K + tid] - st.w) : 0.f;
+  for (int i = tid; i < kBits / 32; i += NT) seen[i] = 0u;
+  if (tid == 0) dup = 0;
   __syncthreads();
-  if (tid < p.K && sm.id[tid] >= 0) {
-    const int id = sm.id[tid], u = (id + row.pad) / E;
-    float mass;
-    if (u >= u_lo && u < u_hi && first_of_id(sm, p.K, tid, mass)) {
-      const float q = ex2((Tr::to_f(row.x[id]) - st.x) * p.c) * st.y;
-      out[id] = Tr::from_f((q - mass * st.w) * up);
+  if (mine && (atomicOr(&seen[at / 32], 1u << (at % 32)) >> (at % 32)) & 1u) dup = 1;
+  if (!slow_range(st.x)) {
+    const float rm = __fmul_rn(st.x, p.c), coef = st.z * up * ex2(-fmaf(st.x, p.c, -rm));
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int u = u_lo + tid + k * NT;
+      if (u < u_hi) store_vec(out, row, u, grad_vec<T, false>(v[k], p.c, rm, coef));
     }
+  } else {
+    for (int u = u_lo + tid; u < u_hi; u += NT)
+      store_vec(out, row, u, grad_vec<T, true>(row.load(u), p.c, st.x, st.z * up));
   }
+  __syncthreads();
+  if (!mine) return;
+  if (dup) {  // the p of all entries with this id, at the first of them
+    mass = 0.f;
+    for (int j = 0; j < p.K; ++j)
+      if (p.t_ids[r * p.K + j] == id) {
+        if (j < tid) return;
+        mass += expf(p.t_lp[r * p.K + j] - st.w);
+      }
+  }
+  const float q = ex2((xk - st.x) * p.c) * st.y;
+  out[id] = Tr::from_f((q - (st.y == 0.f ? 0.f : mass)) * up);
 }
 
 // loss = scale * sum of the rows' losses, one CTA, fixed order.
@@ -425,47 +923,97 @@ void check(const LogitRows& in, int K, const char* what) {
     throw std::runtime_error(std::string(what) + ": between 1 and 128 teacher values a row");
 }
 
-constexpr int kSmemLimit = 96 * 1024;  // two CTAs an SM
+constexpr int kSmemThree = 64 * 1024;   // three CTAs an SM
+constexpr int kSmemMost = 208 * 1024;
+constexpr int kBitmapMost = 160 * 1024;
 
-template <typename T, int CL, bool GRAD>
-void launch_cl(Params p, int64_t rows, cudaStream_t stream) {
-  const int n_vec = (p.V + 2 * Traits<T>::E - 2) / Traits<T>::E;
-  const int per = (n_vec + CL - 1) / CL;
-  const int bitmap = (per + 15) / 16 * 16;
-  p.keep = 0;
-  if (GRAD) {
-    p.keep = (per + NT - 1) / NT;
-    const int fit = (kSmemLimit - bitmap) / (NT * 16);
-    p.keep = p.keep < fit ? p.keep : (fit > 0 ? fit : 0);
-  }
-  const int smem = p.keep * NT * 16 + bitmap;
-  auto kernel = distill_kernel<T, CL, GRAD>;
-  static bool attr[kMaxDevices] = {};
-  set_smem_attr_once(kernel, 208 * 1024, attr, "distill_loss");
-  if (smem > 208 * 1024) throw std::runtime_error("distill_loss: vocabulary too large");
+cudaLaunchAttribute cluster_of(int n) {
   cudaLaunchAttribute cl;
   cl.id = cudaLaunchAttributeClusterDimension;
-  cl.val.clusterDim.x = CL;
+  cl.val.clusterDim.x = n;
   cl.val.clusterDim.y = cl.val.clusterDim.z = 1;
-  launch_pdl(kernel, dim3((unsigned)(rows * CL)), dim3(NT), smem, stream, CL > 1 ? &cl : nullptr,
-             p);
+  return cl;
+}
+// Vectors of a CTA where CL of them share a row.
+template <typename T>
+int slice_vectors(int V, int cl) {
+  return ((V + 2 * Traits<T>::E - 2) / Traits<T>::E + cl - 1) / cl;
+}
+// Shared memory that holds them, in equal parts a warp.
+template <typename T>
+int slice_bytes(int V, int cl) {
+  return warp_vectors(slice_vectors<T>(V, cl)) * kWarps * 16;
 }
 
-template <typename T, bool GRAD>
-void launch_t(const Params& p, int64_t rows, cudaStream_t stream) {
+template <typename T, int CL>
+void launch_fused(Params p, cudaStream_t stream) {
+  auto kernel = distill_fused_kernel<T, CL>;
+  static bool attr[kMaxDevices] = {};
+  set_smem_attr_once(kernel, kSmemMost, attr, "distill_loss");
+  const int smem = slice_bytes<T>(p.V, CL);
+  // Clusters that run at the same time, asked for once a size.
+  struct Known {
+    int dev = -1, smem = 0, clusters = 0;
+  };
+  static thread_local Known known;
   int dev = 0;
   cudaGetDevice(&dev);
-  int cl = row_split(rows, p.V / Traits<T>::E, num_sms(dev), NT);
-  // The gradient pass wants the whole slice in shared memory.
-  if (GRAD)
-    while (cl < 8 && (int64_t)p.V * (int)sizeof(T) / cl > kSmemLimit - 16 * 1024) cl *= 2;
-  // bitmaps of a very large vocabulary
-  while (cl < 8 && p.V / Traits<T>::E / cl > 64 * 1024) cl *= 2;
+  p.err = device_status_ptr(dev);
+  const cudaLaunchAttribute cl = cluster_of(CL);
+  if (known.dev != dev || known.smem != smem) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(CL);
+    cfg.blockDim = dim3(NT);
+    cfg.dynamicSmemBytes = smem;
+    cfg.attrs = const_cast<cudaLaunchAttribute*>(&cl);
+    cfg.numAttrs = 1;
+    int n = 0;
+    const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+    if (e != cudaSuccess || n < 1)
+      throw std::runtime_error(std::string("distill_loss: no cluster fits: ") +
+                               cudaGetErrorString(e));
+    known = Known{dev, smem, n};
+  }
+  const int64_t clusters = p.rows < known.clusters ? p.rows : known.clusters;
+  launch_pdl(kernel, dim3((unsigned)(clusters * CL)), dim3(NT), smem, stream,
+             CL > 1 ? &cl : nullptr, p);
+}
+
+template <typename T, int CL, bool GRAD>
+void launch_stream(const Params& p, cudaStream_t stream) {
+  auto kernel = distill_stream_kernel<T, CL, GRAD>;
+  static bool attr[kMaxDevices] = {};
+  set_smem_attr_once(kernel, kBitmapMost, attr, "distill_loss");
+  const cudaLaunchAttribute cl = cluster_of(CL);
+  const int bitmap = (slice_vectors<T>(p.V, CL) + 15) / 16 * 16;
+  launch_pdl(kernel, dim3((unsigned)(p.rows * CL)), dim3(NT), bitmap, stream,
+             CL > 1 ? &cl : nullptr, p);
+}
+
+template <typename T>
+void launch_t(const Params& p, cudaStream_t stream) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const int sms = num_sms(dev);
+  if (p.grad && slice_bytes<T>(p.V, kMaxCluster) <= kSmemMost) {
+    int cl = row_split(p.rows, p.V / Traits<T>::E, sms, NT);
+    while (cl < kMaxCluster && slice_bytes<T>(p.V, cl) > kSmemThree) cl *= 2;
+    switch (cl) {
+      case 1: return launch_fused<T, 1>(p, stream);
+      case 2: return launch_fused<T, 2>(p, stream);
+      case 4: return launch_fused<T, 4>(p, stream);
+      default: return launch_fused<T, 8>(p, stream);
+    }
+  }
+  if (p.grad) return launch_stream<T, 8, true>(p, stream);
+  int cl = row_split(p.rows, p.V / Traits<T>::E, 2 * sms, NT);
+  // bitmaps of a very large vocabulary: 32 KB, for four CTAs an SM
+  while (cl < kMaxCluster && slice_vectors<T>(p.V, cl) > 32 * 1024) cl *= 2;
   switch (cl) {
-    case 1: return launch_cl<T, 1, GRAD>(p, rows, stream);
-    case 2: return launch_cl<T, 2, GRAD>(p, rows, stream);
-    case 4: return launch_cl<T, 4, GRAD>(p, rows, stream);
-    default: return launch_cl<T, 8, GRAD>(p, rows, stream);
+    case 1: return launch_stream<T, 1, false>(p, stream);
+    case 2: return launch_stream<T, 2, false>(p, stream);
+    case 4: return launch_stream<T, 4, false>(p, stream);
+    default: return launch_stream<T, 8, false>(p, stream);
   }
 }
 
@@ -474,16 +1022,14 @@ void launch_t(const Params& p, int64_t rows, cudaStream_t stream) {
 void distill_launch(const DistillArgs& a, cudaStream_t stream) {
   check(a.in, a.K, "distill_loss");
   if (a.in.rows > 0) {
-    Params p{a.in.x, a.t_ids, a.t_lp, a.weights, a.in.ld, a.in.V, a.K, 0, a.tail,
+    Params p{a.in.x, a.t_ids, a.t_lp, a.weights, a.in.ld, a.in.V, a.K, a.in.rows, a.tail,
              (float)(1.4426950408889634 / a.temperature), (float)(1.0 / a.temperature),
              (float)((double)a.grad_scale / a.temperature), a.row_loss,
-             reinterpret_cast<float4*>(a.stats), a.grad};
+             reinterpret_cast<float4*>(a.stats), a.grad, nullptr};
     if (a.in.bf16)
-      a.grad ? launch_t<__nv_bfloat16, true>(p, a.in.rows, stream)
-             : launch_t<__nv_bfloat16, false>(p, a.in.rows, stream);
+      launch_t<__nv_bfloat16>(p, stream);
     else
-      a.grad ? launch_t<float, true>(p, a.in.rows, stream)
-             : launch_t<float, false>(p, a.in.rows, stream);
+      launch_t<float>(p, stream);
   }
   if (a.loss)
     launch_pdl(sum_rows_kernel, dim3(1), dim3(1024), 0, stream, nullptr, (const float*)a.row_loss,
@@ -499,11 +1045,11 @@ void distill_bwd_launch(const DistillBwdArgs& a, cudaStream_t stream) {
     const unsigned n = (unsigned)(a.in.rows - r0 < 65535 ? a.in.rows - r0 : 65535);
     BwdParams b{};
     b.f = Params{reinterpret_cast<const char*>(a.in.x) + r0 * a.in.ld * eb, a.t_ids + r0 * a.K,
-                 a.t_lp + r0 * a.K, a.weights ? a.weights + r0 : nullptr, a.in.ld, a.in.V, a.K, 0,
+                 a.t_lp + r0 * a.K, a.weights ? a.weights + r0 : nullptr, a.in.ld, a.in.V, a.K, n,
                  a.tail, (float)(1.4426950408889634 / a.temperature), (float)(1.0 / a.temperature),
                  (float)((double)a.g_scale / a.temperature), nullptr,
                  reinterpret_cast<float4*>(const_cast<float*>(a.stats)) + r0,
-                 reinterpret_cast<char*>(a.grad) + r0 * a.in.V * eb};
+                 reinterpret_cast<char*>(a.grad) + r0 * a.in.V * eb, nullptr};
     b.g = a.g_rows + r0 * a.g_stride;
     b.g_stride = a.g_stride;
     if (a.in.bf16)

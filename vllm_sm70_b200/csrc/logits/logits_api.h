@@ -59,7 +59,8 @@ struct DistillArgs {
   bool tail;
   float grad_scale;    // dL/d(row loss * weight): 1 (sum) or 1 / rows (mean)
   float* row_loss;     // [rows], times weight
-  float* stats;        // [rows, 4] for distill_bwd: m, M / s, outside coefficient, 1 (0: empty row)
+  float* stats;        // [rows, 4] for distill_bwd: m, M / s, outside coefficient,
+                       // the teacher's log-normaliser
   void* grad;          // [rows, V] contiguous or nullptr (forward only)
   float* loss;         // scalar: grad_scale * sum(row_loss), or nullptr
 };

@@ -52,6 +52,14 @@ __device__ __forceinline__ uint4 ldg_stream(const void* p) {
   return v;
 }
 
+// 16 bytes to shared memory behind the thread's back; both 16-byte aligned.
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+
 // Order-preserving 32-bit key: a larger value has a larger key, -0 and +0
 // the same; NaN has key 0, below every number's.
 __device__ __forceinline__ uint32_t key_of(float f) {
@@ -325,17 +333,9 @@ __device__ __forceinline__ void rebase(Acc& a, float m, float c) {
   a.m = m;
 }
 
-// max over the CTA of a float that is no NaN; `red` holds a float a warp.
-template <int NT>
-__device__ __forceinline__ float block_max(float v, float* red) {
-  const uint32_t k = __reduce_max_sync(0xffffffffu, key_of(v));
-  __syncthreads();  // red may still be read from before
-  if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = value_of(k);
-  __syncthreads();
-  float m = red[0];
-#pragma unroll
-  for (int w = 1; w < NT / 32; ++w) m = fmaxf(m, red[w]);
-  return m;
+// max over the warp of a float that is no NaN
+__device__ __forceinline__ float warp_max(float v) {
+  return value_of(__reduce_max_sync(0xffffffffu, key_of(v)));
 }
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
