@@ -148,6 +148,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> distill_loss(
   a.stats = stats.data_ptr<float>();
   a.grad = with_grad ? grad.data_ptr() : nullptr;
   a.loss = with_loss ? loss.data_ptr<float>() : nullptr;
+  a.counter = reinterpret_cast<int*>(loss.data_ptr<float>());  // until the loss is written
   distill_launch(a, stream_now());
   return {rows, stats, grad, loss};
 }

@@ -67,6 +67,7 @@ struct Params {
   float4* stats;
   void* grad;
   unsigned int* err;
+  int* taken;  // rows taken beyond the clusters' first
 };
 
 constexpr int kIds = kMaxTeacherK / 32;  // teacher entries a lane holds
@@ -300,8 +301,9 @@ __host__ __device__ __forceinline__ int warp_vectors(int per) {
   return (per + 32 * kWarps - 1) / (32 * kWarps) * 32;
 }
 
-// Loss and gradient of rows held in shared memory: CL CTAs a row, cluster
-// blockIdx.x / CL takes rows blockIdx.x / CL + i * gridDim.x / CL.
+// Loss and gradient of rows held in shared memory: CL CTAs a row. A cluster
+// begins with the row of its number and takes the others from a counter: some
+// SMs hold fewer CTAs than others, whose clusters are faster.
 template <typename T, int CL>
 __global__ void __launch_bounds__(NT, 3) distill_fused_kernel(const Params p) {
   using Tr = Traits<T>;
@@ -313,6 +315,7 @@ __global__ void __launch_bounds__(NT, 3) distill_fused_kernel(const Params p) {
   // row before, and only then writes over that.
   __shared__ unsigned long long parts[2][3][CL * kWarps];
   __shared__ unsigned long long xks[2][kMaxTeacherK];  // in the cluster's first CTA
+  __shared__ unsigned long long ahead[2][2];  // the next row, and its weight
   __shared__ uint64_t bar[2];
   __shared__ int t_id[2][kMaxTeacherK];  // as given
   __shared__ float t_lp[2][kMaxTeacherK];
@@ -327,13 +330,13 @@ __global__ void __launch_bounds__(NT, 3) distill_fused_kernel(const Params p) {
   }
   for (int i = threadIdx.x; i < 6 * CL * kWarps; i += NT) (&parts[0][0][0])[i] = 0ull;
   for (int i = threadIdx.x; i < 2 * kMaxTeacherK; i += NT) (&xks[0][0])[i] = 0ull;
+  if (threadIdx.x < 4) (&ahead[0][0])[threadIdx.x] = 0ull;
   if constexpr (CL > 1)
     asm volatile("barrier.cluster.arrive.release;" ::: "memory");
   else
     __syncthreads();
   pdl_wait();
   pdl_trigger();
-  const int64_t stride = gridDim.x / CL;
   // My warp's vectors of any row: [first, first + cap), those that exist.
   const int per = ((p.V + 2 * E - 2) / E + CL - 1) / CL, cap = warp_vectors(per);
   const int first = part * per + warp * cap, last = min(first + cap, (part + 1) * per);
@@ -370,37 +373,20 @@ __global__ void __launch_bounds__(NT, 3) distill_fused_kernel(const Params p) {
   }
   if constexpr (CL > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 
-  for (uint32_t n = 0; r < p.rows;) {  // n: rows that counted
-    const int64_t r_next = r + stride;
-    const float w_next = weight(r_next);
-    const Row<T> next(p.x, min(r_next, p.rows - 1), p.ld, p.V);
-    const int end = min(last, row.n_vec), end_next = w_next != 0.f ? min(last, next.n_vec) : first;
+  for (uint32_t n = 0; r < p.rows; ++n) {
+    const int end = w != 0.f ? min(last, row.n_vec) : first;
     T* out = reinterpret_cast<T*>(p.grad) + r * p.V;
-    if (w == 0.f) {  // uniform over the cluster
-      for (int u = first + lane; u < end; u += 32)
-        store_vec(out, row, u, make_uint4(0u, 0u, 0u, 0u));
-      if (part == 0 && threadIdx.x == 0) {
-        p.row_loss[r] = 0.f;
-        p.stats[r] = make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-      for (int u = first + lane; u < end_next; u += 32) fetch(next, u);
-      if (w_next != 0.f) fetch_teacher(r_next, n & 1);
-      r = r_next, w = w_next, row = next;
-      continue;
+    // The next row, by the time of the exchange.
+    int64_t r_next = 0;
+    float w_next = 0.f;
+    if (part == 0 && threadIdx.x == 0) {
+      r_next = p.rows;
+      if (p.taken) r_next = gridDim.x / CL + atomicAdd(p.taken, 1);
+      w_next = weight(r_next);
     }
     const int buf = n & 1;
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncwarp();
-    float norm, sum_p;
-    {
-      Teacher t;
-      t.load(t_id[buf], t_lp[buf], p.K);
-      t.prepare(p);
-      norm = t.norm, sum_p = t.sum_p;
-#pragma unroll
-      for (int i = 0; i < kIds; ++i)
-        if (lane + 32 * i < p.K) t_p[buf][lane + 32 * i] = t.p[i];
-    }
 
     // The teacher's elements of my part out of the row: value, then a tag of
     // the entry (repeated ids overwrite one another's), then -inf.
@@ -409,7 +395,7 @@ __global__ void __launch_bounds__(NT, 3) distill_fused_kernel(const Params p) {
 #pragma unroll 1
     for (int i = 0; 32 * i < p.K; ++i) {
       const int k = lane + 32 * i;
-      if (k >= p.K) break;
+      if (k >= p.K || w == 0.f) break;
       const int id = t_id[buf][k], at = id + row.pad;
       if (id >= 0 && id < p.V && at / E >= first && at / E < end) {
         const float x = Tr::to_f(elem[at]);
@@ -422,19 +408,19 @@ __global__ void __launch_bounds__(NT, 3) distill_fused_kernel(const Params p) {
     if (__any_sync(0xffffffffu, own != 0)) {
       __syncwarp();
 #pragma unroll 1
-      for (int i = 0; i < kIds; ++i)
+      for (int i = 0; 32 * i < p.K; ++i)
         if ((own >> i) & 1u)
           reinterpret_cast<Tag*>(elem)[t_id[buf][lane + 32 * i] + row.pad] = (Tag)(lane + 32 * i);
       __syncwarp();
       bool dup = false;
 #pragma unroll 1
-      for (int i = 0; i < kIds; ++i)
+      for (int i = 0; 32 * i < p.K; ++i)
         if ((own >> i) & 1u)
           dup |= reinterpret_cast<const Tag*>(elem)[t_id[buf][lane + 32 * i] + row.pad] !=
                  (Tag)(lane + 32 * i);
       __syncwarp();
 #pragma unroll 1
-      for (int i = 0; i < kIds; ++i)
+      for (int i = 0; 32 * i < p.K; ++i)
         if ((own >> i) & 1u)
           reinterpret_cast<Tag*>(elem)[t_id[buf][lane + 32 * i] + row.pad] = (Tag)Tr::kNegInf;
       if (__any_sync(0xffffffffu, dup)) own = first_of_ids(own, t_id[buf], p.K);
@@ -491,12 +477,20 @@ __global__ void __launch_bounds__(NT, 3) distill_fused_kernel(const Params p) {
         for (int e = 0; e < E; ++e) s += ex2((Tr::to_f(elem[u * E + e]) - m) * c);
     }
     float s_in = 0.f;
-#pragma unroll
-    for (int i = 0; i < kIds; ++i)
+#pragma unroll 1
+    for (int i = 0; 32 * i < p.K; ++i)
       if ((own >> i) & 1u) s_in += ex2((t_x[buf][lane + 32 * i] - shift_of(m_w)) * c);
     s = warp_sum(s);
     s_in = warp_sum(s_in);
     // To every CTA of the cluster; each warp hears from every other.
+    if (part == 0 && warp == 0) {
+      const int rn = __shfl_sync(0xffffffffu, (int)min(r_next, p.rows), 0);
+      const float wn = __shfl_sync(0xffffffffu, w_next, 0);
+      if (lane < CL) {
+        send<CL>(&ahead[buf][0], lane, __int_as_float(rn), n + 1);
+        send<CL>(&ahead[buf][1], lane, wn, n + 1);
+      }
+    }
     if (lane < CL) {
       send<CL>(&parts[buf][0][part * kWarps + warp], lane, m_w, n + 1);
       send<CL>(&parts[buf][1][part * kWarps + warp], lane, s, n + 1);
@@ -507,6 +501,17 @@ __global__ void __launch_bounds__(NT, 3) distill_fused_kernel(const Params p) {
         mbar_arrive(&bar[buf]);
       else
         mbar_arrive_cluster_relaxed(mapa_shared(smem_u32(&bar[buf]), lane));
+    }
+    // Meanwhile the teacher's probabilities.
+    float norm, sum_p;
+    {
+      Teacher t;
+      t.load(t_id[buf], t_lp[buf], w != 0.f ? p.K : 0);
+      t.prepare(p);
+      norm = t.norm, sum_p = t.sum_p;
+#pragma unroll
+      for (int i = 0; i < kIds; ++i)
+        if (lane + 32 * i < p.K) t_p[buf][lane + 32 * i] = t.p[i];
     }
     bool met = mbar_wait(&bar[buf], (n >> 1) & 1u, p.err);
     float4 got[2];
@@ -522,7 +527,25 @@ __global__ void __launch_bounds__(NT, 3) distill_fused_kernel(const Params p) {
     }
     __syncwarp();
 
+    float rn;
+    met &= receive(&ahead[buf][0], n + 1, rn, p.err);
+    met &= receive(&ahead[buf][1], n + 1, w_next, p.err);
+    if (!__all_sync(0xffffffffu, met)) break;  // (the status word is set)
+    r_next = __float_as_int(rn);
+    const Row<T> next(p.x, min(r_next, p.rows - 1), p.ld, p.V);
+    const int end_next = w_next != 0.f ? min(last, next.n_vec) : first;
     if (w_next != 0.f) fetch_teacher(r_next, buf ^ 1);
+    if (w == 0.f) {
+      if (part == 0 && threadIdx.x == 0) {
+        p.row_loss[r] = 0.f;
+        p.stats[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      for (int u = first + lane; u < min(last, row.n_vec); u += 32)
+        store_vec(out, row, u, make_uint4(0u, 0u, 0u, 0u));
+      for (int u = first + lane; u < end_next; u += 32) fetch(next, u);
+      r = r_next, w = w_next, row = next;
+      continue;
+    }
 
     // Every warp finishes the row's numbers (the same in all of them).
     const float3 q = join(got[0], got[1], c);
@@ -542,9 +565,9 @@ __global__ void __launch_bounds__(NT, 3) distill_fused_kernel(const Params p) {
       }
       t.sum_p = sum_p;
       const float loss = row_loss(t, p, q, xk);
-      met = __all_sync(0xffffffffu, met);
+      if (!__all_sync(0xffffffffu, met)) break;
       if (lane == 0) {
-        p.row_loss[r] = met ? loss * w : NAN;
+        p.row_loss[r] = loss * w;
         p.stats[r] = st;
       }
     }
@@ -586,7 +609,7 @@ __global__ void __launch_bounds__(NT, 3) distill_fused_kernel(const Params p) {
     }
     __syncwarp();
 #pragma unroll 1
-    for (int i = 0; i < kIds; ++i)
+    for (int i = 0; 32 * i < p.K; ++i)
       if ((own >> i) & 1u) {
         const int k = lane + 32 * i, id = t_id[buf][k];
         float mass = t_p[buf][k];
@@ -594,7 +617,6 @@ __global__ void __launch_bounds__(NT, 3) distill_fused_kernel(const Params p) {
         const float qk = ex2((t_x[buf][k] - st.x) * c) * st.y;
         out[id] = Tr::from_f((qk - (st.y == 0.f ? 0.f : mass)) * up);
       }
-    ++n;
     r = r_next, w = w_next, row = next;
   }
   // (No CTA leaves while another's exchange may still reach it.)
@@ -946,7 +968,7 @@ int slice_bytes(int V, int cl) {
 }
 
 template <typename T, int CL>
-void launch_fused(Params p, cudaStream_t stream) {
+void launch_fused(Params p, int* counter, cudaStream_t stream) {
   auto kernel = distill_fused_kernel<T, CL>;
   static bool attr[kMaxDevices] = {};
   set_smem_attr_once(kernel, kSmemMost, attr, "distill_loss");
@@ -975,6 +997,12 @@ void launch_fused(Params p, cudaStream_t stream) {
     known = Known{dev, smem, n};
   }
   const int64_t clusters = p.rows < known.clusters ? p.rows : known.clusters;
+  if (clusters < p.rows) {
+    p.taken = counter;
+    const cudaError_t e = cudaMemsetAsync(counter, 0, sizeof(int), stream);
+    if (e != cudaSuccess)
+      throw std::runtime_error(std::string("distill_loss: ") + cudaGetErrorString(e));
+  }
   launch_pdl(kernel, dim3((unsigned)(clusters * CL)), dim3(NT), smem, stream,
              CL > 1 ? &cl : nullptr, p);
 }
@@ -991,7 +1019,7 @@ void launch_stream(const Params& p, cudaStream_t stream) {
 }
 
 template <typename T>
-void launch_t(const Params& p, cudaStream_t stream) {
+void launch_t(const Params& p, int* counter, cudaStream_t stream) {
   int dev = 0;
   cudaGetDevice(&dev);
   const int sms = num_sms(dev);
@@ -999,10 +1027,10 @@ void launch_t(const Params& p, cudaStream_t stream) {
     int cl = row_split(p.rows, p.V / Traits<T>::E, sms, NT);
     while (cl < kMaxCluster && slice_bytes<T>(p.V, cl) > kSmemThree) cl *= 2;
     switch (cl) {
-      case 1: return launch_fused<T, 1>(p, stream);
-      case 2: return launch_fused<T, 2>(p, stream);
-      case 4: return launch_fused<T, 4>(p, stream);
-      default: return launch_fused<T, 8>(p, stream);
+      case 1: return launch_fused<T, 1>(p, counter, stream);
+      case 2: return launch_fused<T, 2>(p, counter, stream);
+      case 4: return launch_fused<T, 4>(p, counter, stream);
+      default: return launch_fused<T, 8>(p, counter, stream);
     }
   }
   if (p.grad) return launch_stream<T, 8, true>(p, stream);
@@ -1025,11 +1053,11 @@ void distill_launch(const DistillArgs& a, cudaStream_t stream) {
     Params p{a.in.x, a.t_ids, a.t_lp, a.weights, a.in.ld, a.in.V, a.K, a.in.rows, a.tail,
              (float)(1.4426950408889634 / a.temperature), (float)(1.0 / a.temperature),
              (float)((double)a.grad_scale / a.temperature), a.row_loss,
-             reinterpret_cast<float4*>(a.stats), a.grad, nullptr};
+             reinterpret_cast<float4*>(a.stats), a.grad, nullptr, nullptr};
     if (a.in.bf16)
-      launch_t<__nv_bfloat16>(p, stream);
+      launch_t<__nv_bfloat16>(p, a.counter, stream);
     else
-      launch_t<float>(p, stream);
+      launch_t<float>(p, a.counter, stream);
   }
   if (a.loss)
     launch_pdl(sum_rows_kernel, dim3(1), dim3(1024), 0, stream, nullptr, (const float*)a.row_loss,
@@ -1049,7 +1077,7 @@ void distill_bwd_launch(const DistillBwdArgs& a, cudaStream_t stream) {
                  a.tail, (float)(1.4426950408889634 / a.temperature), (float)(1.0 / a.temperature),
                  (float)((double)a.g_scale / a.temperature), nullptr,
                  reinterpret_cast<float4*>(const_cast<float*>(a.stats)) + r0,
-                 reinterpret_cast<char*>(a.grad) + r0 * a.in.V * eb, nullptr};
+                 reinterpret_cast<char*>(a.grad) + r0 * a.in.V * eb, nullptr, nullptr};
     b.g = a.g_rows + r0 * a.g_stride;
     b.g_stride = a.g_stride;
     if (a.in.bf16)

@@ -62,6 +62,7 @@ struct DistillArgs {
   float* stats;        // [rows, 4] for distill_bwd: m, M / s, outside coefficient,
                        // the teacher's log-normaliser
   void* grad;          // [rows, V] contiguous or nullptr (forward only)
+  int* counter;        // one int of scratch, with grad
   float* loss;         // scalar: grad_scale * sum(row_loss), or nullptr
 };
 void distill_launch(const DistillArgs& a, cudaStream_t stream);
