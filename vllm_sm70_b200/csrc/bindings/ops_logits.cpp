@@ -1,6 +1,7 @@
 // torch.ops._b200_C: operators over rows of logits (log-probabilities of
 // given tokens, distillation from a teacher's top values).
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
 #include <torch/torch.h>
@@ -14,6 +15,12 @@ namespace b200 {
 namespace {
 
 using OptTensor = c10::optional<at::Tensor>;
+
+// at::empty without the dispatcher: at few rows the outputs' allocations are
+// most of a call's time on the host.
+at::Tensor make(at::IntArrayRef size, const at::TensorOptions& o) {
+  return at::detail::empty_cuda(size, o);
+}
 
 cudaStream_t stream_now() { return at::cuda::getCurrentCUDAStream().stream(); }
 
@@ -61,9 +68,9 @@ Six token_logprobs(const at::Tensor& logits, const at::Tensor& ids, int64_t top_
   c10::cuda::CUDAGuard g(logits.device());
   const auto f = logits.options().dtype(at::kFloat), i = logits.options().dtype(at::kInt);
   const int64_t T = a.in.rows;
-  auto lp = at::empty({T}, f), ent = at::empty({T}, f), lse = at::empty({T}, f);
-  auto rank = at::empty({T}, i), stats = at::empty({T, 4}, f);
-  auto top_ids = at::empty({T, top_n}, i), top_lp = at::empty({T, top_n}, f);
+  auto lp = make({T}, f), ent = make({T}, f), lse = make({T}, f);
+  auto rank = make({T}, i), stats = make({T, 4}, f);
+  auto top_ids = make({T, top_n}, i), top_lp = make({T, top_n}, f);
   a.ids = ids.data_ptr();
   a.ids64 = ids.scalar_type() == at::kLong;
   a.top_n = (int)top_n;
@@ -95,7 +102,7 @@ at::Tensor token_logprobs_bwd(const at::Tensor& logits, const at::Tensor& ids,
       TORCH_CHECK((*t)->numel() == a.in.rows, what, ": upstream gradients must be [rows]");
     }
   c10::cuda::CUDAGuard g(logits.device());
-  auto grad = at::empty({a.in.rows, a.in.V}, logits.options());
+  auto grad = make({a.in.rows, a.in.V}, logits.options());
   a.ids = ids.data_ptr();
   a.ids64 = ids.scalar_type() == at::kLong;
   a.temperature = (float)temperature;
@@ -134,9 +141,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> distill_loss(
   check_temperature(temperature, what);
   c10::cuda::CUDAGuard g(logits.device());
   const auto f = logits.options().dtype(at::kFloat);
-  auto rows = at::empty({a.in.rows}, f), stats = at::empty({a.in.rows, 4}, f);
-  auto grad = at::empty({with_grad ? a.in.rows : 0, a.in.V}, logits.options());
-  auto loss = at::empty({}, f);
+  auto rows = make({a.in.rows}, f), stats = make({a.in.rows, 4}, f);
+  auto grad = make({with_grad ? a.in.rows : 0, a.in.V}, logits.options());
+  auto loss = make({}, f);
   a.t_ids = t_ids.data_ptr<int>();
   a.t_lp = t_lp.data_ptr<float>();
   a.K = (int)t_ids.size(1);
@@ -168,7 +175,7 @@ at::Tensor distill_loss_bwd(const at::Tensor& logits, const at::Tensor& t_ids,
   TORCH_CHECK(g_rows.dim() == 0 || g_rows.numel() == a.in.rows, what,
               ": the upstream gradient must be a scalar or [rows]");
   c10::cuda::CUDAGuard g(logits.device());
-  auto grad = at::empty({a.in.rows, a.in.V}, logits.options());
+  auto grad = make({a.in.rows, a.in.V}, logits.options());
   a.t_ids = t_ids.data_ptr<int>();
   a.t_lp = t_lp.data_ptr<float>();
   a.K = (int)t_ids.size(1);
