@@ -109,6 +109,15 @@ def test_wide_trees(b200_ops):
     _check(*_setup([300, 131], [100, 131], (16, 2, 256), 16))
 
 
+@pytest.mark.parametrize("heads", [(32, 8, 128), (16, 2, 256), (8, 2, 64)])
+@pytest.mark.parametrize("lens,nodes", [
+    ([5000, 300, 64], [64, 64, 64]),        # two tiles of rows at 4 heads a key head
+    ([9000], [96]), ([4000, 700], [128, 64]), ([900, 5, 3000], [64, 0, 128]),
+    ([1500] * 9, [256] * 9), ([2000, 2100], [300, 290])])
+def test_row_tiles_over_the_same_keys(b200_ops, heads, lens, nodes):
+    _check(*_setup(lens, nodes, heads, 16, seed=len(lens)))
+
+
 def test_ragged_batch_and_long_context(b200_ops):
     g = torch.Generator().manual_seed(3)
     lens = torch.randint(1, 900, (300,), generator=g).tolist()

@@ -22,6 +22,10 @@
 // kernel joins in share order; whole units are written directly. The split
 // depends on the lengths only, so results repeat bit for bit.
 //
+// Where every sequence has a multiple of `team` row tiles, the shares are those
+// of teams of that many CTAs: each takes another row tile over the same keys at
+// about the same time, which HBM then delivers once, and L2 to the others.
+//
 // Thirteen warps a CTA:
 //   warp 0     K producer, warp 1 V producer: one (cache block, 64-column)
 //              box a lane, one warp-wide bulk-tensor instruction a tile (that
@@ -75,6 +79,7 @@ constexpr int kSoftmaxWarps = 8;
 constexpr int kBarBytes = 1024;  // barriers and published units
 constexpr int kUnits = 4;       // published units
 constexpr int kRowBytes = 3 * FM * 4;  // a reference and two sums a row
+constexpr int kMaxTeam = 8;  // CTAs that read the same keys
 constexpr int kMinShare = 2;  // key tiles of a CTA, at least
 
 template <int D_>
@@ -99,7 +104,7 @@ struct Cfg {
 // pieces up to the one of CTA `last`.
 struct __align__(16) Cut {
   int q0, kvh, row0, rows;
-  int last, pad[3];
+  int last, step, pad[2];  // step: from one of its CTAs to the next
 };
 
 struct Params {
@@ -178,22 +183,29 @@ __device__ __forceinline__ Seq share_seq(const Seq& q, int l) {
 }
 
 // The units of a CTA's share, in order: unit = key head * n_rt + row tile,
-// key tiles [j0, j1) of it.
+// key tiles [j0, j1) of it. Of `team` row tiles that are taken together, this
+// is the sub-th.
 template <int FN>
 struct Walk {
   int s, unit, j0, j1, kvh, row0;
   int off, left;
+  int team, sub;
   Seq q;
+  __device__ __forceinline__ void set(const Seq& x) {
+    q = x;
+    q.n_rt /= team;
+    q.total /= team;
+  }
   __device__ __forceinline__ bool next(const Params& p) {
     if (left <= 0) return false;
     while (off >= q.total) {
       if (++s >= p.num_seqs) return false;
-      q = load_seq<FN>(p, s);
+      set(load_seq<FN>(p, s));
       off = 0;
     }
     unit = off / q.n_tiles;
     kvh = unit / q.n_rt;
-    row0 = (unit - kvh * q.n_rt) * FM;
+    row0 = ((unit - kvh * q.n_rt) * team + sub) * FM;
     j0 = off - unit * q.n_tiles;
     const int n = min(q.n_tiles - j0, left);
     j1 = j0 + n;
@@ -357,12 +369,16 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
     int share = 0;
     if (!is_v) {
       long long total = 0, sums = 0;
+      uint32_t by = (2u << kMaxTeam) - 1u;  // bit d: d divides every number of row tiles
       Seq mine;
       for (int b = 0; b < p.num_seqs; b += 32) {
         long long c = 0;
         if (b + lane < p.num_seqs) {
           const Seq q = load_seq<FN>(p, b + lane);
           c = q.total;
+#pragma unroll
+          for (int d = 2; d <= kMaxTeam; ++d)
+            if (q.n_rt % d) by &= ~(1u << d);
           if (b == 0) mine = q;
         }
 #pragma unroll
@@ -373,9 +389,13 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
         if (b == 0) sums = c;
         total += __shfl_sync(0xffffffffu, c, 31);
       }
-      const long long per =
-          max((long long)kMinShare, (total + gridDim.x - 1) / (long long)gridDim.x);
-      const long long t0 = per * blockIdx.x, n = min(per, total - t0);
+      const int team = 31 - __clz(__reduce_and_sync(0xffffffffu, by));
+      walk.team = team;
+      walk.sub = (int)blockIdx.x % team;
+      total /= team;
+      const int teams = (int)gridDim.x / team, me = (int)blockIdx.x / team;
+      const long long per = max((long long)kMinShare, (total + teams - 1) / teams);
+      const long long t0 = per * me, n = me < teams ? min(per, total - t0) : 0;
       share = (int)per;
       walk.left = (int)max(0ll, n);
       walk.s = walk.off = 0;
@@ -396,12 +416,12 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
           }
         }
         const long long before = __shfl_up_sync(0xffffffffu, c, 1);
-        const uint32_t hit = __ballot_sync(0xffffffffu, seen + c > t0);
+        const uint32_t hit = __ballot_sync(0xffffffffu, seen + c > t0 * team);
         if (hit) {
           const int l = __ffs(hit) - 1;
           walk.s = b + l;
-          walk.off = (int)(t0 - seen - __shfl_sync(0xffffffffu, lane > 0 ? before : 0, l));
-          walk.q = share_seq(mine, l);
+          walk.off = (int)(t0 - (seen + __shfl_sync(0xffffffffu, lane > 0 ? before : 0, l)) / team);
+          walk.set(share_seq(mine, l));
           found = true;
         }
         seen += __shfl_sync(0xffffffffu, c, 31);
@@ -437,8 +457,10 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
           // Tiles of the unit from its first on; an earlier edge than this
           // one joins a unit that began more than a share before.
           const bool mine = more && x.j0 > 0 && x.j0 <= share;
-          const int last = (int)blockIdx.x + (walk.q.n_tiles - x.j0 - 1) / max(share, 1);
-          p.cut[blockIdx.x] = Cut{x.q0, x.kvh, x.row0, mine ? min(FM, x.rows) : 0, last, {0, 0, 0}};
+          const int last =
+              (int)blockIdx.x + (walk.q.n_tiles - x.j0 - 1) / max(share, 1) * walk.team;
+          p.cut[blockIdx.x] = Cut{x.q0, x.kvh,     x.row0, mine ? min(FM, x.rows) : 0,
+                                  last, walk.team, {0, 0}};
         }
       }
       ++published;
@@ -929,9 +951,9 @@ __global__ void __launch_bounds__(kJoinRows * 32) tree_join_kernel(const Params 
   if (row >= cut.rows) return;
   const int g = cut.row0 + row, t = g / p.G, head = cut.kvh * p.G + g - t * p.G;
   const bool on = D >= 128 || lane < D / 4;
-  const int n = cut.last - c1 + 2;
-  // Piece i: the first is the last of share c1 - 1, the others open theirs.
-  auto piece = [&](int i) { return ((long long)(c1 - 1 + i) * 2 + (i == 0 ? 1 : 0)) * FM + row; };
+  const int n = (cut.last - c1) / cut.step + 2;
+  // Piece i: the first is the last of the share before, the others open theirs.
+  auto piece = [&](int i) { return ((long long)(c1 + (i - 1) * cut.step) * 2 + (i == 0 ? 1 : 0)) * FM + row; };
   float m = -INFINITY;
   for (int i = lane; i < n; i += 32) m = fmaxf(m, p.part_ml[piece(i)].x);
   float den = 0.f;
