@@ -45,7 +45,7 @@ constexpr int U = 4;          // vectors of a thread worked on at a time
 constexpr int kCand = 512;    // elements above tau kept before tau is raised
 constexpr int kEq = 256;      // elements equal to tau kept before they are found in id order
 constexpr int kHits = 512;    // groups read again by themselves; more: the whole slice
-constexpr int kSlots = 64;    // maxima of groups kept a thread
+constexpr int kSlots = 64;    // groups of a thread where CTAs can be added
 constexpr int kMaxCluster = 8;
 
 struct FwdParams {
@@ -54,7 +54,6 @@ struct FwdParams {
   int64_t ld;
   int V, top_n;
   bool ids64;
-  int shift;       // groups of a slot, as a power of two
   float c, inv_t;  // log2(e) / T, 1 / T
   float* logprob;
   int* rank;
@@ -69,7 +68,7 @@ struct Smem {
   Acc acc[kWarps];
   int cnt[kWarps];
   uint32_t jth[kWarps];        // each warp's j-th largest maximum
-  int hit[kHits];              // slot * NT + thread of groups that reach tau
+  int hit[kHits];              // group * NT + thread of those that reach tau
   unsigned long long cand[kCand + kEq];
   int eq[kEq];
   int scan[kWarps];
@@ -100,15 +99,14 @@ __device__ __forceinline__ uint32_t find_tau(const Smem& sm, int n) {
 // Calls f(key, id) for every element of the groups in sm.hit.
 template <typename T, typename F>
 __device__ __forceinline__ void visit(const Smem& sm, const Row<T>& row, const Slice& sl,
-                                      int shift, F f) {
+                                      F f) {
   const int n_groups = (sl.b - sl.a + U * NT - 1) / (U * NT);
   const bool all = sm.n_hit > kHits;
-  const int n = all ? sl.hi - sl.lo : (sm.n_hit * U) << shift;
+  const int n = all ? sl.hi - sl.lo : sm.n_hit * U;
   for (int w = threadIdx.x; w < n; w += NT) {
     int u = sl.lo + w;
     if (!all) {
-      const int h = sm.hit[(w / U) >> shift];
-      const int it = ((h / NT) << shift) + ((w / U) & ((1 << shift) - 1)), k = w % U, t = h % NT;
+      const int h = sm.hit[w / U], it = h / NT, t = h % NT, k = w % U;
       u = sl.a + (it * U + k) * NT + t;
       if (it == n_groups) u = k > 0 ? -1 : t == 0 ? sl.head : t == 1 ? sl.tail : -1;
       else if (u >= sl.b) u = -1;
@@ -130,9 +128,9 @@ __device__ __forceinline__ void visit(const Smem& sm, const Row<T>& row, const S
 // the ids of those equal to it into sm.eq (up to kEq; sm.n_eq counts them).
 // The order in which they arrive does not matter: the lists are ranked.
 template <typename T>
-__device__ __forceinline__ void collect(Smem& sm, const Row<T>& row, const Slice& sl, int shift,
+__device__ __forceinline__ void collect(Smem& sm, const Row<T>& row, const Slice& sl,
                                         uint32_t tau) {
-  visit(sm, row, sl, shift, [&](uint32_t k, int id) {
+  visit(sm, row, sl, [&](uint32_t k, int id) {
     if (k > tau) {
       const int at = atomicAdd(&sm.n_gt, 1);
       if (at < kCand) sm.cand[at] = entry(k, id);
@@ -147,7 +145,7 @@ __device__ __forceinline__ void collect(Smem& sm, const Row<T>& row, const Slice
 // Exact n-th largest key among the elements of the groups in sm.hit (more
 // than n of them lie above the present tau).
 template <typename T>
-__device__ __noinline__ uint32_t raise_tau(Smem& sm, Row<T> row, Slice sl, int shift, int n) {
+__device__ __noinline__ uint32_t raise_tau(Smem& sm, Row<T> row, Slice sl, int n) {
   uint32_t tau = 0;
   for (int b = 31; b >= 0; --b) {
     const uint32_t cand = tau | (1u << b);
@@ -155,7 +153,7 @@ __device__ __noinline__ uint32_t raise_tau(Smem& sm, Row<T> row, Slice sl, int s
     if (threadIdx.x == 0) sm.n_at = 0;
     __syncthreads();
     int c = 0;
-    visit(sm, row, sl, shift, [&](uint32_t k, int) { c += k >= cand ? 1 : 0; });
+    visit(sm, row, sl, [&](uint32_t k, int) { c += k >= cand ? 1 : 0; });
     c = __reduce_add_sync(0xffffffffu, c);
     if (threadIdx.x % 32 == 0 && c) atomicAdd(&sm.n_at, c);
     __syncthreads();
@@ -286,8 +284,6 @@ __global__ void __launch_bounds__(NT, 4) token_logprobs_kernel(const FwdParams p
   // it are counted on their own.
   const bool y_masked = xy == -INFINITY;
   extern __shared__ uint16_t slots[];
-  const int shift = p.shift;
-  float slot_max = -INFINITY;
   int n_slots = 0;
   for_groups<NT, U>(row, sl, [&](const uint4(&v)[U], int u, int it) {
     typename Tr::Max vm[U];
@@ -297,9 +293,8 @@ __global__ void __launch_bounds__(NT, 4) token_logprobs_kernel(const FwdParams p
     const float mx = Tr::value(Tr::vmax(Tr::vmax(vm[0], vm[1]), Tr::vmax(vm[2], vm[3])));
     if constexpr (TOP) {
       // The upper half of the float keeps the order.
-      slot_max = (it & ((1 << shift) - 1)) == 0 ? mx : fmaxf(slot_max, mx);
-      slots[(it >> shift) * NT + tid] = (uint16_t)(__float_as_uint(slot_max) >> 16);
-      n_slots = (it >> shift) + 1;
+      slots[it * NT + tid] = (uint16_t)(__float_as_uint(mx) >> 16);
+      n_slots = it + 1;
     }
     if (mx > m) {
       const float rn = __fmul_rn(fmaxf(mx, kFloor), c), d = r0 - rn;
@@ -453,10 +448,10 @@ __global__ void __launch_bounds__(NT, 4) token_logprobs_kernel(const FwdParams p
         }
     }
     __syncthreads();
-    collect(sm, row, sl, shift, tau);
+    collect(sm, row, sl, tau);
     if (sm.n_gt > kCand) {
-      tau = raise_tau(sm, row, sl, shift, n);
-      collect(sm, row, sl, shift, tau);
+      tau = raise_tau(sm, row, sl, n);
+      collect(sm, row, sl, tau);
     }
     const int n_gt = min(sm.n_gt, kCand);
     n_list = n_gt;
@@ -609,8 +604,18 @@ __global__ void __launch_bounds__(NT) token_logprobs_bwd_kernel(const BwdParams 
   }
 }
 
+// Groups of a thread where CL CTAs share a row, a last one for the partial
+// vectors among them.
+template <typename T>
+int groups_of(int V, int cl) {
+  const int n_vec = (V + 2 * Traits<T>::E - 2) / Traits<T>::E;
+  return ((n_vec + cl - 1) / cl + U * NT - 1) / (U * NT) + 1;
+}
+// Their maxima's bytes at the largest vocabulary, 8 CTAs a row.
+constexpr int kSlotBytes = ((kMaxVocab / 4 + 2) / kMaxCluster / (U * NT) + 2) * NT * 2;
+
 template <typename T, int CL>
-void launch_fwd(FwdParams p, int64_t rows, cudaStream_t stream) {
+void launch_fwd(const FwdParams& p, int64_t rows, cudaStream_t stream) {
   cudaLaunchAttribute cl;
   cl.id = cudaLaunchAttributeClusterDimension;
   cl.val.clusterDim.x = CL;
@@ -618,12 +623,9 @@ void launch_fwd(FwdParams p, int64_t rows, cudaStream_t stream) {
   const dim3 grid((unsigned)(rows * CL));
   const cudaLaunchAttribute* extra = CL > 1 ? &cl : nullptr;
   auto kernel = p.top_n > 0 ? token_logprobs_kernel<T, CL, true> : token_logprobs_kernel<T, CL, false>;
-  // Groups of a thread, a last one for the partial vectors among them.
-  const int n_vec = (p.V + 2 * Traits<T>::E - 2) / Traits<T>::E;
-  const int groups = ((n_vec + CL - 1) / CL + U * NT - 1) / (U * NT) + 1;
-  p.shift = 0;
-  while ((groups - 1) >> p.shift >= kSlots) ++p.shift;
-  const int smem = p.top_n > 0 ? (((groups - 1) >> p.shift) + 1) * NT * 2 : 0;
+  static bool attr[kMaxDevices] = {};
+  if (p.top_n > 0) set_smem_attr_once(kernel, kSlotBytes, attr, "token_logprobs");
+  const int smem = p.top_n > 0 ? groups_of<T>(p.V, CL) * NT * 2 : 0;
   launch_pdl(kernel, grid, dim3(NT), smem, stream, extra, p);
 }
 
@@ -631,7 +633,10 @@ template <typename T>
 void launch_fwd_t(const FwdParams& p, int64_t rows, cudaStream_t stream) {
   int dev = 0;
   cudaGetDevice(&dev);
-  switch (row_split(rows, p.V / Traits<T>::E, 2 * num_sms(dev), NT)) {
+  int cl = row_split(rows, p.V / Traits<T>::E, 2 * num_sms(dev), NT);
+  // (32 KB of maxima a CTA: four an SM)
+  while (p.top_n > 0 && cl < kMaxCluster && groups_of<T>(p.V, cl) > kSlots) cl *= 2;
+  switch (cl) {
     case 1: return launch_fwd<T, 1>(p, rows, stream);
     case 2: return launch_fwd<T, 2>(p, rows, stream);
     case 4: return launch_fwd<T, 4>(p, rows, stream);
@@ -653,7 +658,7 @@ void token_logprobs_launch(const TokenLogprobsArgs& a, cudaStream_t stream) {
     throw std::runtime_error("token_logprobs: top_n must be in [0, min(64, vocabulary)]");
   if (a.in.rows <= 0) return;
   FwdParams p{a.in.x,  a.ids,       a.in.ld,    a.in.V,
-              a.top_n, a.ids64,     0, (float)(1.4426950408889634 / a.temperature), (float)(1.0 / a.temperature),
+              a.top_n, a.ids64,     (float)(1.4426950408889634 / a.temperature), (float)(1.0 / a.temperature),
               a.logprob, a.rank,    a.entropy,  a.lse,
               a.top_ids, a.top_lp,  reinterpret_cast<float4*>(a.stats)};
   if (a.in.bf16)
