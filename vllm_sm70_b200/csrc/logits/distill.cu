@@ -275,16 +275,25 @@ __device__ __forceinline__ void send(unsigned long long* to, int rank, float v, 
                  "l"(word_of(v, seq))
                  : "memory");
 }
+__device__ __forceinline__ unsigned long long peek(unsigned long long* from) {
+  unsigned long long q;
+  asm volatile("ld.relaxed.cluster.shared::cta.b64 %0, [%1];"
+               : "=l"(q)
+               : "r"(smem_u32(from))
+               : "memory");
+  return q;
+}
+__device__ __forceinline__ float value_in(unsigned long long word) {
+  return __uint_as_float((uint32_t)word);
+}
 // Waits for the word of exchange `seq` (2 s at most, see mbar_wait); false
 // where it does not come.
-__device__ __forceinline__ bool receive(unsigned long long* from, uint32_t seq, float& v,
-                                        unsigned int* err) {
+__device__ __forceinline__ bool receive(unsigned long long* from, uint32_t seq,
+                                        unsigned long long& word, unsigned int* err) {
   unsigned long long t0 = 0;
   for (uint32_t spins = 0;; ++spins) {
-    unsigned long long q;
-    asm volatile("ld.relaxed.cluster.shared::cta.b64 %0, [%1];" : "=l"(q) : "r"(smem_u32(from)) : "memory");
-    v = __uint_as_float((uint32_t)q);
-    if ((uint32_t)(q >> 32) == seq) return true;
+    word = peek(from);
+    if ((uint32_t)(word >> 32) == seq) return true;
     if ((spins & 63u) == 63u) {
       if (t0 == 0) t0 = globaltimer();
       if (globaltimer() - t0 > kWaitTimeoutNs) {
@@ -392,38 +401,45 @@ __global__ void __launch_bounds__(NT, 3) distill_fused_kernel(const Params p) {
     // the entry (repeated ids overwrite one another's), then -inf.
     uint32_t own = 0;  // entries lane + 32 i here, the first of their id
     float m_k = -INFINITY;
-#pragma unroll 1
-    for (int i = 0; 32 * i < p.K; ++i) {
-      const int k = lane + 32 * i;
-      if (k >= p.K || w == 0.f) break;
-      const int id = t_id[buf][k], at = id + row.pad;
-      if (id >= 0 && id < p.V && at / E >= first && at / E < end) {
-        const float x = Tr::to_f(elem[at]);
-        t_x[buf][k] = x;
-        m_k = fmaxf(m_k, x);
-        own |= 1u << i;
-        send<CL>(&xks[buf][k], 0, x, n + 1);
+    int at[kIds], here = 0;
+#pragma unroll
+    for (int i = 0; i < kIds; ++i) {
+      at[i] = -1;
+      if (32 * i < p.K && w != 0.f) {
+        const int k = lane + 32 * i, id = k < p.K ? t_id[buf][k] : -1;
+        const bool in = id >= 0 && id < p.V &&
+                        (uint32_t)(id + row.pad - first * E) < (uint32_t)(max(end - first, 0) * E);
+        if (in) at[i] = id + row.pad;
+        here += __popc(__ballot_sync(0xffffffffu, in));
       }
     }
-    if (__any_sync(0xffffffffu, own != 0)) {
-      __syncwarp();
-#pragma unroll 1
-      for (int i = 0; 32 * i < p.K; ++i)
-        if ((own >> i) & 1u)
-          reinterpret_cast<Tag*>(elem)[t_id[buf][lane + 32 * i] + row.pad] = (Tag)(lane + 32 * i);
+    if (here > 0) {
+#pragma unroll
+      for (int i = 0; i < kIds; ++i)
+        if (at[i] >= 0) {
+          const float x = Tr::to_f(elem[at[i]]);
+          t_x[buf][lane + 32 * i] = x;
+          m_k = fmaxf(m_k, x);
+          own |= 1u << i;
+          send<CL>(&xks[buf][lane + 32 * i], 0, x, n + 1);
+        }
       __syncwarp();
       bool dup = false;
-#pragma unroll 1
-      for (int i = 0; 32 * i < p.K; ++i)
-        if ((own >> i) & 1u)
-          dup |= reinterpret_cast<const Tag*>(elem)[t_id[buf][lane + 32 * i] + row.pad] !=
-                 (Tag)(lane + 32 * i);
-      __syncwarp();
-#pragma unroll 1
-      for (int i = 0; 32 * i < p.K; ++i)
-        if ((own >> i) & 1u)
-          reinterpret_cast<Tag*>(elem)[t_id[buf][lane + 32 * i] + row.pad] = (Tag)Tr::kNegInf;
-      if (__any_sync(0xffffffffu, dup)) own = first_of_ids(own, t_id[buf], p.K);
+      if (here > 1) {
+#pragma unroll
+        for (int i = 0; i < kIds; ++i)
+          if (at[i] >= 0) reinterpret_cast<Tag*>(elem)[at[i]] = (Tag)(lane + 32 * i);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < kIds; ++i)
+          if (at[i] >= 0)
+            dup |= reinterpret_cast<const Tag*>(elem)[at[i]] != (Tag)(lane + 32 * i);
+        dup = __any_sync(0xffffffffu, dup);
+      }
+#pragma unroll
+      for (int i = 0; i < kIds; ++i)
+        if (at[i] >= 0) reinterpret_cast<Tag*>(elem)[at[i]] = (Tag)Tr::kNegInf;
+      if (dup) own = first_of_ids(own, t_id[buf], p.K);
       __syncwarp();
     }
 
@@ -514,24 +530,39 @@ __global__ void __launch_bounds__(NT, 3) distill_fused_kernel(const Params p) {
         if (lane + 32 * i < p.K) t_p[buf][lane + 32 * i] = t.p[i];
     }
     bool met = mbar_wait(&bar[buf], (n >> 1) & 1u, p.err);
+    // (All words first: they are there as a rule.)
+    constexpr int kParts = CL * kWarps, kMine = (kParts + 31) / 32;
+    unsigned long long word[3 * kMine + 2];
+#pragma unroll
+    for (int i = 0; i < kMine; ++i)
+#pragma unroll
+      for (int e = 0; e < 3; ++e)
+        word[3 * i + e] = peek(&parts[buf][e][min(lane + 32 * i, kParts - 1)]);
+    word[3 * kMine] = peek(&ahead[buf][0]);
+    word[3 * kMine + 1] = peek(&ahead[buf][1]);
+    bool there = true;
+#pragma unroll
+    for (int i = 0; i < 3 * kMine + 2; ++i) there &= (uint32_t)(word[i] >> 32) == n + 1;
+    if (!there) {
+#pragma unroll
+      for (int i = 0; i < kMine; ++i)
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+          met &= receive(&parts[buf][e][min(lane + 32 * i, kParts - 1)], n + 1, word[3 * i + e], p.err);
+      met &= receive(&ahead[buf][0], n + 1, word[3 * kMine], p.err);
+      met &= receive(&ahead[buf][1], n + 1, word[3 * kMine + 1], p.err);
+    }
     float4 got[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       got[i] = make_float4(-INFINITY, 0.f, 0.f, 0.f);
-      const int from = lane + 32 * i;
-      if (from < CL * kWarps) {
-        met &= receive(&parts[buf][0][from], n + 1, got[i].x, p.err);
-        met &= receive(&parts[buf][1][from], n + 1, got[i].y, p.err);
-        met &= receive(&parts[buf][2][from], n + 1, got[i].z, p.err);
-      }
+      if (i < kMine && lane + 32 * i < kParts)
+        got[i] = make_float4(value_in(word[3 * i]), value_in(word[3 * i + 1]),
+                             value_in(word[3 * i + 2]), 0.f);
     }
-    __syncwarp();
-
-    float rn;
-    met &= receive(&ahead[buf][0], n + 1, rn, p.err);
-    met &= receive(&ahead[buf][1], n + 1, w_next, p.err);
+    w_next = value_in(word[3 * kMine + 1]);
     if (!__all_sync(0xffffffffu, met)) break;  // (the status word is set)
-    r_next = __float_as_int(rn);
+    r_next = __float_as_int(value_in(word[3 * kMine]));
     const Row<T> next(p.x, min(r_next, p.rows - 1), p.ld, p.V);
     const int end_next = w_next != 0.f ? min(last, next.n_vec) : first;
     if (w_next != 0.f) fetch_teacher(r_next, buf ^ 1);
@@ -560,7 +591,11 @@ __global__ void __launch_bounds__(NT, 3) distill_fused_kernel(const Params p) {
         t.lp[i] -= norm;
         if (lane + 32 * i < p.K) {
           t.p[i] = t_p[buf][lane + 32 * i];
-          if (t.id[i] >= 0 && t.id[i] < p.V) met &= receive(&xks[buf][lane + 32 * i], n + 1, xk[i], p.err);
+          if (t.id[i] >= 0 && t.id[i] < p.V) {
+            unsigned long long x;
+            met &= receive(&xks[buf][lane + 32 * i], n + 1, x, p.err);
+            xk[i] = value_in(x);
+          }
         }
       }
       t.sum_p = sum_p;
