@@ -10,7 +10,9 @@
 // what was seen: e_j = 2^((x_j - m) c), c = log2(e) / T. x_j - m is rounded
 // once, relative to itself, so elements near the top are exact to 2^-24 however
 // large m is, and m may be the type's lowest value (m c would overflow).
-// p_j = e_j / s, log p_j = ((x_j - m) c - log2 s) ln 2.
+// p_j = e_j / s, log p_j = ((x_j - m) c - log2 s) ln 2. The long sums take one
+// fused product x_j c - r instead, r the rounded m c: what r lacks of m c is
+// known exactly (one more fused product) and taken out of the sum at the end.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
