@@ -327,6 +327,34 @@ def test_scalar_upstream_and_second_backward(b200_ops):
     torch.testing.assert_close(g2, g1, atol=1e-9, rtol=1e-5)
 
 
+@pytest.mark.parametrize("reduction", ["none", "mean"])
+def test_differentiable_once(b200_ops, reduction):
+    x = _rows(5, 777, torch.float32, 8).requires_grad_(True)
+    ids, lp = _teacher(5, 777, 4, 1)
+    y = torch.arange(5, device="cuda")
+    for loss in (ops.distill_loss(x, ids, lp, reduction=reduction).sum(),
+                 ops.token_logprobs(x, y).logprobs.sum()):
+        g, = torch.autograd.grad(loss, x, create_graph=True)
+        assert torch.isfinite(g).all()
+        with pytest.raises(RuntimeError, match="cannot be differentiated again"):
+            g.sum().backward()
+
+
+def test_launches_are_counted(b200_ops):
+    from vllm_sm70_b200.utils import launch_count
+    x = _rows(5, 777, torch.bfloat16, 8).requires_grad_(True)
+    ids, lp = _teacher(5, 777, 4, 1)
+    ops.distill_loss(x, ids, lp)  # (the first call adds the native counter)
+    before = launch_count.total()
+    loss = ops.distill_loss(x, ids, lp)
+    assert launch_count.total() - before == 2
+    loss.backward()
+    assert launch_count.total() - before == 3
+    with torch.no_grad():
+        ops.token_logprobs(x, torch.arange(5, device="cuda"))
+    assert launch_count.total() - before == 4
+
+
 def test_same_bits_twice_and_other_stream(b200_ops):
     x = _rows(40, 70001, torch.bfloat16, 12)
     y = torch.arange(40, device="cuda") * 31

@@ -3,9 +3,11 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 #include <torch/torch.h>
 
+#include <atomic>
 #include <cmath>
 #include <tuple>
 
@@ -202,10 +204,164 @@ void scale_by(at::Tensor& x, const at::Tensor& scale) {
   scale_by_launch(x.data_ptr(), bf, x.numel(), scale.data_ptr<float>(), stream_now());
 }
 
+// ---------------------------------------------------------------- training
+// The autograd functions stand here and not in Python: at few rows a step is
+// the host's time, and a backward pass that holds no Python function needs no
+// change of threads for the interpreter (a step of 33 x 32003: 99 -> 85 us).
+using torch::autograd::AutogradContext;
+using torch::autograd::Function;
+using torch::autograd::variable_list;
+
+std::atomic<int64_t> g_backward_launches{0};
+int64_t backward_launches() { return g_backward_launches.load(); }
+
+// Through the dispatcher, so that fakes trace.
+template <typename F>
+c10::TypedOperatorHandle<F> handle(const char* name) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
+}
+Six call_token_logprobs(const at::Tensor& x, const at::Tensor& ids, int64_t top_n, double t) {
+  static auto op = handle<decltype(token_logprobs)>("_b200_C::token_logprobs");
+  return op.call(x, ids, top_n, t);
+}
+at::Tensor call_token_logprobs_bwd(const at::Tensor& x, const at::Tensor& ids,
+                                   const at::Tensor& stats, const OptTensor& g_lp,
+                                   const OptTensor& g_ent, double t) {
+  static auto op = handle<decltype(token_logprobs_bwd)>("_b200_C::token_logprobs_bwd");
+  g_backward_launches += 1;
+  return op.call(x, ids, stats, g_lp, g_ent, t);
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> call_distill(
+    const at::Tensor& x, const at::Tensor& ids, const at::Tensor& lp, const OptTensor& w, double t,
+    bool tail, double scale, bool with_loss, bool with_grad) {
+  static auto op = handle<decltype(distill_loss)>("_b200_C::distill_loss");
+  return op.call(x, ids, lp, w, t, tail, scale, with_loss, with_grad);
+}
+at::Tensor call_distill_bwd(const at::Tensor& x, const at::Tensor& ids, const at::Tensor& lp,
+                            const OptTensor& w, double t, bool tail, const at::Tensor& stats,
+                            const at::Tensor& g, double scale) {
+  static auto op = handle<decltype(distill_loss_bwd)>("_b200_C::distill_loss_bwd");
+  g_backward_launches += 1;
+  return op.call(x, ids, lp, w, t, tail, stats, g, scale);
+}
+void call_scale_by(at::Tensor& x, const at::Tensor& f) {
+  static auto op = handle<decltype(scale_by)>("_b200_C::scale_by");
+  g_backward_launches += 1;
+  op.call(x, f);
+}
+
+OptTensor opt(const at::Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+
+// A gradient that a graph of gradients may hold, and that raises where it is
+// differentiated itself.
+at::Tensor once(at::Tensor grad) {
+  if (!at::GradMode::is_enabled()) return grad;
+  auto error = std::make_shared<torch::autograd::DelayedError>(
+      "this operator's gradient cannot be differentiated again", 1);
+  grad = grad.detach();
+  grad.set_requires_grad(true);
+  return (*error)({grad})[0];
+}
+
+struct TokenLogprobsFn : public Function<TokenLogprobsFn> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& ids,
+                               int64_t top_n, double t) {
+    auto [lp, rank, ent, lse, top_ids, top_lp, stats] = call_token_logprobs(x, ids, top_n, t);
+    ctx->save_for_backward({x, ids, stats});
+    ctx->saved_data["t"] = t;
+    ctx->mark_non_differentiable({rank, lse, top_ids, top_lp});
+    ctx->set_materialize_grads(false);
+    return {lp, rank, ent, lse, top_ids, top_lp};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    if (!g[0].defined() && !g[2].defined()) return variable_list(4);
+    const auto saved = ctx->get_saved_variables();
+    at::AutoDispatchBelowADInplaceOrView guard;
+    const at::Tensor lp = g[0].defined() ? g[0].contiguous() : at::Tensor();
+    const at::Tensor ent = g[2].defined() ? g[2].contiguous() : at::Tensor();
+    at::Tensor grad = call_token_logprobs_bwd(saved[0], saved[1], saved[2], opt(lp), opt(ent),
+                                              ctx->saved_data["t"].toDouble());
+    return {once(grad), at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+struct DistillRowsFn : public Function<DistillRowsFn> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& ids,
+                            const at::Tensor& lp, const OptTensor& w, double t, bool tail) {
+    auto [rows, stats, grad, loss] = call_distill(x, ids, lp, w, t, tail, 1.0, false, false);
+    ctx->save_for_backward({x, ids, lp, w ? *w : at::Tensor(), stats});
+    ctx->saved_data["t"] = t;
+    ctx->saved_data["tail"] = tail;
+    return rows;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const auto s = ctx->get_saved_variables();
+    at::AutoDispatchBelowADInplaceOrView guard;
+    at::Tensor grad = call_distill_bwd(s[0], s[1], s[2], opt(s[3]), ctx->saved_data["t"].toDouble(),
+                                       ctx->saved_data["tail"].toBool(), s[4], g[0].contiguous(),
+                                       1.0);
+    return {once(grad), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+// Loss and gradient in one pass over the logits; the upstream scalar is applied
+// in backward (nothing is written where it is 1).
+struct DistillScalarFn : public Function<DistillScalarFn> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& ids,
+                            const at::Tensor& lp, const OptTensor& w, double t, bool tail,
+                            double scale) {
+    auto [rows, stats, grad, loss] = call_distill(x, ids, lp, w, t, tail, scale, true, true);
+    ctx->save_for_backward({x, ids, lp, w ? *w : at::Tensor(), stats});
+    ctx->saved_data["t"] = t;
+    ctx->saved_data["tail"] = tail;
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["grad"] = grad;
+    return loss;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const auto s = ctx->get_saved_variables();
+    at::AutoDispatchBelowADInplaceOrView guard;
+    auto held = ctx->saved_data.find("grad");
+    at::Tensor grad;
+    if (held != ctx->saved_data.end()) {
+      grad = held->second.toTensor();
+      ctx->saved_data.erase(held);
+      call_scale_by(grad, g[0]);
+    } else {  // the graph is run again: the first run gave its gradient away
+      grad = call_distill_bwd(s[0], s[1], s[2], opt(s[3]), ctx->saved_data["t"].toDouble(),
+                              ctx->saved_data["tail"].toBool(), s[4], g[0],
+                              ctx->saved_data["scale"].toDouble());
+    }
+    return {once(grad),   at::Tensor(), at::Tensor(), at::Tensor(),
+            at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>
+token_logprobs_train(const at::Tensor& x, const at::Tensor& ids, int64_t top_n, double t) {
+  auto r = TokenLogprobsFn::apply(x, ids, top_n, t);
+  return {r[0], r[1], r[2], r[3], r[4], r[5]};
+}
+at::Tensor distill_rows_train(const at::Tensor& x, const at::Tensor& ids, const at::Tensor& lp,
+                              const OptTensor& w, double t, bool tail) {
+  return DistillRowsFn::apply(x, ids, lp, w, t, tail);
+}
+at::Tensor distill_scalar_train(const at::Tensor& x, const at::Tensor& ids, const at::Tensor& lp,
+                                const OptTensor& w, double t, bool tail, double scale) {
+  return DistillScalarFn::apply(x, ids, lp, w, t, tail, scale);
+}
+
 }  // namespace
 }  // namespace b200
 
 TORCH_LIBRARY_FRAGMENT(_b200_C, m) {
+  m.def("token_logprobs_train(Tensor logits, Tensor token_ids, int top_n, float temperature) -> "
+        "(Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def("distill_rows_train(Tensor logits, Tensor teacher_ids, Tensor teacher_logprobs, "
+        "Tensor? weights, float temperature, bool tail) -> Tensor");
+  m.def("distill_scalar_train(Tensor logits, Tensor teacher_ids, Tensor teacher_logprobs, "
+        "Tensor? weights, float temperature, bool tail, float scale) -> Tensor");
+  m.def("backward_launches() -> int", &b200::backward_launches);
   m.def("token_logprobs(Tensor logits, Tensor token_ids, int top_n, float temperature) -> "
         "(Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
   m.def("token_logprobs_bwd(Tensor logits, Tensor token_ids, Tensor stats, Tensor? g_logprob, "
@@ -225,4 +381,10 @@ TORCH_LIBRARY_IMPL(_b200_C, CUDA, m) {
   m.impl("distill_loss", &b200::distill_loss);
   m.impl("distill_loss_bwd", &b200::distill_loss_bwd);
   m.impl("scale_by", &b200::scale_by);
+}
+
+TORCH_LIBRARY_IMPL(_b200_C, CompositeImplicitAutograd, m) {
+  m.impl("token_logprobs_train", &b200::token_logprobs_train);
+  m.impl("distill_rows_train", &b200::distill_rows_train);
+  m.impl("distill_scalar_train", &b200::distill_scalar_train);
 }

@@ -40,6 +40,10 @@ NO_FAKE = {
     "ep_finish": "expert-parallel exchange over peer pointers (eager only)",
     "tp_exchange": "peer-memory collective (raw pointer lists)",
     "tree_attention_workspace": "size query (host)",
+    "backward_launches": "host query",
+    "token_logprobs_train": "composite: traces into the ops that it calls",
+    "distill_rows_train": "composite: traces into the ops that it calls",
+    "distill_scalar_train": "composite: traces into the ops that it calls",
     "gemm_ag": "all-gather -> GEMM over peer memory (raw pointer lists)",
 }
 

@@ -125,31 +125,12 @@ def _check_temperature(temperature: float, what: str) -> float:
     return t
 
 
+def _count_backward() -> None:
+    """The native backward passes count their launches themselves."""
+    launch_count.also(torch.ops._b200_C.backward_launches)
+
+
 # ------------------------------------------------------------------ token log-probs
-class _TokenLogprobsFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, ids, top_n, temperature):
-        lp, rank, ent, lse, top_ids, top_lp, stats = torch.ops._b200_C.token_logprobs(
-            logits, ids, top_n, temperature)
-        ctx.save_for_backward(logits, ids, stats)
-        ctx.temperature = temperature
-        ctx.mark_non_differentiable(rank, lse, top_ids, top_lp)
-        ctx.set_materialize_grads(False)
-        return lp, rank, ent, lse, top_ids, top_lp
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g_lp, _rank, g_ent, *_):
-        logits, ids, stats = ctx.saved_tensors
-        if g_lp is None and g_ent is None:
-            return None, None, None, None
-        launch_count.add(1)
-        grad = torch.ops._b200_C.token_logprobs_bwd(
-            logits, ids, stats, None if g_lp is None else g_lp.contiguous(),
-            None if g_ent is None else g_ent.contiguous(), ctx.temperature)
-        return grad, None, None, None
-
-
 def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, top_n: int = 0,
                    temperature: float = 1.0) -> TokenLogprobs:
     """Log-probability, rank and alternatives of one given token a row.
@@ -181,59 +162,12 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, top_n: int = 0
     ids = token_ids.contiguous()
     launch_count.add(1)
     if logits.requires_grad and torch.is_grad_enabled():
-        return TokenLogprobs(*_TokenLogprobsFn.apply(logits, ids, top_n, t))
+        _count_backward()
+        return TokenLogprobs(*torch.ops._b200_C.token_logprobs_train(logits, ids, top_n, t))
     return TokenLogprobs(*torch.ops._b200_C.token_logprobs(logits, ids, top_n, t)[:6])
 
 
 # ------------------------------------------------------------------ distillation
-class _DistillRowsFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, ids, lp, weights, temperature, tail):
-        rows, stats, _, _ = torch.ops._b200_C.distill_loss(logits, ids, lp, weights, temperature,
-                                                           tail, 1.0, False, False)
-        ctx.save_for_backward(logits, ids, lp, weights, stats)
-        ctx.args = (temperature, tail)
-        return rows
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g):
-        logits, ids, lp, weights, stats = ctx.saved_tensors
-        t, tail = ctx.args
-        launch_count.add(1)
-        grad = torch.ops._b200_C.distill_loss_bwd(logits, ids, lp, weights, t, tail, stats,
-                                                  g.contiguous(), 1.0)
-        return grad, None, None, None, None, None
-
-
-class _DistillScalarFn(torch.autograd.Function):
-    """Loss and gradient in one pass over the logits; the upstream scalar is
-    applied in backward (nothing is written where it is 1)."""
-
-    @staticmethod
-    def forward(ctx, logits, ids, lp, weights, temperature, tail, scale):
-        _, stats, grad, loss = torch.ops._b200_C.distill_loss(logits, ids, lp, weights,
-                                                              temperature, tail, scale, True, True)
-        ctx.save_for_backward(logits, ids, lp, weights, stats)
-        ctx.args = (temperature, tail, scale)
-        ctx.grad = grad
-        return loss
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g):
-        grad, ctx.grad = ctx.grad, None
-        launch_count.add(1)
-        if grad is not None:
-            torch.ops._b200_C.scale_by(grad, g)
-        else:  # the graph is run again: the first run gave its gradient away
-            logits, ids, lp, weights, stats = ctx.saved_tensors
-            t, tail, scale = ctx.args
-            grad = torch.ops._b200_C.distill_loss_bwd(logits, ids, lp, weights, t, tail, stats,
-                                                      g, scale)
-        return grad, None, None, None, None, None, None
-
-
 def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logprobs: torch.Tensor,
                  weights: torch.Tensor | None = None, temperature: float = 1.0,
                  tail: bool = True, reduction: str = "mean") -> torch.Tensor:
@@ -294,11 +228,13 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logpro
     ids, lp = ids.contiguous(), teacher_logprobs.contiguous()
     w = None if weights is None else weights.contiguous()
     train = logits.requires_grad and torch.is_grad_enabled()
+    if train:
+        _count_backward()
     launch_count.add(1 if reduction == "none" else 2)
     if reduction == "none":
         if train:
-            return _DistillRowsFn.apply(logits, ids, lp, w, t, tail)
+            return torch.ops._b200_C.distill_rows_train(logits, ids, lp, w, t, tail)
         return torch.ops._b200_C.distill_loss(logits, ids, lp, w, t, tail, 1.0, False, False)[0]
     if train:
-        return _DistillScalarFn.apply(logits, ids, lp, w, t, tail, scale)
+        return torch.ops._b200_C.distill_scalar_train(logits, ids, lp, w, t, tail, scale)
     return torch.ops._b200_C.distill_loss(logits, ids, lp, w, t, tail, scale, True, False)[3]
