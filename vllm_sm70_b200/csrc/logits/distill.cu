@@ -1070,7 +1070,7 @@ void launch_t(const Params& p, int* counter, cudaStream_t stream) {
   cudaGetDevice(&dev);
   const int sms = num_sms(dev);
   if (p.grad && slice_bytes<T>(p.V, kMaxCluster) <= kSmemMost) {
-    int cl = row_split(p.rows, p.V / Traits<T>::E, sms, NT);
+    int cl = row_split(p.rows, p.V / Traits<T>::E, 5 * sms / 2, NT);
     while (cl < kMaxCluster && slice_bytes<T>(p.V, cl) > kSmemSlice) cl *= 2;
     switch (cl) {
       case 1: return launch_fused<T, 1>(p, counter, stream);
@@ -1080,7 +1080,7 @@ void launch_t(const Params& p, int* counter, cudaStream_t stream) {
     }
   }
   if (p.grad) return launch_stream<T, 8, true>(p, stream);
-  int cl = row_split(p.rows, p.V / Traits<T>::E, 2 * sms, NT);
+  int cl = row_split(p.rows, p.V / Traits<T>::E, 4 * sms, NT);
   // bitmaps of a very large vocabulary: 32 KB, for four CTAs an SM
   while (cl < kMaxCluster && slice_vectors<T>(p.V, cl) > 32 * 1024) cl *= 2;
   switch (cl) {

@@ -345,11 +345,13 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// CTAs that share a row, by the number of rows: enough CTAs to fill the
-// device's SMs twice over, while a CTA keeps at least `min_vec` vectors.
-inline int row_split(int64_t rows, int64_t n_vec, int num_sm, int min_vec) {
+// CTAs that share a row, by the number of rows: as many as run at the same
+// time (`resident`), while a CTA keeps at least `min_vec` vectors. (A second
+// wave costs more than larger parts: 128 rows of 128256 took 13 us at 8 CTAs a
+// row, in two waves.)
+inline int row_split(int64_t rows, int64_t n_vec, int resident, int min_vec) {
   int cl = 1;
-  while (cl < 8 && rows * cl < 2 * (int64_t)num_sm && n_vec / (2 * cl) >= min_vec) cl *= 2;
+  while (cl < 8 && rows * 2 * cl <= resident && n_vec / (2 * cl) >= min_vec) cl *= 2;
   return cl;
 }
 

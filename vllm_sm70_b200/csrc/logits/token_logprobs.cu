@@ -134,17 +134,21 @@ __device__ __forceinline__ void visit(const Smem& sm, const Row<T>& row, const S
   }
 }
 
-// Elements above tau into sm.cand (up to kCand; sm.n_gt counts all of them),
-// the ids of those equal to it into sm.eq (up to kEq; sm.n_eq counts them).
+// Elements above tau into sm.cand (up to kCand; sm.n_gt counts them, or is
+// larger than that), the ids of those equal to it into sm.eq (up to kEq;
+// sm.n_eq likewise).
 // The order in which they arrive does not matter: the lists are ranked.
 template <typename T>
 __device__ __forceinline__ void collect(Smem& sm, const Row<T>& row, const Slice& sl,
                                         uint32_t tau) {
   visit(sm, row, sl, [&](uint32_t k, int id) {
+    // (Counts above what the lists hold only say so.)
     if (k > tau) {
+      if (*(volatile int*)&sm.n_gt > kCand) return;
       const int at = atomicAdd(&sm.n_gt, 1);
       if (at < kCand) sm.cand[at] = entry(k, id);
     } else if (k == tau) {
+      if (*(volatile int*)&sm.n_eq > kEq) return;
       const int at = atomicAdd(&sm.n_eq, 1);
       if (at < kEq) sm.eq[at] = id;
     }
@@ -449,7 +453,12 @@ __global__ void __launch_bounds__(NT, 4) token_logprobs_kernel(const FwdParams p
   if constexpr (TOP) {
     uint32_t tau = find_tau(sm, n);
     if (key >= tau) {
-      const uint32_t tau_up = key_of(__uint_as_float(__float_as_uint(value_of(tau)) & 0xffff0000u));
+      uint32_t tau_up = key_of(__uint_as_float(__float_as_uint(value_of(tau)) & 0xffff0000u));
+      // Nothing but -inf reaches tau: groups of those are not read again, the
+      // first of them are found in id order.
+      const bool masked = tau == key_of(-INFINITY);
+      tau_up += masked ? 1u : 0u;
+      if (masked) sm.n_eq = kEq + 1;
 #pragma unroll 4
       for (int i = 0; i < n_slots; ++i)
         if (key_of(__uint_as_float((uint32_t)slots[i * NT + tid] << 16)) >= tau_up) {
@@ -644,7 +653,7 @@ template <typename T>
 void launch_fwd_t(const FwdParams& p, int64_t rows, cudaStream_t stream) {
   int dev = 0;
   cudaGetDevice(&dev);
-  int cl = row_split(rows, p.V / Traits<T>::E, 2 * num_sms(dev), NT);
+  int cl = row_split(rows, p.V / Traits<T>::E, 4 * num_sms(dev), NT);
   // (32 KB of maxima a CTA: four an SM)
   while (p.top_n > 0 && cl < kMaxCluster && groups_of<T>(p.V, cl) > kSlots) cl *= 2;
   switch (cl) {
