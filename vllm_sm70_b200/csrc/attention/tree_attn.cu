@@ -402,9 +402,13 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
       const int team = 31 - __clz(__reduce_and_sync(0xffffffffu, by));
       walk.team = team;
       walk.sub = (int)blockIdx.x % team;
-      total /= team;
+      // (64-bit divisions take microseconds off a short call.)
+      if (team > 1) total /= team;
       const int teams = (int)gridDim.x / team, me = (int)blockIdx.x / team;
-      const long long per = max((long long)kMinShare, (total + teams - 1) / teams);
+      const long long per =
+          max((long long)kMinShare, total < (1ll << 30)
+                                        ? (long long)(((uint32_t)total + teams - 1) / (uint32_t)teams)
+                                        : (total + teams - 1) / teams);
       const long long t0 = per * me, n = me < teams ? min(per, total - t0) : 0;
       share = (int)per;
       walk.left = (int)max(0ll, n);
@@ -430,7 +434,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
         if (hit) {
           const int l = __ffs(hit) - 1;
           walk.s = b + l;
-          walk.off = (int)(t0 - (seen + __shfl_sync(0xffffffffu, lane > 0 ? before : 0, l)) / team);
+          const long long base = seen + __shfl_sync(0xffffffffu, lane > 0 ? before : 0, l);
+          walk.off = (int)(t0 - (team > 1 ? base / team : base));
           walk.set(share_seq(mine, l));
           found = true;
         }
@@ -1065,9 +1070,11 @@ void launch_d(const TreeAttnArgs& a, cudaStream_t stream) {
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.err = device_status_ptr(dev);
   launch_pdl(kernel, dim3(grid), dim3(kThreads), C::kSmem, stream, nullptr, tk, tv, p);
+  const long long most = p.T * p.G < FM ? p.T * p.G : FM;
   if (grid > 1)
-    launch_pdl(tree_join_kernel<D>, dim3(grid - 1, FM / kJoinRows), dim3(kJoinRows * 32), 0, stream,
-               nullptr, p);
+    // (A row tile has no more rows than the call.)
+    launch_pdl(tree_join_kernel<D>, dim3(grid - 1, (int)((most + kJoinRows - 1) / kJoinRows)),
+               dim3(kJoinRows * 32), 0, stream, nullptr, p);
 }
 
 }  // namespace
