@@ -127,6 +127,16 @@ def test_ragged_batch_and_long_context(b200_ops):
     _check(*_setup([30001], [64], (16, 2, 256), 16))
 
 
+@pytest.mark.parametrize("heads", [(8, 2, 64), (8, 2, 128), (16, 2, 256)])
+def test_many_short_sequences(b200_ops, heads):
+    """Units of a few tiles, whose edges fall anywhere in a share."""
+    g = torch.Generator().manual_seed(5)
+    lens = torch.randint(1, 400, (450,), generator=g).tolist()
+    nodes = [min(n, int(k)) for n, k in zip(lens, torch.randint(1, 7, (450,), generator=g))]
+    _check(*_setup(lens, nodes, heads, 16))
+    _check(*_setup([130] * 160, [4] * 160, heads, 16))
+
+
 def test_sequences_without_nodes_or_keys(b200_ops):
     q, kc, vc, bt, sl, cu, m = _setup([50, 60, 70, 300], [3, 0, 0, 2], (32, 8, 128), 16)
     _check(q, kc, vc, bt, sl, cu, m)

@@ -16,8 +16,9 @@
 //
 // Work split. One persistent CTA an SM. The key tiles of all (sequence, key
 // head, row tile) units form one list, and CTA c takes the c-th equal share
-// of it, whatever the contexts' lengths: ragged batches stay balanced and one
-// long context spreads over the whole device. A unit cut at a share's edge
+// of it (a unit's edge counts as some tiles), whatever the contexts' lengths:
+// ragged batches stay balanced and one long context spreads over the whole
+// device. A unit cut at a share's edge
 // leaves (max, sum, unnormalised o) pieces in the workspace, which a second
 // kernel joins in share order; whole units are written directly. The split
 // depends on the lengths only, so results repeat bit for bit.
@@ -104,6 +105,11 @@ struct Cfg {
   static constexpr int kTile = kDC * kChunk;      // K or V of a tile
   static constexpr int NK = D == 64 ? 6 : 2;      // K ring slots
   static constexpr int NV = D == 64 ? 6 : 3;      // V: held until P is there, two tiles on
+  // What a unit's edge costs, in tiles: a masked tile, the output, at D = 256
+  // also the wait for Q's one buffer. Shares of several short units get fewer
+  // tiles: 16 trees of 24 nodes, 16/2 heads of 256, window 4096: 72 -> 64 us;
+  // 64 of 8 nodes, 16/16 heads of 64: 217 -> 194; long units do not notice.
+  static constexpr int kEdge = D <= 128 ? 2 : 10;
   static constexpr int kSmem = NQ * kQBytes + (NK + NV) * kTile + kBarBytes + kRowBytes;
   static_assert(3 * FN + D <= 512, "TMEM columns");
   static_assert(kSmem <= 232448, "shared memory");
@@ -157,9 +163,9 @@ __device__ __forceinline__ uint32_t ld_word(const uint32_t* p) {
 // One sequence's part of the work.
 struct Seq {
   int q0, q_len, seq_len, nodes, prefix, k_first, k_lo, n_tiles, n_rt;
-  int total;  // tiles of all its units (the host bounds it)
+  int total;  // tiles of all its units with their edges (the host bounds it)
 };
-template <int FN>
+template <int FN, int kEdge>
 __device__ __forceinline__ Seq load_seq(const Params& p, int s) {
   Seq r;
   r.q0 = p.cu_q[s];
@@ -172,7 +178,7 @@ __device__ __forceinline__ Seq load_seq(const Params& p, int s) {
   r.k_lo = r.k_first / FN * FN;
   r.n_tiles = max(1, (r.seq_len - r.k_lo + FN - 1) / FN);
   r.n_rt = (r.q_len * p.G + FM - 1) / FM;
-  r.total = r.n_tiles * r.n_rt * p.Hkv;
+  r.total = (r.n_tiles + kEdge) * r.n_rt * p.Hkv;
   return r;
 }
 
@@ -195,7 +201,7 @@ __device__ __forceinline__ Seq share_seq(const Seq& q, int l) {
 // The units of a CTA's share, in order: unit = key head * n_rt + row tile,
 // key tiles [j0, j1) of it. Of `team` row tiles that are taken together, this
 // is the sub-th.
-template <int FN>
+template <int FN, int kEdge>
 struct Walk {
   int s, unit, j0, j1, kvh, row0;
   int off, left;
@@ -207,21 +213,25 @@ struct Walk {
     q.total /= team;
   }
   __device__ __forceinline__ bool next(const Params& p) {
-    if (left <= 0) return false;
-    while (off >= q.total) {
-      if (++s >= p.num_seqs) return false;
-      set(load_seq<FN>(p, s));
-      off = 0;
+    while (left > 0) {
+      while (off >= q.total) {
+        if (++s >= p.num_seqs) return false;
+        set(load_seq<FN, kEdge>(p, s));
+        off = 0;
+      }
+      const int len = q.n_tiles + kEdge;
+      unit = off / len;
+      j0 = off - unit * len;
+      const int n = min(len - j0, left);
+      j1 = min(j0 + n, q.n_tiles);
+      off += n;
+      left -= n;
+      if (j0 >= q.n_tiles) continue;  // the share began at a unit's edge
+      kvh = unit / q.n_rt;
+      row0 = ((unit - kvh * q.n_rt) * team + sub) * FM;
+      return true;
     }
-    unit = off / q.n_tiles;
-    kvh = unit / q.n_rt;
-    row0 = ((unit - kvh * q.n_rt) * team + sub) * FM;
-    j0 = off - unit * q.n_tiles;
-    const int n = min(q.n_tiles - j0, left);
-    j1 = j0 + n;
-    off += n;
-    left -= n;
-    return true;
+    return false;
   }
 };
 
@@ -375,7 +385,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
     const int bi = lane % nb, h = lane / nb;
     // The share (warp 0): a scan over the sequences, 32 at a time, for the
     // total and then for the sequence in which this CTA's first tile lies.
-    Walk<FN> walk;
+    Walk<FN, C::kEdge> walk;
     int share = 0;
     if (!is_v) {
       long long total = 0, sums = 0;
@@ -384,7 +394,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
       for (int b = 0; b < p.num_seqs; b += 32) {
         long long c = 0;
         if (b + lane < p.num_seqs) {
-          const Seq q = load_seq<FN>(p, b + lane);
+          const Seq q = load_seq<FN, C::kEdge>(p, b + lane);
           c = q.total;
 #pragma unroll
           for (int d = 2; d <= kMaxTeam; ++d)
@@ -420,7 +430,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
         if (b > 0) {
           c = 0;
           if (b + lane < p.num_seqs) {
-            mine = load_seq<FN>(p, b + lane);
+            mine = load_seq<FN, C::kEdge>(p, b + lane);
             c = mine.total;
           }
 #pragma unroll
@@ -1089,7 +1099,7 @@ void tree_attention_launch(const TreeAttnArgs& a, cudaStream_t stream) {
   if (a.block_size < 8 || (a.block_size & (a.block_size - 1)) != 0)
     throw std::runtime_error("tree_attention: block_size must be a power of two >= 8");
   // Tiles of one sequence are counted in 32 bits.
-  const double tiles = ((double)a.max_blocks * a.block_size / 64 + 1) * a.Hkv *
+  const double tiles = ((double)a.max_blocks * a.block_size / 64 + 12) * a.Hkv *
                        ((double)a.num_tokens * (a.Hq / a.Hkv) / FM + 1);
   if (tiles > 2e9) throw std::runtime_error("tree_attention: block table too wide for the batch");
   if (a.num_tokens <= 0 || a.num_seqs <= 0) return;
