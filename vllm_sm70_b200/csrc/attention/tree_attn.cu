@@ -54,7 +54,7 @@
 // TMEM columns: S0 | S1 | S2 | O.
 //
 // Measured (32 query, 8 key heads of 128, blocks of 16): 64 trees of 16 nodes
-// over 4096 tokens 137 us, 5080 GB/s of the 6454 that a copy reaches; the
+// over 4096 tokens 135 us, 5160 GB/s of the 6454 that a copy reaches; the
 // steady state is HBM's, the rest is the start (~10 us to the first scores),
 // a few us at each unit's edge, and the join. 2 trees of 64 nodes over 60001
 // tokens 129 us (159 when each row tile read its keys from HBM): 730 TFLOP/s,
