@@ -249,6 +249,52 @@ def test_distill(b200_ops, T, V, K, tail, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,V", [(3, 1000003), (2, 2 ** 22 - 3)])
+def test_distill_rows_that_no_cluster_holds(b200_ops, T, V, dtype):
+    x = _rows(T, V, dtype, 5, pad=3, offset=1)
+    ids, lp = _teacher(T, V, 20, 7)
+    ids[0, 5] = ids[0, 3]
+    _check_distill(x, ids, lp, torch.tensor([1.5, 0.5, 0.0], device="cuda")[:T], 1.0, True, dtype)
+    _check_distill(x, ids, lp, None, 2.0, False, dtype)
+    xg = x.detach().requires_grad_(True)
+    g, = torch.autograd.grad(ops.distill_loss(xg, ids, lp), xg)
+    assert bool((g != 0).all())  # every element has its own, however small
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,V", [(500, 30011), (40, 128257), (7, 5003), (330, 70001)])
+def test_every_element_has_its_gradient(b200_ops, T, V, dtype):
+    """None is left out or written over, however small it is."""
+    x = _rows(T, V, dtype, 5, pad=3, offset=1).requires_grad_(True)
+    ids, lp = _teacher(T, V, 20, 7)
+    y = ids[:, 0].contiguous()
+    for loss in (ops.distill_loss(x, ids, lp), ops.distill_loss(x, ids, lp, reduction="none").sum(),
+                 ops.token_logprobs(x, y).logprobs.sum()):
+        g, = torch.autograd.grad(loss, x)
+        assert bool((g != 0).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_distill_graph(b200_ops, dtype):
+    """More rows than clusters (the rows come from a counter), replayed."""
+    x = _rows(500, 30011, dtype, 3).requires_grad_(True)
+    ids, lp = _teacher(500, 30011, 9, 2)
+    g, = torch.autograd.grad(ops.distill_loss(x, ids, lp), x)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(ops.distill_loss(x, ids, lp), x)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got, = torch.autograd.grad(ops.distill_loss(x, ids, lp), x)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got.zero_()
+        graph.replay()
+        assert torch.equal(got, g)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("pad,offset", [(1, 0), (3, 1), (0, 5)])
 def test_distill_strided(b200_ops, dtype, pad, offset):
     x = _rows(7, 5003, dtype, 4, pad, offset)

@@ -842,10 +842,12 @@ __global__ void __launch_bounds__(NT, 4) distill_stream_kernel(const Params p) {
   const float up = w * p.gscale;
   if (!slow_range(st.x)) {
     const float rm = __fmul_rn(st.x, c), coef = st.z * up * ex2(-fmaf(st.x, c, -rm));
-    for_groups<NT, U>(row, sl, [&](const uint4(&v)[U], int u, int) {
+    const int groups = (sl.b - sl.a + U * NT - 1) / (U * NT);
+    for_groups<NT, U>(row, sl, [&](const uint4(&v)[U], int u, int it) {
+      if (it == groups) return;  // the partial vectors, below
 #pragma unroll
       for (int k = 0; k < U; ++k)
-        if (u + k * NT >= sl.a && u + k * NT < sl.b)
+        if (u + k * NT < sl.b)
           store_vec(out, row, u + k * NT, grad_vec<T, false>(v[k], c, rm, coef));
     });
     const int e = tid == 0 ? sl.head : tid == 1 ? sl.tail : -1;
