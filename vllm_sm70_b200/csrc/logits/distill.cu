@@ -58,6 +58,8 @@ using namespace rows;
 constexpr int NT = 256;
 constexpr int kWarps = NT / 32;
 constexpr int U = 4;
+constexpr int kBwdThreads = 128;
+static_assert(kMaxTeacherK <= kBwdThreads, "a thread a teacher entry");
 constexpr int kMaxCluster = 8;
 
 struct Params {
@@ -868,7 +870,7 @@ __global__ void __launch_bounds__(NT, 4) distill_stream_kernel(const Params p) {
 }
 
 // The same gradient for an upstream value a row: elementwise on the saved
-// numbers. One CTA a (row, chunk of NT * U vectors).
+// numbers. One CTA a (row, chunk of kBwdThreads * U vectors).
 struct BwdParams {
   Params f;
   const float* g;
@@ -876,10 +878,10 @@ struct BwdParams {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(NT) distill_bwd_kernel(const BwdParams b) {
+__global__ void __launch_bounds__(kBwdThreads) distill_bwd_kernel(const BwdParams b) {
   using Tr = Traits<T>;
   constexpr int E = Tr::E;
-  constexpr int kBits = NT * U * E;  // elements of the chunk
+  constexpr int kBits = kBwdThreads * U * E;  // elements of the chunk
   __shared__ uint32_t seen[kBits / 32];
   __shared__ int dup;
   pdl_wait();
@@ -888,19 +890,19 @@ __global__ void __launch_bounds__(NT) distill_bwd_kernel(const BwdParams b) {
   const int64_t r = blockIdx.y;
   const int tid = threadIdx.x;
   const Row<T> row(p.x, r, p.ld, p.V);
-  const int u_lo = blockIdx.x * (NT * U), u_hi = min(u_lo + NT * U, row.n_vec);
+  const int u_lo = blockIdx.x * (kBwdThreads * U), u_hi = min(u_lo + kBwdThreads * U, row.n_vec);
   if (u_lo >= u_hi) return;
   T* out = reinterpret_cast<T*>(p.grad) + r * p.V;
   const float w = p.weights ? p.weights[r] : 1.f;
   const float up = w == 0.f ? 0.f : w * p.gscale * b.g[r * b.g_stride];
   if (up == 0.f) {
-    for (int u = u_lo + tid; u < u_hi; u += NT) store_vec(out, row, u, make_uint4(0u, 0u, 0u, 0u));
+    for (int u = u_lo + tid; u < u_hi; u += kBwdThreads) store_vec(out, row, u, make_uint4(0u, 0u, 0u, 0u));
     return;
   }
   uint4 v[U];
 #pragma unroll
   for (int k = 0; k < U; ++k) {
-    const int u = u_lo + tid + k * NT;
+    const int u = u_lo + tid + k * kBwdThreads;
     v[k] = u < u_hi ? row.load(u) : make_uint4(0u, 0u, 0u, 0u);
   }
   // Thread k's teacher entry, if it is of this chunk, and whether an id of
@@ -911,7 +913,7 @@ __global__ void __launch_bounds__(NT) distill_bwd_kernel(const BwdParams b) {
   const float4 st = p.stats[r];
   const float xk = mine ? Tr::to_f(row.x[id]) : 0.f;
   float mass = mine ? expf(p.t_lp[r * p.K + tid] - st.w) : 0.f;
-  for (int i = tid; i < kBits / 32; i += NT) seen[i] = 0u;
+  for (int i = tid; i < kBits / 32; i += kBwdThreads) seen[i] = 0u;
   if (tid == 0) dup = 0;
   __syncthreads();
   if (mine && (atomicOr(&seen[at / 32], 1u << (at % 32)) >> (at % 32)) & 1u) dup = 1;
@@ -919,11 +921,11 @@ __global__ void __launch_bounds__(NT) distill_bwd_kernel(const BwdParams b) {
     const float rm = __fmul_rn(st.x, p.c), coef = st.z * up * ex2(-fmaf(st.x, p.c, -rm));
 #pragma unroll
     for (int k = 0; k < U; ++k) {
-      const int u = u_lo + tid + k * NT;
+      const int u = u_lo + tid + k * kBwdThreads;
       if (u < u_hi) store_vec(out, row, u, grad_vec<T, false>(v[k], p.c, rm, coef));
     }
   } else {
-    for (int u = u_lo + tid; u < u_hi; u += NT)
+    for (int u = u_lo + tid; u < u_hi; u += kBwdThreads)
       store_vec(out, row, u, grad_vec<T, true>(row.load(u), p.c, st.x, st.z * up));
   }
   __syncthreads();
@@ -1116,7 +1118,7 @@ void distill_bwd_launch(const DistillBwdArgs& a, cudaStream_t stream) {
   check(a.in, a.K, "distill_loss_bwd");
   const int E = a.in.bf16 ? 8 : 4;
   const int64_t eb = a.in.bf16 ? 2 : 4;
-  const unsigned chunks = (unsigned)((a.in.V + 2 * E - 2) / E + NT * U - 1) / (NT * U);
+  const unsigned chunks = (unsigned)((a.in.V + 2 * E - 2) / E + kBwdThreads * U - 1) / (kBwdThreads * U);
   for (int64_t r0 = 0; r0 < a.in.rows; r0 += 65535) {  // grid.y limit
     const unsigned n = (unsigned)(a.in.rows - r0 < 65535 ? a.in.rows - r0 : 65535);
     BwdParams b{};
@@ -1129,10 +1131,10 @@ void distill_bwd_launch(const DistillBwdArgs& a, cudaStream_t stream) {
     b.g = a.g_rows + r0 * a.g_stride;
     b.g_stride = a.g_stride;
     if (a.in.bf16)
-      launch_pdl(distill_bwd_kernel<__nv_bfloat16>, dim3(chunks, n), dim3(NT), 0, stream, nullptr,
+      launch_pdl(distill_bwd_kernel<__nv_bfloat16>, dim3(chunks, n), dim3(kBwdThreads), 0, stream, nullptr,
                  b);
     else
-      launch_pdl(distill_bwd_kernel<float>, dim3(chunks, n), dim3(NT), 0, stream, nullptr, b);
+      launch_pdl(distill_bwd_kernel<float>, dim3(chunks, n), dim3(kBwdThreads), 0, stream, nullptr, b);
   }
 }
 
