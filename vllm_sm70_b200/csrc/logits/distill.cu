@@ -72,6 +72,7 @@ struct Params {
   int64_t rows;
   bool tail;
   float c, inv_t, gscale;  // log2(e) / T; 1 / T; upstream gradient / T of a row of weight 1
+  float least;             // floor_of(c)
   float* row_loss;
   float4* stats;
   void* grad;
@@ -228,9 +229,6 @@ __device__ __forceinline__ uint4 grad_vec(const uint4& v, float c, float m_or_r,
   }
   return Tr::pack(g);
 }
-
-// Whether m c can be taken apart from x c.
-__device__ __forceinline__ bool slow_range(float m) { return !(m >= kSlowBelow && m <= kSlowAbove); }
 
 // The elements of vector u that the row has, one by one.
 template <typename T>
@@ -466,7 +464,7 @@ __global__ void __launch_bounds__(NT, 3) distill_fused_kernel(const Params p) {
     for (int u = tail + lane; u < end; u += 32) vm = Tr::vmax(vm, Tr::vmax(mine[u]));
     const float m_w = warp_max(fmaxf(Tr::value(vm), m_k));
     float s = 0.f;
-    if (!slow_range(m_w)) {
+    if (!slow_range(m_w, c, kFar)) {
       const float rw = __fmul_rn(m_w, c);
       const uint64_t c2 = f32x2_pack(c, c), nr2 = f32x2_pack(-rw, -rw);
       uint64_t s2[4];
@@ -618,7 +616,7 @@ __global__ void __launch_bounds__(NT, 3) distill_fused_kernel(const Params p) {
     // The gradient: every element as an outside one (the teacher's are -inf by
     // now), then the teacher's over it. The next row's vectors follow.
     const float up = w * p.gscale;
-    const bool slow = slow_range(st.x);
+    const bool slow = slow_range(st.x, c, kFar);
     const float rm = __fmul_rn(st.x, c), coef = st.z * up * (slow ? 1.f : ex2(-fmaf(st.x, c, -rm)));
     // Whole steps of 128 full vectors without checks.
     uint4* dst = reinterpret_cast<uint4*>(out - row.pad);
@@ -749,7 +747,7 @@ __global__ void __launch_bounds__(NT, 4) distill_stream_kernel(const Params p) {
     static_assert(U == 4, "tree of maxima");
     const float mx = Tr::value(Tr::vmax(Tr::vmax(vm[0], vm[1]), Tr::vmax(vm[2], vm[3])));
     if (mx > m) {
-      const float rn = __fmul_rn(fmaxf(mx, kFloor), c);
+      const float rn = __fmul_rn(fmaxf(mx, p.least), c);
       s *= m == -INFINITY ? (s != s ? s : 0.f) : ex2(r0 - rn);
       m = mx;
       r0 = rn;
@@ -772,11 +770,11 @@ __global__ void __launch_bounds__(NT, 4) distill_stream_kernel(const Params p) {
   });
   // A warp's sums against its own maximum, in a fixed order.
   const float m_w = warp_max(m);
-  if (slow_range(m_w) && m_w != -INFINITY) {
+  if (slow_range(m_w, c, kFar) && m_w != -INFINITY) {
     s = slow_sum(row, sl, bitmap, m_w, c);
   } else {
     const float e = fmaf(m, c, -r0);  // what r0 lacks of m c
-    if (m >= kSlowBelow)
+    if (m > p.least)
       s *= ex2(-e) * (m == m_w ? 1.f : ex2((m - m_w) * c));
     else
       s = s != s ? s : 0.f;  // nothing against the warp's maximum
@@ -842,7 +840,7 @@ __global__ void __launch_bounds__(NT, 4) distill_stream_kernel(const Params p) {
   // this slice over it (same CTA, after the barrier).
   const float4 st = numbers;
   const float up = w * p.gscale;
-  if (!slow_range(st.x)) {
+  if (!slow_range(st.x, c, kFar)) {
     const float rm = __fmul_rn(st.x, c), coef = st.z * up * ex2(-fmaf(st.x, c, -rm));
     const int groups = (sl.b - sl.a + U * NT - 1) / (U * NT);
     for_groups<NT, U>(row, sl, [&](const uint4(&v)[U], int u, int it) {
@@ -917,7 +915,7 @@ __global__ void __launch_bounds__(kBwdThreads) distill_bwd_kernel(const BwdParam
   if (tid == 0) dup = 0;
   __syncthreads();
   if (mine && (atomicOr(&seen[at / 32], 1u << (at % 32)) >> (at % 32)) & 1u) dup = 1;
-  if (!slow_range(st.x)) {
+  if (!slow_range(st.x, p.c, kFar)) {
     const float rm = __fmul_rn(st.x, p.c), coef = st.z * up * ex2(-fmaf(st.x, p.c, -rm));
 #pragma unroll
     for (int k = 0; k < U; ++k) {
@@ -1102,7 +1100,8 @@ void distill_launch(const DistillArgs& a, cudaStream_t stream) {
   if (a.in.rows > 0) {
     Params p{a.in.x, a.t_ids, a.t_lp, a.weights, a.in.ld, a.in.V, a.K, a.in.rows, a.tail,
              (float)(1.4426950408889634 / a.temperature), (float)(1.0 / a.temperature),
-             (float)((double)a.grad_scale / a.temperature), a.row_loss,
+             (float)((double)a.grad_scale / a.temperature),
+             floor_of((float)(1.4426950408889634 / a.temperature)), a.row_loss,
              reinterpret_cast<float4*>(a.stats), a.grad, nullptr, nullptr};
     if (a.in.bf16)
       launch_t<__nv_bfloat16>(p, a.counter, stream);
@@ -1125,7 +1124,7 @@ void distill_bwd_launch(const DistillBwdArgs& a, cudaStream_t stream) {
     b.f = Params{reinterpret_cast<const char*>(a.in.x) + r0 * a.in.ld * eb, a.t_ids + r0 * a.K,
                  a.t_lp + r0 * a.K, a.weights ? a.weights + r0 : nullptr, a.in.ld, a.in.V, a.K, n,
                  a.tail, (float)(1.4426950408889634 / a.temperature), (float)(1.0 / a.temperature),
-                 (float)((double)a.g_scale / a.temperature), nullptr,
+                 (float)((double)a.g_scale / a.temperature), 0.f, nullptr,
                  reinterpret_cast<float4*>(const_cast<float*>(a.stats)) + r0,
                  reinterpret_cast<char*>(a.grad) + r0 * a.in.V * eb, nullptr, nullptr};
     b.g = a.g_rows + r0 * a.g_stride;

@@ -18,6 +18,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <cstring>
 
 #include "common/launch.h"
 #include "common/ptx.cuh"
@@ -33,11 +34,31 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// Where a sum needs x (x - m) finite, elements below this count as this: their
-// exponentials are zero all the same unless the whole row lies down there
-// (rows whose maximum does are summed element by element, slow_sums).
-constexpr float kFloor = -1e30f;
-constexpr float kSlowBelow = -1e29f, kSlowAbove = 1e30f;
+// How far out a maximum m may lie for m c to be taken out of x c. r is off by up
+// to 2^-24 |m c|, and against r every exponential of the row is off by as many
+// powers of 2, which have to fit fp32: 64 of them at kFar. A sum of e_j d_j
+// (the entropy's) loses 2^-24 of r's error times its number of steps besides:
+// half a power of 2 at kFarEntropy. Parts of rows whose maximum lies further
+// out are summed element by element (slow_sum, slow_sums).
+constexpr float kFar = 1610612736.f;  // 1.5 * 2^30
+constexpr float kFarEntropy = 16777216.f;  // 2^24
+__device__ __forceinline__ bool slow_range(float m, float c, float far) {
+  return !(fabsf(m * c) <= far);
+}
+
+// In sums that go on before the maximum is known, elements below this count as
+// this: -2^31 / c, cut to a bf16 value. Against a maximum within kFar their
+// exponentials are zero all the same, and what a thread sums while it has seen
+// nothing else stays finite.
+inline float floor_of(float c) {
+  const float f = -2147483648.f / c;
+  uint32_t b;
+  memcpy(&b, &f, 4);
+  b &= 0xffff0000u;
+  float r;
+  memcpy(&r, &b, 4);
+  return r;
+}
 
 __device__ __forceinline__ float max_nan(float a, float b) {
   float d;
@@ -104,11 +125,12 @@ struct Traits<__nv_bfloat16> {
   __device__ static __forceinline__ bool all_below(Max m, float y) {
     return __hblt2(m, __float2bfloat162_rn(y));
   }
-  // Elements 2i and 2i + 1, not below kFloor.
-  __device__ static __forceinline__ void pair_floor(const uint4& v, int i, float& a, float& b) {
+  // Elements 2i and 2i + 1, not below `least` (a bf16 value).
+  __device__ static __forceinline__ void pair_floor(const uint4& v, int i, float least, float& a,
+                                                    float& b) {
     const uint32_t w = i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
     const __nv_bfloat162 f = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&w),
-                                         __float2bfloat162_rn(kFloor));
+                                         __float2bfloat162_rn(least));
     const uint32_t u = *reinterpret_cast<const uint32_t*>(&f);
     a = bf16_bits_lo(u);
     b = bf16_bits_hi(u);
@@ -165,10 +187,11 @@ struct Traits<float> {
   __device__ static __forceinline__ float value(Max m) { return m; }
   __device__ static __forceinline__ float max_of(const uint4& v) { return vmax(v); }
   __device__ static __forceinline__ bool all_below(Max m, float y) { return m < y; }
-  __device__ static __forceinline__ void pair_floor(const uint4& v, int i, float& a, float& b) {
+  __device__ static __forceinline__ void pair_floor(const uint4& v, int i, float least, float& a,
+                                                    float& b) {
     pair(v, i, a, b);
-    a = max_nan(a, kFloor);
-    b = max_nan(b, kFloor);
+    a = max_nan(a, least);
+    b = max_nan(b, least);
   }
   template <bool GE>
   __device__ static __forceinline__ void count(const uint4& v, float y, uint32_t& acc) {

@@ -66,6 +66,7 @@ struct FwdParams {
   int V, top_n;
   bool ids64;
   float c, inv_t;  // log2(e) / T, 1 / T
+  float least;     // floor_of(c)
   float* logprob;
   int* rank;
   float* entropy;
@@ -229,8 +230,8 @@ __device__ __noinline__ void collect_equal(Smem& sm, Row<T> row, Slice sl, uint3
   __syncthreads();
 }
 
-// This thread's sums of a row whose maximum lies so far out that x c or the
-// floor would not do: element by element against its own maximum.
+// This thread's sums where its warp's maximum lies far out: element by element
+// against its own maximum.
 template <typename T>
 __device__ __noinline__ Acc slow_sums(Row<T> row, int lo, int hi, float c) {
   Acc a{-INFINITY, 0.f, 0.f};
@@ -312,7 +313,7 @@ __global__ void __launch_bounds__(NT, 4) token_logprobs_kernel(const FwdParams p
       n_slots = it + 1;
     }
     if (mx > m) {
-      const float rn = __fmul_rn(fmaxf(mx, kFloor), c), d = r0 - rn;
+      const float rn = __fmul_rn(fmaxf(mx, p.least), c), d = r0 - rn;
       const float f = m == -INFINITY ? 0.f : ex2(d);
       t = f == 0.f ? 0.f : f * (t + d * s);
       s = f == 0.f ? 0.f * s : f * s;
@@ -326,7 +327,7 @@ __global__ void __launch_bounds__(NT, 4) token_logprobs_kernel(const FwdParams p
 #pragma unroll
       for (int i = 0; i < E / 2; ++i) {
         float xa, xb, da, db;
-        Tr::pair_floor(v[k], i, xa, xb);
+        Tr::pair_floor(v[k], i, p.least, xa, xb);
         const uint64_t d2 = f32x2_fma(f32x2_pack(xa, xb), c2, nr2);
         f32x2_unpack(d2, da, db);
         const uint64_t e2 = f32x2_pack(ex2(da), ex2(db));
@@ -377,9 +378,9 @@ __global__ void __launch_bounds__(NT, 4) token_logprobs_kernel(const FwdParams p
   const uint32_t key_w = __reduce_max_sync(0xffffffffu, key);
   const float m_w = value_of(key_w);
   Acc a{m, s, t};
-  if (m_w >= kSlowBelow && m_w <= kSlowAbove) {
+  if (!slow_range(m_w, c, kFarEntropy)) {
     const float e = fmaf(m, c, -r0);  // what r lacks of m c
-    if (m >= kSlowBelow) {
+    if (m > p.least) {
       a.t = (t - e * s) * ex2(-e);
       a.s = s * ex2(-e);
     } else {
@@ -680,6 +681,7 @@ void token_logprobs_launch(const TokenLogprobsArgs& a, cudaStream_t stream) {
   if (a.in.rows <= 0) return;
   FwdParams p{a.in.x,  a.ids,       a.in.ld,    a.in.V,
               a.top_n, a.ids64,     (float)(1.4426950408889634 / a.temperature), (float)(1.0 / a.temperature),
+              floor_of((float)(1.4426950408889634 / a.temperature)),
               a.logprob, a.rank,    a.entropy,  a.lse,
               a.top_ids, a.top_lp,  reinterpret_cast<float4*>(a.stats)};
   if (a.in.bf16)
