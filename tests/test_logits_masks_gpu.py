@@ -96,3 +96,34 @@ def test_distillation_of_masked_rows(b200_ops, value, t, dtype):
         lp = torch.log_softmax(torch.randn(rows, 8, device="cuda", generator=g), 1) - 0.2
         for tail in (True, False):
             _check_distill(x, ids, lp, t, tail)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,V", [(400, 20011), (3, 200003)])
+def test_one_token_left_at_the_lowest_value(b200_ops, rows, V, dtype):
+    """All but two elements at the type's lowest value, in rows at every
+    alignment: warps that hold nothing else sum their own vectors again, the
+    same ones."""
+    E = 128 // torch.finfo(dtype).bits
+    x = torch.full((rows, V), torch.finfo(dtype).min, device="cuda", dtype=dtype)
+    r = torch.arange(rows, device="cuda")
+    # the last lane of a warp, where a row begins inside a 16-byte vector
+    p = 32 * E * (1 + r % 70)
+    x[r, p] = 1.5
+    x[:, 5] = 0.5
+    _check_scores(x, p, 2)
+    ids = torch.full((rows, 1), 5, device="cuda")
+    lp = torch.full((rows, 1), -0.25, device="cuda")
+    _check_distill(x, ids, lp)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_lowest_value_in_rows_that_no_cluster_holds(b200_ops, dtype):
+    E = 128 // torch.finfo(dtype).bits
+    V = 2 ** 22 - 3
+    x = torch.full((2, V), torch.finfo(dtype).min, device="cuda", dtype=dtype)
+    x[:, 5] = 0.5
+    x[0, 32 * E * 3] = 1.5
+    x[1, 32 * E * 9] = 1.5
+    ids = torch.full((2, 1), 5, device="cuda")
+    _check_distill(x, ids, torch.full((2, 1), -0.25, device="cuda"))

@@ -254,7 +254,7 @@ template <typename T>
 __device__ __noinline__ float slow_sum(Row<T> row, Slice sl, const uint8_t* bitmap, float m,
                                        float c) {
   float s = 0.f;
-  for (int u = sl.lo + threadIdx.x; u < sl.hi; u += NT) {
+  for_vectors<NT>(sl, [&](int u) {
     uint4 v = row.load(u);
     Traits<T>::blank(v, bitmap[u - sl.lo]);
     for (int i = 0; i < Traits<T>::E / 2; ++i) {
@@ -262,7 +262,7 @@ __device__ __noinline__ float slow_sum(Row<T> row, Slice sl, const uint8_t* bitm
       Traits<T>::pair(v, i, a, b);
       s += ex2((a - m) * c) + ex2((b - m) * c);
     }
-  }
+  });
   return s;
 }
 

@@ -327,6 +327,17 @@ __device__ __forceinline__ void for_groups(const Row<T>& row, const Slice& s, F&
   }
 }
 
+// Calls f(u) for the vectors that for_groups gives this thread: a warp that
+// goes over its part again meets what it summed, and nothing of another's.
+template <int NT, typename F>
+__device__ __forceinline__ void for_vectors(const Slice& s, F&& f) {
+  const int tid = threadIdx.x;
+#pragma unroll 1
+  for (int u = s.a + tid; u < s.b; u += NT) f(u);
+  const int e = tid == 0 ? s.head : tid == 1 ? s.tail : -1;
+  if (e >= 0) f(e);
+}
+
 __device__ __forceinline__ int64_t load_id(const void* ids, bool ids64, int64_t row) {
   return ids64 ? reinterpret_cast<const int64_t*>(ids)[row]
                : (int64_t) reinterpret_cast<const int*>(ids)[row];

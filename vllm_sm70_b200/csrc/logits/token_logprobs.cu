@@ -233,9 +233,9 @@ __device__ __noinline__ void collect_equal(Smem& sm, Row<T> row, Slice sl, uint3
 // This thread's sums where its warp's maximum lies far out: element by element
 // against its own maximum.
 template <typename T>
-__device__ __noinline__ Acc slow_sums(Row<T> row, int lo, int hi, float c) {
+__device__ __noinline__ Acc slow_sums(Row<T> row, Slice sl, float c) {
   Acc a{-INFINITY, 0.f, 0.f};
-  for (int u = lo + threadIdx.x; u < hi; u += NT) {
+  for_vectors<NT>(sl, [&](int u) {
     const uint4 v = row.load(u);
     const float mx = Traits<T>::max_of(v);
     if (mx > a.m) rebase(a, mx, c);
@@ -251,7 +251,7 @@ __device__ __noinline__ Acc slow_sums(Row<T> row, int lo, int hi, float c) {
         a.t += e == 0.f ? 0.f : e * d;
       }
     }
-  }
+  });
   return a;
 }
 
@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(NT, 4) token_logprobs_kernel(const FwdParams p
   } else if (m_w == -INFINITY) {
     a = Acc{-INFINITY, s != s ? s : 0.f, 0.f};
   } else {
-    a = slow_sums(row, sl.lo, sl.hi, c);
+    a = slow_sums(row, sl, c);
   }
   rebase(a, m_w, c);
   a.s = warp_sum(a.s);
