@@ -1,0 +1,79 @@
+"""GPU: distill_loss where the teacher's tokens and the others lie far apart
+in the student, against the 64-bit oracle.
+
+Tolerances. A row's loss is p_t times the gap, and more: fp32 holds the gap
+to 2^-23 of itself, the teacher's p to 2^-22, their sum and p_t to 2^-21, and
+p_t is 0.05 or more: relative errors below 2^-16 < TOL. The gradient outside
+is p_t times a softmax over the others alone, inside it is q - p: the bound of
+the logits tests (5e-5, and half a unit of 2^-8 in bf16) holds for both.
+"""
+import math
+
+import pytest
+import torch
+
+from vllm_sm70_b200 import ops
+from vllm_sm70_b200.ops import logits as L
+
+pytestmark = pytest.mark.gpu
+TOL = 5e-5
+DTYPES = [torch.bfloat16, torch.float32]
+# (rows, V): a CTA and a cluster a row, many rows, a row that no cluster holds
+SHAPES = [(3, 64), (3, 32003), (2, 151936), (700, 8195), (2, 2 ** 21 + 5)]
+
+
+def _assert_grad(got, want, dtype):
+    rel = (2.0 ** -8 if dtype == torch.bfloat16 else 0.0) + TOL
+    err = (got.double() - want).abs()
+    lim = rel * want.abs() + TOL * want.abs().amax(1, keepdim=True) + 1e-30
+    assert bool((err <= lim).all()), float((err - lim).max())
+
+
+def _check(x, ids, lp, t, tail=True):
+    xd = x.detach().double().requires_grad_(True)
+    want = L.distill_rows_ref(xd, ids, lp, None, t, tail, dtype=torch.float64)
+    e, = torch.autograd.grad(want.sum(), xd)
+    want = want.detach()
+    assert bool(torch.isfinite(want).all()) and bool(torch.isfinite(e).all())
+    with torch.no_grad():
+        rows = ops.distill_loss(x, ids, lp, None, t, tail, reduction="none")
+    torch.testing.assert_close(rows.double(), want, atol=2 * TOL, rtol=TOL)
+    xg = x.detach().requires_grad_(True)
+    for red, scale in (("none", 1.0), ("sum", 1.0), ("mean", 1.0 / x.shape[0])):
+        loss = ops.distill_loss(xg, ids, lp, None, t, tail, reduction=red).sum()
+        g, = torch.autograd.grad(loss, xg, retain_graph=True)
+        _assert_grad(g, e * scale, x.dtype)
+        g, = torch.autograd.grad(loss, xg)  # from the saved numbers
+        _assert_grad(g, e * scale, x.dtype)
+
+
+def _rows(rows, V, K, dtype, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(rows, V, device="cuda", generator=g)
+    ids = (torch.randint(0, V, (rows, 1), device="cuda", generator=g)
+           + (V // K) * torch.arange(K, device="cuda")) % V
+    lp = torch.log_softmax(torch.randn(rows, K, device="cuda", generator=g), 1) + math.log(0.9)
+    return x.to(dtype), ids, lp
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,V", SHAPES)
+@pytest.mark.parametrize("gap,t", [(80, 1.0), (90, 1.0), (130, 1.0), (1000, 1.0), (1e4, 1.0),
+                                   (12, 0.1), (100, 0.1), (12, 0.01), (-100, 1.0), (-100, 0.1)])
+def test_gaps(b200_ops, rows, V, gap, t, dtype):
+    x, ids, lp = _rows(rows, V, 5, dtype, V)
+    x.scatter_add_(1, ids, torch.full_like(ids, 1).to(dtype) * gap)
+    _check(x, ids, lp, t)
+    if gap < 0:
+        _check(x, ids, lp, t, tail=False)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,V", SHAPES)
+@pytest.mark.parametrize("value", [-1e4, -1e9, -1e20, None])
+def test_only_the_teachers_tokens_are_allowed(b200_ops, rows, V, value, dtype):
+    """All others at a finite mask."""
+    x, ids, lp = _rows(rows, V, 5, dtype, V)
+    m = torch.full_like(x, torch.finfo(dtype).min if value is None else value)
+    m.scatter_(1, ids, x.gather(1, ids))
+    _check(m, ids, lp, 1.0)

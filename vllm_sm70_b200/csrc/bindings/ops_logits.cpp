@@ -143,7 +143,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> distill_loss(
   check_temperature(temperature, what);
   c10::cuda::CUDAGuard g(logits.device());
   const auto f = logits.options().dtype(at::kFloat);
-  auto rows = make({a.in.rows}, f), stats = make({a.in.rows, 4}, f);
+  auto rows = make({a.in.rows}, f), stats = make({a.in.rows, 8}, f);
   auto grad = make({with_grad ? a.in.rows : 0, a.in.V}, logits.options());
   auto loss = make({}, f);
   a.t_ids = t_ids.data_ptr<int>();
@@ -173,7 +173,7 @@ at::Tensor distill_loss_bwd(const at::Tensor& logits, const at::Tensor& t_ids,
   check_temperature(temperature, what);
   check_like(stats, logits, at::kFloat, what, "stats");
   check_like(g_rows, logits, at::kFloat, what, "upstream gradient");
-  TORCH_CHECK(stats.numel() == 4 * a.in.rows, what, ": stats must be [rows, 4]");
+  TORCH_CHECK(stats.numel() == 8 * a.in.rows, what, ": stats must be [rows, 8]");
   TORCH_CHECK(g_rows.dim() == 0 || g_rows.numel() == a.in.rows, what,
               ": the upstream gradient must be a scalar or [rows]");
   c10::cuda::CUDAGuard g(logits.device());

@@ -11,6 +11,11 @@
 // q_t is the sum over the other j themselves (never 1 - sum q_k, which would
 // cancel for a student that agrees with its teacher): the row's teacher ids
 // are left out of the sum, and their K exponentials are added on their own.
+// Each of the two sums stands against its own maximum, m_o and m_i, so that
+// neither is lost where the other lies far above it (a student that is sure of
+// a teacher's token by 90 nats, which at a low temperature are a few logits):
+// log q_t comes from the two logarithms, and the other j's gradient is taken
+// against m_o, e_j (M 2^((m_o - m) c) / s - p_t / s_o), e_j = 2^((x_j - m_o) c).
 //
 // A row with weight 0 has loss 0 and gradient 0 whatever it holds, and is not
 // read. Ids outside [0, V) are absent: their mass joins the tail.
@@ -21,7 +26,7 @@
 //     as much as an SM has), two or three of them an SM. A warp copies its own
 //     part of the row with asynchronous copies, takes out the teacher's
 //     elements (they read as -inf from then on), and sums the rest; the warps
-//     of the whole cluster exchange (max, sums) through each other's shared
+//     of the whole cluster exchange (maxima, sums) through each other's shared
 //     memory, the row's only meeting. Then each warp writes its part of the
 //     gradient, and as it is done with a vector starts the copy of the next
 //     row's into its place: the clusters are persistent and memory is read
@@ -169,30 +174,64 @@ __device__ __noinline__ float mass_of_id(int id, const int* ids, const float* p,
   return m;
 }
 
-// The slices' or warps' sums (max, sum outside, sum at the ids), two a lane,
-// against the largest max.
-__device__ __forceinline__ float3 join(const float4& a, const float4& b, float c) {
-  const float m = warp_max(fmaxf(a.x, b.x));
-  // a part without any element above -inf has no sums to rebase
-  const float fa = a.x == -INFINITY || a.x == m ? 1.f : ex2((a.x - m) * c);
-  const float fb = b.x == -INFINITY || b.x == m ? 1.f : ex2((b.x - m) * c);
-  return make_float3(m, warp_sum(a.y * fa + b.y * fb), warp_sum(a.z * fa + b.z * fb));
+// Maximum and sum of the elements outside the teacher's ids, and of those at
+// the ids (the first of each), of a warp, a slice or a row.
+struct __align__(16) Sums {  // (exchanged as one vector)
+  float m_out, s_out, m_in, s_in;
+};
+
+// a's factor to stand against m. (A part without any element above -inf has
+// no sum to rebase.)
+__device__ __forceinline__ float against(float a, float m, float c) {
+  return a == -INFINITY || a == m ? 1.f : ex2((a - m) * c);
 }
 
-// The row's numbers: m, M / s, the coefficient of the elements outside, the
-// teacher's normaliser. M / s is 0 for a row without a distribution.
-__device__ __forceinline__ float4 row_numbers(float norm, float sum_p, bool tail, float3 q) {
-  const float s = q.y + q.z, p_t = tail ? fmaxf(0.f, 1.f - sum_p) : 0.f;
-  const float mass = sum_p + p_t, inv = s == 0.f ? 0.f : 1.f / s;
-  // A student with no mass outside has q_j = 0 there.
-  const float ratio = p_t > 0.f && q.y != 0.f ? p_t * s / q.y : 0.f;
-  return make_float4(shift_of(q.x), mass * inv, q.y == 0.f ? 0.f : (mass - ratio) * inv, norm);
+// Two parts a lane, added up over the warp.
+__device__ __forceinline__ Sums join(const Sums& a, const Sums& b, float c) {
+  Sums q;
+  q.m_out = warp_max(fmaxf(a.m_out, b.m_out));
+  q.m_in = warp_max(fmaxf(a.m_in, b.m_in));
+  q.s_out = warp_sum(a.s_out * against(a.m_out, q.m_out, c) +
+                     b.s_out * against(b.m_out, q.m_out, c));
+  q.s_in = warp_sum(a.s_in * against(a.m_in, q.m_in, c) + b.s_in * against(b.m_in, q.m_in, c));
+  return q;
+}
+
+// What the gradient takes of a row. With x against m_out or m:
+//   outside: 2^((x - m_out) c) k_out       at an id: 2^((x - m) c) k_in - its p
+// k_in (M / s) is 0 for a row without a distribution.
+struct Numbers {
+  float m_out, k_out, m, k_in, norm;  // norm: the teacher's log-normaliser
+};
+__device__ __forceinline__ void save(float4* stats, int64_t r, const Numbers& n) {
+  stats[2 * r] = make_float4(n.m_out, n.k_out, n.m, n.k_in);
+  stats[2 * r + 1] = make_float4(n.norm, 0.f, 0.f, 0.f);
+}
+__device__ __forceinline__ Numbers saved(const float4* stats, int64_t r) {
+  const float4 n = stats[2 * r];
+  return Numbers{n.x, n.y, n.z, n.w, stats[2 * r + 1].x};
+}
+// The sum of all exponentials, against m.
+__device__ __forceinline__ float total(const Sums& q, float m, float c) {
+  return q.s_out * against(q.m_out, m, c) + q.s_in * against(q.m_in, m, c);
+}
+
+__device__ __forceinline__ Numbers row_numbers(float norm, float sum_p, bool tail, const Sums& q,
+                                               float c) {
+  const float m = fmaxf(q.m_out, q.m_in), s = total(q, m, c);
+  const float p_t = tail ? fmaxf(0.f, 1.f - sum_p) : 0.f, mass = sum_p + p_t;
+  const float k_in = s == 0.f ? 0.f : mass / s;
+  // (Without any mass outside every q_j there is 0.)
+  const float k_out = q.s_out == 0.f ? 0.f
+                                     : k_in * against(q.m_out, m, c) -
+                                           (p_t > 0.f ? p_t / q.s_out : 0.f);
+  return Numbers{shift_of(q.m_out), k_out, shift_of(m), k_in, norm};
 }
 
 // The row's loss, on a whole warp; xk: the student's logits at the ids.
-__device__ __forceinline__ float row_loss(const Teacher& t, const Params& p, float3 q,
+__device__ __forceinline__ float row_loss(const Teacher& t, const Params& p, const Sums& q,
                                           const float (&xk)[kIds]) {
-  const float s = q.y + q.z, m0 = shift_of(q.x);
+  const float m = fmaxf(q.m_out, q.m_in), m0 = shift_of(m), s = total(q, m, p.c);
   // An empty row: every log q is -inf, the loss inf where the teacher has mass.
   const float l2 = s == 0.f ? 0.f : log2f(s);
   float loss = 0.f;
@@ -206,7 +245,8 @@ __device__ __forceinline__ float row_loss(const Teacher& t, const Params& p, flo
   }
   loss = warp_sum(loss);
   const float p_t = p.tail ? fmaxf(0.f, 1.f - t.sum_p) : 0.f;
-  if (p_t > 0.f) loss += p_t * (logf(p_t) - (log2f(q.y) - l2) * kLn2);
+  if (p_t > 0.f)
+    loss += p_t * (logf(p_t) - fmaf(q.m_out - m0, p.inv_t, (log2f(q.s_out) - l2) * kLn2));
   return loss;
 }
 
@@ -329,7 +369,7 @@ __global__ void __launch_bounds__(NT, 3) distill_fused_kernel(const Params p) {
   // the same there, so none waits for another to read it. Two rows' worth: a
   // warp that has the sums of a row knows that all others are done with the
   // row before, and only then writes over that.
-  __shared__ unsigned long long parts[2][3][CL * kWarps];
+  __shared__ unsigned long long parts[2][4][CL * kWarps];
   __shared__ unsigned long long xks[2][kMaxTeacherK];  // in the cluster's first CTA
   __shared__ unsigned long long ahead[2][2];  // the next row, and its weight
   __shared__ uint64_t bar[2];
@@ -344,7 +384,7 @@ __global__ void __launch_bounds__(NT, 3) distill_fused_kernel(const Params p) {
     mbar_init(&bar[1], CL * kWarps);
     fence_barrier_init();
   }
-  for (int i = threadIdx.x; i < 6 * CL * kWarps; i += NT) (&parts[0][0][0])[i] = 0ull;
+  for (int i = threadIdx.x; i < 8 * CL * kWarps; i += NT) (&parts[0][0][0])[i] = 0ull;
   for (int i = threadIdx.x; i < 2 * kMaxTeacherK; i += NT) (&xks[0][0])[i] = 0ull;
   if (threadIdx.x < 4) (&ahead[0][0])[threadIdx.x] = 0ull;
   if constexpr (CL > 1)
@@ -462,7 +502,7 @@ __global__ void __launch_bounds__(NT, 3) distill_fused_kernel(const Params p) {
     }
 #pragma unroll 1
     for (int u = tail + lane; u < end; u += 32) vm = Tr::vmax(vm, Tr::vmax(mine[u]));
-    const float m_w = warp_max(fmaxf(Tr::value(vm), m_k));
+    const float m_w = warp_max(Tr::value(vm)), m_in = here > 0 ? warp_max(m_k) : -INFINITY;
     float s = 0.f;
     if (!slow_range(m_w, c, kFar)) {
       const float rw = __fmul_rn(m_w, c);
@@ -502,9 +542,9 @@ __global__ void __launch_bounds__(NT, 3) distill_fused_kernel(const Params p) {
     float s_in = 0.f;
 #pragma unroll 1
     for (int i = 0; 32 * i < p.K; ++i)
-      if ((own >> i) & 1u) s_in += ex2((t_x[buf][lane + 32 * i] - shift_of(m_w)) * c);
+      if ((own >> i) & 1u) s_in += ex2((t_x[buf][lane + 32 * i] - shift_of(m_in)) * c);
     s = warp_sum(s);
-    s_in = warp_sum(s_in);
+    if (here > 0) s_in = warp_sum(s_in);
     // To every CTA of the cluster; each warp hears from every other.
     if (part == 0 && warp == 0) {
       const int rn = __shfl_sync(0xffffffffu, (int)min(r_next, p.rows), 0);
@@ -517,7 +557,8 @@ __global__ void __launch_bounds__(NT, 3) distill_fused_kernel(const Params p) {
     if (lane < CL) {
       send<CL>(&parts[buf][0][part * kWarps + warp], lane, m_w, n + 1);
       send<CL>(&parts[buf][1][part * kWarps + warp], lane, s, n + 1);
-      send<CL>(&parts[buf][2][part * kWarps + warp], lane, s_in, n + 1);
+      send<CL>(&parts[buf][2][part * kWarps + warp], lane, m_in, n + 1);
+      send<CL>(&parts[buf][3][part * kWarps + warp], lane, s_in, n + 1);
       // (The barrier is where a warp sleeps until all have sent; what it then
       // reads carries its own proof.)
       if constexpr (CL == 1)
@@ -539,44 +580,44 @@ __global__ void __launch_bounds__(NT, 3) distill_fused_kernel(const Params p) {
     bool met = mbar_wait(&bar[buf], (n >> 1) & 1u, p.err);
     // (All words first: they are there as a rule.)
     constexpr int kParts = CL * kWarps, kMine = (kParts + 31) / 32;
-    unsigned long long word[3 * kMine + 2];
+    unsigned long long word[4 * kMine + 2];
 #pragma unroll
     for (int i = 0; i < kMine; ++i)
 #pragma unroll
-      for (int e = 0; e < 3; ++e)
-        word[3 * i + e] = peek(&parts[buf][e][min(lane + 32 * i, kParts - 1)]);
-    word[3 * kMine] = peek(&ahead[buf][0]);
-    word[3 * kMine + 1] = peek(&ahead[buf][1]);
+      for (int e = 0; e < 4; ++e)
+        word[4 * i + e] = peek(&parts[buf][e][min(lane + 32 * i, kParts - 1)]);
+    word[4 * kMine] = peek(&ahead[buf][0]);
+    word[4 * kMine + 1] = peek(&ahead[buf][1]);
     bool there = true;
 #pragma unroll
-    for (int i = 0; i < 3 * kMine + 2; ++i) there &= (uint32_t)(word[i] >> 32) == n + 1;
+    for (int i = 0; i < 4 * kMine + 2; ++i) there &= (uint32_t)(word[i] >> 32) == n + 1;
     if (!there) {
 #pragma unroll
       for (int i = 0; i < kMine; ++i)
 #pragma unroll
-        for (int e = 0; e < 3; ++e)
-          met &= receive(&parts[buf][e][min(lane + 32 * i, kParts - 1)], n + 1, word[3 * i + e], p.err);
-      met &= receive(&ahead[buf][0], n + 1, word[3 * kMine], p.err);
-      met &= receive(&ahead[buf][1], n + 1, word[3 * kMine + 1], p.err);
+        for (int e = 0; e < 4; ++e)
+          met &= receive(&parts[buf][e][min(lane + 32 * i, kParts - 1)], n + 1, word[4 * i + e], p.err);
+      met &= receive(&ahead[buf][0], n + 1, word[4 * kMine], p.err);
+      met &= receive(&ahead[buf][1], n + 1, word[4 * kMine + 1], p.err);
     }
-    float4 got[2];
+    Sums got[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      got[i] = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+      got[i] = Sums{-INFINITY, 0.f, -INFINITY, 0.f};
       if (i < kMine && lane + 32 * i < kParts)
-        got[i] = make_float4(value_in(word[3 * i]), value_in(word[3 * i + 1]),
-                             value_in(word[3 * i + 2]), 0.f);
+        got[i] = Sums{value_in(word[4 * i]), value_in(word[4 * i + 1]), value_in(word[4 * i + 2]),
+                      value_in(word[4 * i + 3])};
     }
-    w_next = value_in(word[3 * kMine + 1]);
+    w_next = value_in(word[4 * kMine + 1]);
     if (!__all_sync(0xffffffffu, met)) break;  // (the status word is set)
-    r_next = __float_as_int(value_in(word[3 * kMine]));
+    r_next = __float_as_int(value_in(word[4 * kMine]));
     const Row<T> next(p.x, min(r_next, p.rows - 1), p.ld, p.V);
     const int end_next = w_next != 0.f ? min(last, next.n_vec) : first;
     if (w_next != 0.f) fetch_teacher(r_next, buf ^ 1);
     if (w == 0.f) {
       if (part == 0 && threadIdx.x == 0) {
         p.row_loss[r] = 0.f;
-        p.stats[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+        save(p.stats, r, Numbers{});
       }
       for (int u = first + lane; u < min(last, row.n_vec); u += 32)
         store_vec(out, row, u, make_uint4(0u, 0u, 0u, 0u));
@@ -586,8 +627,8 @@ __global__ void __launch_bounds__(NT, 3) distill_fused_kernel(const Params p) {
     }
 
     // Every warp finishes the row's numbers (the same in all of them).
-    const float3 q = join(got[0], got[1], c);
-    const float4 st = row_numbers(norm, sum_p, p.tail, q);
+    const Sums q = join(got[0], got[1], c);
+    const Numbers st = row_numbers(norm, sum_p, p.tail, q, c);
     if (part == 0 && warp == 0) {
       Teacher t;
       t.load(t_id[buf], t_lp[buf], p.K);
@@ -610,14 +651,15 @@ __global__ void __launch_bounds__(NT, 3) distill_fused_kernel(const Params p) {
       if (!__all_sync(0xffffffffu, met)) break;
       if (lane == 0) {
         p.row_loss[r] = loss * w;
-        p.stats[r] = st;
+        save(p.stats, r, st);
       }
     }
     // The gradient: every element as an outside one (the teacher's are -inf by
     // now), then the teacher's over it. The next row's vectors follow.
     const float up = w * p.gscale;
-    const bool slow = slow_range(st.x, c, kFar);
-    const float rm = __fmul_rn(st.x, c), coef = st.z * up * (slow ? 1.f : ex2(-fmaf(st.x, c, -rm)));
+    const bool slow = slow_range(st.m_out, c, kFar);
+    const float rm = __fmul_rn(st.m_out, c),
+                coef = st.k_out * up * (slow ? 1.f : ex2(-fmaf(st.m_out, c, -rm)));
     // Whole steps of 128 full vectors without checks.
     uint4* dst = reinterpret_cast<uint4*>(out - row.pad);
     const uint4* src = reinterpret_cast<const uint4*>(next.x - next.pad);
@@ -643,7 +685,7 @@ __global__ void __launch_bounds__(NT, 3) distill_fused_kernel(const Params p) {
 #pragma unroll 1
         for (int v = u; v < min(u0 + 128, end); v += 32)
           store_vec(out, row, v,
-                    slow ? grad_vec<T, true>(mine[v], c, st.x, coef)
+                    slow ? grad_vec<T, true>(mine[v], c, st.m_out, coef)
                          : grad_vec<T, false>(mine[v], c, rm, coef));
       }
 #pragma unroll 1
@@ -656,8 +698,8 @@ __global__ void __launch_bounds__(NT, 3) distill_fused_kernel(const Params p) {
         const int k = lane + 32 * i, id = t_id[buf][k];
         float mass = t_p[buf][k];
         if (own & kDup) mass = mass_of_id(id, t_id[buf], t_p[buf], p.K);
-        const float qk = ex2((t_x[buf][k] - st.x) * c) * st.y;
-        out[id] = Tr::from_f((qk - (st.y == 0.f ? 0.f : mass)) * up);
+        const float qk = ex2((t_x[buf][k] - st.m) * c) * st.k_in;
+        out[id] = Tr::from_f((qk - (st.k_in == 0.f ? 0.f : mass)) * up);
       }
     r = r_next, w = w_next, row = next;
   }
@@ -669,7 +711,7 @@ __global__ void __launch_bounds__(NT, 3) distill_fused_kernel(const Params p) {
 struct Smem {
   Acc acc[kWarps];
   int dup;                   // some id of this slice is there twice
-  float4 part[kMaxCluster];  // a slice's max, sum outside, sum at the ids
+  Sums part[kMaxCluster];
 };
 
 // Loss, and with GRAD the gradient, of rows that are streamed: CL CTAs a row.
@@ -696,7 +738,7 @@ __global__ void __launch_bounds__(NT, 4) distill_stream_kernel(const Params p) {
         store_vec(out, row, u, make_uint4(0u, 0u, 0u, 0u));
     if (part == 0 && tid == 0) {
       p.row_loss[r] = 0.f;
-      p.stats[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+      save(p.stats, r, Numbers{});
     }
     if constexpr (CL > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
     return;
@@ -784,7 +826,7 @@ __global__ void __launch_bounds__(NT, 4) distill_stream_kernel(const Params p) {
   __syncthreads();
 
   // Warp 0 adds the warps up, with the ids' own exponentials.
-  float3 q;
+  Sums q;
   float mass[kIds];
   if (warp == 0) {
     t.prepare(p);
@@ -797,38 +839,40 @@ __global__ void __launch_bounds__(NT, 4) distill_stream_kernel(const Params p) {
         if (mass[i] == -1.f) own &= ~(1u << i);
     }
     Acc a = lane < kWarps ? sm.acc[lane] : Acc{-INFINITY, 0.f, 0.f};
-    float m_all = a.m;
+    const float m_out = warp_max(a.m);
+    rebase(a, m_out, c);
+    float m_in = -INFINITY, s_in = 0.f;
 #pragma unroll
     for (int i = 0; i < kIds; ++i)
-      if ((own >> i) & 1u) m_all = fmaxf(m_all, xk[i]);
-    m_all = warp_max(m_all);
-    rebase(a, m_all, c);
-    float s_in = 0.f;
+      if ((own >> i) & 1u) m_in = fmaxf(m_in, xk[i]);
+    m_in = warp_max(m_in);
 #pragma unroll
     for (int i = 0; i < kIds; ++i)
-      if ((own >> i) & 1u) s_in += ex2((xk[i] - shift_of(m_all)) * c);
-    q = make_float3(m_all, warp_sum(a.s), warp_sum(s_in));
+      if ((own >> i) & 1u) s_in += ex2((xk[i] - shift_of(m_in)) * c);
+    q = Sums{m_out, warp_sum(a.s), m_in, warp_sum(s_in)};
     if constexpr (CL > 1) {
       asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
       // Every CTA of the cluster gets every slice's sums.
       if (lane < CL)
-        st_dsmem_f4(mapa_shared(smem_u32(&sm.part[part]), lane), make_float4(q.x, q.y, q.z, 0.f));
+        st_dsmem_f4(mapa_shared(smem_u32(&sm.part[part]), lane),
+                    make_float4(q.m_out, q.s_out, q.m_in, q.s_in));
     }
   } else if constexpr (CL > 1) {
     asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
   }
   if constexpr (CL > 1) cluster_sync_all();
-  __shared__ float4 numbers;
+  __shared__ Numbers numbers;
   if (warp == 0) {
-    if constexpr (CL > 1)
-      q = join(lane < CL ? sm.part[lane] : make_float4(-INFINITY, 0.f, 0.f, 0.f),
-               make_float4(-INFINITY, 0.f, 0.f, 0.f), c);
-    const float4 st = row_numbers(t.norm, t.sum_p, p.tail, q);
+    if constexpr (CL > 1) {
+      const Sums none{-INFINITY, 0.f, -INFINITY, 0.f};
+      q = join(lane < CL ? sm.part[lane] : none, none, c);
+    }
+    const Numbers st = row_numbers(t.norm, t.sum_p, p.tail, q, c);
     if (part == 0) {
       const float loss = row_loss(t, p, q, xk);
       if (lane == 0) {
         p.row_loss[r] = loss * w;
-        p.stats[r] = st;
+        save(p.stats, r, st);
       }
     }
     if (lane == 0) numbers = st;
@@ -838,10 +882,10 @@ __global__ void __launch_bounds__(NT, 4) distill_stream_kernel(const Params p) {
 
   // The gradient: every element as an outside one, then the teacher's ids of
   // this slice over it (same CTA, after the barrier).
-  const float4 st = numbers;
+  const Numbers st = numbers;
   const float up = w * p.gscale;
-  if (!slow_range(st.x, c, kFar)) {
-    const float rm = __fmul_rn(st.x, c), coef = st.z * up * ex2(-fmaf(st.x, c, -rm));
+  if (!slow_range(st.m_out, c, kFar)) {
+    const float rm = __fmul_rn(st.m_out, c), coef = st.k_out * up * ex2(-fmaf(st.m_out, c, -rm));
     const int groups = (sl.b - sl.a + U * NT - 1) / (U * NT);
     for_groups<NT, U>(row, sl, [&](const uint4(&v)[U], int u, int it) {
       if (it == groups) return;  // the partial vectors, below
@@ -854,15 +898,15 @@ __global__ void __launch_bounds__(NT, 4) distill_stream_kernel(const Params p) {
     if (e >= 0) store_part(out, row, e, grad_vec<T, false>(row.load(e), c, rm, coef));
   } else {
     for (int u = sl.lo + tid; u < sl.hi; u += NT)
-      store_vec(out, row, u, grad_vec<T, true>(row.load(u), c, st.x, st.z * up));
+      store_vec(out, row, u, grad_vec<T, true>(row.load(u), c, st.m_out, st.k_out * up));
   }
   __syncthreads();
   if (warp == 0) {
 #pragma unroll
     for (int i = 0; i < kIds; ++i)
       if ((own >> i) & 1u) {
-        const float qk = ex2((xk[i] - st.x) * c) * st.y;
-        out[t.id[i]] = Tr::from_f((qk - (st.y == 0.f ? 0.f : mass[i])) * up);
+        const float qk = ex2((xk[i] - st.m) * c) * st.k_in;
+        out[t.id[i]] = Tr::from_f((qk - (st.k_in == 0.f ? 0.f : mass[i])) * up);
       }
   }
 }
@@ -908,15 +952,15 @@ __global__ void __launch_bounds__(kBwdThreads) distill_bwd_kernel(const BwdParam
   const int id = tid < p.K ? p.t_ids[r * p.K + tid] : -1;
   const int at = id + row.pad - u_lo * E;
   const bool mine = id >= 0 && id < p.V && at >= 0 && at / E < u_hi - u_lo;
-  const float4 st = p.stats[r];
+  const Numbers st = saved(p.stats, r);
   const float xk = mine ? Tr::to_f(row.x[id]) : 0.f;
-  float mass = mine ? expf(p.t_lp[r * p.K + tid] - st.w) : 0.f;
+  float mass = mine ? expf(p.t_lp[r * p.K + tid] - st.norm) : 0.f;
   for (int i = tid; i < kBits / 32; i += kBwdThreads) seen[i] = 0u;
   if (tid == 0) dup = 0;
   __syncthreads();
   if (mine && (atomicOr(&seen[at / 32], 1u << (at % 32)) >> (at % 32)) & 1u) dup = 1;
-  if (!slow_range(st.x, p.c, kFar)) {
-    const float rm = __fmul_rn(st.x, p.c), coef = st.z * up * ex2(-fmaf(st.x, p.c, -rm));
+  if (!slow_range(st.m_out, p.c, kFar)) {
+    const float rm = __fmul_rn(st.m_out, p.c), coef = st.k_out * up * ex2(-fmaf(st.m_out, p.c, -rm));
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       const int u = u_lo + tid + k * kBwdThreads;
@@ -924,7 +968,7 @@ __global__ void __launch_bounds__(kBwdThreads) distill_bwd_kernel(const BwdParam
     }
   } else {
     for (int u = u_lo + tid; u < u_hi; u += kBwdThreads)
-      store_vec(out, row, u, grad_vec<T, true>(row.load(u), p.c, st.x, st.z * up));
+      store_vec(out, row, u, grad_vec<T, true>(row.load(u), p.c, st.m_out, st.k_out * up));
   }
   __syncthreads();
   if (!mine) return;
@@ -933,11 +977,11 @@ __global__ void __launch_bounds__(kBwdThreads) distill_bwd_kernel(const BwdParam
     for (int j = 0; j < p.K; ++j)
       if (p.t_ids[r * p.K + j] == id) {
         if (j < tid) return;
-        mass += expf(p.t_lp[r * p.K + j] - st.w);
+        mass += expf(p.t_lp[r * p.K + j] - st.norm);
       }
   }
-  const float q = ex2((xk - st.x) * p.c) * st.y;
-  out[id] = Tr::from_f((q - (st.y == 0.f ? 0.f : mass)) * up);
+  const float q = ex2((xk - st.m) * p.c) * st.k_in;
+  out[id] = Tr::from_f((q - (st.k_in == 0.f ? 0.f : mass)) * up);
 }
 
 // loss = scale * sum of the rows' losses, one CTA, fixed order.
@@ -1125,7 +1169,7 @@ void distill_bwd_launch(const DistillBwdArgs& a, cudaStream_t stream) {
                  a.t_lp + r0 * a.K, a.weights ? a.weights + r0 : nullptr, a.in.ld, a.in.V, a.K, n,
                  a.tail, (float)(1.4426950408889634 / a.temperature), (float)(1.0 / a.temperature),
                  (float)((double)a.g_scale / a.temperature), 0.f, nullptr,
-                 reinterpret_cast<float4*>(const_cast<float*>(a.stats)) + r0,
+                 reinterpret_cast<float4*>(const_cast<float*>(a.stats)) + 2 * r0,
                  reinterpret_cast<char*>(a.grad) + r0 * a.in.V * eb, nullptr, nullptr};
     b.g = a.g_rows + r0 * a.g_stride;
     b.g_stride = a.g_stride;

@@ -59,8 +59,7 @@ struct DistillArgs {
   bool tail;
   float grad_scale;    // dL/d(row loss * weight): 1 (sum) or 1 / rows (mean)
   float* row_loss;     // [rows], times weight
-  float* stats;        // [rows, 4] for distill_bwd: m, M / s, outside coefficient,
-                       // the teacher's log-normaliser
+  float* stats;        // [rows, 8] for distill_bwd: Numbers of distill.cu
   void* grad;          // [rows, V] contiguous or nullptr (forward only)
   int* counter;        // one int of scratch, with grad
   float* loss;         // scalar: grad_scale * sum(row_loss), or nullptr

@@ -81,7 +81,7 @@ def register_all() -> None:
     def _distill_loss(logits, ids, lp, weights, temperature, tail, scale, with_loss, with_grad):
         T, V = logits.shape
         f = torch.float32
-        return (logits.new_empty(T, dtype=f), logits.new_empty((T, 4), dtype=f),
+        return (logits.new_empty(T, dtype=f), logits.new_empty((T, 8), dtype=f),
                 logits.new_empty((T if with_grad else 0, V)), logits.new_empty((), dtype=f))
 
     @torch.library.register_fake(f"{LIB}::distill_loss_bwd")
