@@ -77,3 +77,25 @@ def test_only_the_teachers_tokens_are_allowed(b200_ops, rows, V, value, dtype):
     m = torch.full_like(x, torch.finfo(dtype).min if value is None else value)
     m.scatter_(1, ids, x.gather(1, ids))
     _check(m, ids, lp, 1.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [5003, 2 ** 21 + 5])
+@pytest.mark.parametrize("tail", [True, False])
+def test_teacher_rows_without_a_distribution(b200_ops, V, tail, dtype):
+    """What token_logprobs says of a row whose mask leaves nothing: ids with
+    log-probs of -inf, which are no mass."""
+    x, _, _ = _rows(4, V, 5, dtype, 1)
+    teacher = x.roll(1, 0).clone()
+    teacher[1] = -float("inf")
+    s = ops.token_logprobs(teacher, torch.zeros(4, dtype=torch.int64, device="cuda"), top_n=6)
+    assert bool((s.top_logprobs[1] == -float("inf")).all())
+    _check(x, s.top_ids, s.top_logprobs, 1.0, tail)
+    xg = x.detach().requires_grad_(True)
+    for red in ("none", "sum"):
+        loss = ops.distill_loss(xg, s.top_ids, s.top_logprobs, tail=tail, reduction=red)
+        g, = torch.autograd.grad(loss.sum(), xg)
+        if not tail:
+            assert bool((g[1] == 0).all())
+            if red == "none":
+                assert float(loss[1].detach()) == 0

@@ -117,7 +117,8 @@ struct Teacher {
 #pragma unroll
       for (int i = 0; i < kIds; ++i)
         if (32 * i < q.K && id[i] >= 0) z += expf(lp[i] - mx);
-      norm = mx + logf(warp_sum(z));
+      // A teacher that gives none of its ids any probability has no mass.
+      norm = mx == -INFINITY ? 0.f : mx + logf(warp_sum(z));
     }
 #pragma unroll
     for (int i = 0; i < kIds; ++i) {

@@ -183,7 +183,8 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logpro
     * ``tail=True``: ``sum_k p_k (log p_k - log q_k) + p_t (log p_t - log
       q_t)``, where ``p_t`` and ``q_t`` are the masses outside the K tokens
       (``p_t = max(0, 1 - sum p_k)``);
-    * ``tail=False``: the sum over the K alone, ``p`` renormalised over them.
+    * ``tail=False``: the sum over the K alone, ``p`` renormalised over them
+      (loss and gradient 0 where none of them has any).
 
     ``weights [rows]`` multiply the rows' losses; a row of weight 0 counts
     nothing, whatever it holds, and is not read. ``reduction``: ``"none"``
