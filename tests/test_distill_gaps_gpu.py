@@ -99,3 +99,18 @@ def test_teacher_rows_without_a_distribution(b200_ops, V, tail, dtype):
             assert bool((g[1] == 0).all())
             if red == "none":
                 assert float(loss[1].detach()) == 0
+
+
+@pytest.mark.parametrize("V", [5003, 2 ** 21 + 5])
+@pytest.mark.parametrize("tail", [True, False])
+def test_nan_of_the_teacher_reaches_loss_and_gradient(b200_ops, V, tail):
+    x, ids, lp = _rows(3, V, 5, torch.float32, 1)
+    lp[1, 2] = float("nan")
+    xg = x.requires_grad_(True)
+    for red in ("none", "sum"):
+        loss = ops.distill_loss(xg, ids, lp, tail=tail, reduction=red)
+        assert torch.isnan(loss).tolist() == ([False, True, False] if red == "none" else True)
+        g, = torch.autograd.grad(loss.sum(), xg)
+        assert torch.isnan(g).any(1).tolist() == [False, True, False]
+    ids[1, 2] = -1  # an absent id's value is not read
+    assert bool(torch.isfinite(ops.distill_loss(xg, ids, lp, tail=tail)))

@@ -91,10 +91,11 @@ def distill_rows_ref(logits: torch.Tensor, teacher_ids: torch.Tensor,
     at = torch.where(ok, ids, torch.zeros_like(ids))
     lp = torch.where(ok, teacher_logprobs.to(dtype), float("-inf"))
     if not tail:
-        lp = lp - torch.logsumexp(lp, 1, keepdim=True)
-        lp = torch.where(ok, lp, float("-inf"))
+        norm = torch.logsumexp(lp, 1, keepdim=True)
+        lp = torch.where(ok, lp - torch.where(norm == float("-inf"), torch.zeros_like(norm), norm),
+                         float("-inf"))
     p = torch.exp(lp)
-    on = p > 0
+    on = ~(p <= 0)  # a NaN counts
     zero = torch.zeros_like(p)
     rows = torch.where(on, p * (torch.where(on, lp, zero) - torch.where(on, lq.gather(1, at), zero)),
                        zero).sum(1)
