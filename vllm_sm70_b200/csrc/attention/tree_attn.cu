@@ -49,8 +49,9 @@
 //   warp 11    issues O += P V (its own warp: an issuing thread spends longer
 //              on waits and descriptors than the tensor core on a product)
 //   warp 12    loads Q rows (the next unit's while the present one runs) and
-//              zeroes V rows that no node sees (past the end, before the
-//              window): they may hold anything, and 0 x NaN is not 0.
+//              zeroes V rows that no node of the tile sees (past the end,
+//              before the window, slots of nodes whose bit is nowhere set):
+//              they may hold anything, and 0 x NaN is not 0.
 // TMEM columns: S0 | S1 | S2 | O.
 //
 // Measured (32 query, 8 key heads of 128, blocks of 16): 64 trees of 16 nodes
@@ -243,9 +244,10 @@ struct __align__(16) Unit {
   int k_first, pad[3];
   template <int FN>
   __device__ __forceinline__ bool dirty(int j) const {
-    // Has tile j rows of V that no node sees?
+    // May tile j have rows of V that no node sees? (A node's own slot is one
+    // where no mask row has its bit.)
     const int kbase = k_lo + j * FN;
-    return kbase + FN > seq_len || kbase < k_first;
+    return kbase + FN > prefix || kbase < k_first;
   }
 };
 
@@ -659,11 +661,28 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
       if (ok && more && NQ > 1) ok = load_q(u + 1, next);
       for (int j = x.j0; j < x.j1 && ok; ++j, ++n) {
         if (!x.template dirty<FN>(j)) continue;
+        const int kbase = x.k_lo + j * FN;
+        // The tile's tree slots that some row of this unit sees; none from
+        // the end on. (Read before the wait for V.)
+        uint32_t seen[FN / 32];
+#pragma unroll
+        for (int w = 0; w < FN / 32; ++w) seen[w] = 0u;
+        if (kbase + FN > x.prefix) {
+          const int last = (x.row0 + min(FM, x.rows) - 1) / p.G;
+          for (int t = x.row0 / p.G + lane; t <= last; t += 32) {
+            MaskRow m{p.mask + (long long)(x.q0 + t) * p.mask_words, p.mask_words, x.nodes, 0u, 0u};
+            m.w0 = __ldg(m.row);
+            if (p.mask_words > 1) m.w1 = __ldg(m.row + 1);
+#pragma unroll
+            for (int w = 0; w < FN / 32; ++w) seen[w] |= m.bits(kbase + 32 * w - x.prefix);
+          }
+#pragma unroll
+          for (int w = 0; w < FN / 32; ++w) seen[w] = __reduce_or_sync(0xffffffffu, seen[w]);
+        }
         // (Its V has landed: warp 11 has waited for it.)
         ok = __all_sync(0xffffffffu, mbar_wait(v_dirty, (uint32_t)(got & 1), p.err));
         if (!ok) break;
         uint8_t* sv = sV + (n % NV) * C::kTile;
-        const int kbase = x.k_lo + j * FN;
         constexpr int kU = D / 8;
         auto zero = [&](int from, int to) {  // rows [from, to)
           for (int i = from * kU + lane; i < to * kU; i += 32) {
@@ -674,6 +693,12 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant_
         };
         zero(0, min(FN, x.k_first - kbase));
         zero(max(0, x.seq_len - kbase), FN);
+#pragma unroll
+        for (int w = 0; w < FN / 32; ++w) {
+          const int k0 = kbase + 32 * w;
+          for (uint32_t b = range_bits(x.prefix - k0, x.seq_len - k0) & ~seen[w]; b; b &= b - 1)
+            zero(32 * w + __ffs(b) - 1, 32 * w + __ffs(b));
+        }
         fence_proxy_async_shared();
         __syncwarp();
         if (lane == 0) mbar_arrive(v_clean);

@@ -124,7 +124,10 @@ def tree_attention(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor,
     node that sees nothing (no prefix, no bits) gets 0. ``window > 0`` limits
     the prefix to the positions ``> prefix + depth - window`` (depth: the bits
     of the row minus one); it has to hold the whole tree (``32 * words``).
-    ``sinks [Hq]`` join the denominators. Head sizes 64, 128 and 256, any
+    ``sinks [Hq]`` join the denominators. Cache entries that no node sees may
+    hold anything, NaN too: those from ``seq_lens[s]`` on, before the window of
+    a node of depth 0, and the slots of nodes whose bit no row sets. What one
+    node sees has to be finite for the others too. Head sizes 64, 128 and 256, any
     number of query heads a key head, block sizes of a power of two from 8.
     Lengths are read on the device: a captured graph replays with new ones.
     """
