@@ -95,3 +95,27 @@ def test_a_tree_that_sees_none_of_itself(b200_ops, heads):
     q, kc, vc, bt, sl, cu, m = _setup(lens, nodes, heads, 16)
     m = _forget(m, kc, vc, bt, lens, nodes, [range(24), range(24), range(1)], float("nan"))
     _check(q, kc, vc, bt, sl, cu, m)
+
+
+def test_rows_of_no_tree_are_left_as_they_are(b200_ops):
+    """Also where a captured graph is replayed with fewer nodes."""
+    lens, nodes = [700, 90], [9, 5]
+    q, kc, vc, bt, sl, cu, m = _setup(lens, nodes, (32, 8, 128), 16)
+    more = torch.cat([q, q[:3]])
+    mm = torch.cat([m, m[:3]])
+    out = torch.full_like(more, 7.0)
+    ops.tree_attention(out, more, kc, vc, bt, sl, cu, mm, 0.09)
+    want = ops.tree_attention(torch.empty_like(q), q, kc, vc, bt, sl, cu, m, 0.09)
+    assert bool((out[14:] == 7).all()) and torch.equal(out[:14], want)
+    ws, now = ops.tree_attention_workspace(128, "cuda"), cu.clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.tree_attention(out, more, kc, vc, bt, sl, now, mm, 0.09, workspace=ws)
+    for n in (17, 14, 11):
+        now.copy_(torch.tensor([0, 9, n]))
+        out.fill_(7.0)
+        graph.replay()
+        want = ops.tree_attention(torch.empty_like(more[:n]), more[:n], kc, vc, bt, sl, now.clone(),
+                                  mm[:n], 0.09)
+        assert bool((out[n:] == 7).all()) and torch.equal(out[:n], want)

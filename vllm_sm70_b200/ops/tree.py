@@ -129,7 +129,9 @@ def tree_attention(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor,
     a node of depth 0, and the slots of nodes whose bit no row sets. What one
     node sees has to be finite for the others too. Head sizes 64, 128 and 256, any
     number of query heads a key head, block sizes of a power of two from 8.
-    Lengths are read on the device: a captured graph replays with new ones.
+    Lengths are read on the device: a captured graph replays with new ones,
+    and with fewer nodes than ``T`` (rows of ``out`` that belong to no tree,
+    from ``cu_q[B]`` on, are left as they are).
     """
     if q.dim() != 3 or out.shape != q.shape or mask.dim() != 2 or mask.shape[0] != q.shape[0]:
         raise ValueError(f"tree_attention: out and q [T, Hq, D] and mask [T, words], got "
@@ -148,6 +150,8 @@ def tree_attention(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor,
                                          mask, scale, window, sinks, workspace)
         launch_count.add(2)
         return out
-    out.copy_(tree_attention_ref(q, k_cache, v_cache, block_table, seq_lens, cu_q, mask, scale,
-                                 window, sinks).to(out.dtype))
+    r = tree_attention_ref(q, k_cache, v_cache, block_table, seq_lens, cu_q, mask, scale, window,
+                           sinks)
+    first, last = int(cu_q[0]), min(int(cu_q[-1]), q.shape[0])
+    out[first:last] = r[first:last].to(out.dtype)
     return out
