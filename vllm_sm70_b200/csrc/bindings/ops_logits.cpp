@@ -250,6 +250,26 @@ void call_scale_by(at::Tensor& x, const at::Tensor& f) {
   op.call(x, f);
 }
 
+// Neither operator has forward-mode derivatives: a tangent is refused, not
+// dropped (below the autograd keys nothing would know of it).
+void refuse_tangent(const at::Tensor& t, const char* what) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(/*level=*/0).defined(), what,
+                              ": forward-mode derivatives are not implemented");
+}
+Six token_logprobs_ad(const at::Tensor& x, const at::Tensor& ids, int64_t top_n, double t) {
+  refuse_tangent(x, "token_logprobs");
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return call_token_logprobs(x, ids, top_n, t);
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> distill_loss_ad(
+    const at::Tensor& x, const at::Tensor& ids, const at::Tensor& lp, const OptTensor& w, double t,
+    bool tail, double scale, bool with_loss, bool with_grad) {
+  for (const at::Tensor* p : {&x, &lp}) refuse_tangent(*p, "distill_loss");
+  if (w) refuse_tangent(*w, "distill_loss");
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return call_distill(x, ids, lp, w, t, tail, scale, with_loss, with_grad);
+}
+
 OptTensor opt(const at::Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 
 // A gradient that a graph of gradients may hold, and that raises where it is
@@ -381,6 +401,11 @@ TORCH_LIBRARY_IMPL(_b200_C, CUDA, m) {
   m.impl("distill_loss", &b200::distill_loss);
   m.impl("distill_loss_bwd", &b200::distill_loss_bwd);
   m.impl("scale_by", &b200::scale_by);
+}
+
+TORCH_LIBRARY_IMPL(_b200_C, Autograd, m) {
+  m.impl("token_logprobs", &b200::token_logprobs_ad);
+  m.impl("distill_loss", &b200::distill_loss_ad);
 }
 
 TORCH_LIBRARY_IMPL(_b200_C, CompositeImplicitAutograd, m) {

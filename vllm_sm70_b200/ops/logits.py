@@ -1,6 +1,7 @@
 """Operators over rows of logits: log-probabilities of given tokens with
 their rank, entropy and top alternatives, and distillation from a teacher's
-top log-probabilities. Both have a backward pass.
+top log-probabilities. Both have a backward pass (reverse mode, once; on CUDA
+tensors forward-mode derivatives raise ``NotImplementedError``).
 
 Rows of logits are ``[rows, V]``, bf16 or fp32, with a unit inner stride and
 any row stride (a slice of a wider buffer is read in place). Sums are held in
