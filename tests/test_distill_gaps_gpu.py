@@ -114,3 +114,36 @@ def test_nan_of_the_teacher_reaches_loss_and_gradient(b200_ops, V, tail):
         assert torch.isnan(g).any(1).tolist() == [False, True, False]
     ids[1, 2] = -1  # an absent id's value is not read
     assert bool(torch.isfinite(ops.distill_loss(xg, ids, lp, tail=tail)))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,V", [(5, 3001), (700, 8195), (2, 2 ** 21 + 5)])
+@pytest.mark.parametrize("up", [0.37, -3.0, 1.0, 1e-3])
+def test_gradient_is_rounded_once_for_any_upstream(b200_ops, up, rows, V, dtype):
+    """Half a unit of the type, once; and the graph gives the same bits again."""
+    x, ids, lp = _rows(rows, V, 5, dtype, 3)
+    ids[0, 4] = ids[0, 1]
+    w = 0.5 + torch.rand(rows, device="cuda")
+    xd = x.double().requires_grad_(True)
+    e, = torch.autograd.grad(
+        L.distill_rows_ref(xd, ids, lp, w.double(), 1.0, True, dtype=torch.float64).mean() * up, xd)
+    loss = ops.distill_loss(x.requires_grad_(True), ids, lp, w) * up
+    g1, = torch.autograd.grad(loss, x, retain_graph=True)
+    g2, = torch.autograd.grad(loss, x)
+    assert torch.equal(g1, g2)
+    # a bf16 value's unit is 2^-7 of the power of two below it: half of it is
+    # between 2^-9 and 2^-8 of the value. Twice rounded is up to 1.5 halves.
+    half = torch.exp2(torch.floor(torch.log2(e.abs().clamp(min=1e-300)))) * 2.0 ** -8 \
+        if dtype == torch.bfloat16 else 0.0
+    err = (g1.double() - e).abs()
+    assert bool((err <= 1.001 * half + TOL * e.abs() + TOL * 0.01 * e.abs().amax(1, keepdim=True)
+                 + 1e-30).all())
+
+
+def test_upstream_of_zero(b200_ops):
+    """Nothing comes back: no gradient, whatever a row holds."""
+    x, ids, lp = _rows(5, 3001, 5, torch.bfloat16, 3)
+    x[2] = float("nan")
+    loss = ops.distill_loss(x.requires_grad_(True), ids, lp) * 0.0
+    g, = torch.autograd.grad(loss, x)
+    assert bool((g == 0).all())

@@ -162,11 +162,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> distill_loss(
   return {rows, stats, grad, loss};
 }
 
-at::Tensor distill_loss_bwd(const at::Tensor& logits, const at::Tensor& t_ids,
-                            const at::Tensor& t_lp, const OptTensor& weights, double temperature,
-                            bool tail, const at::Tensor& stats, const at::Tensor& g_rows,
-                            double scale) {
-  const char* what = "distill_loss_bwd";
+void distill_bwd_into(const at::Tensor& grad, const at::Tensor& logits, const at::Tensor& t_ids,
+                      const at::Tensor& t_lp, const OptTensor& weights, double temperature,
+                      bool tail, const at::Tensor& stats, const at::Tensor& g_rows, double scale,
+                      bool unless_one, const char* what) {
   DistillBwdArgs a{};
   a.in = check_logits(logits, what);
   check_teacher(logits, t_ids, t_lp, weights, what);
@@ -176,8 +175,6 @@ at::Tensor distill_loss_bwd(const at::Tensor& logits, const at::Tensor& t_ids,
   TORCH_CHECK(stats.numel() == 8 * a.in.rows, what, ": stats must be [rows, 8]");
   TORCH_CHECK(g_rows.dim() == 0 || g_rows.numel() == a.in.rows, what,
               ": the upstream gradient must be a scalar or [rows]");
-  c10::cuda::CUDAGuard g(logits.device());
-  auto grad = make({a.in.rows, a.in.V}, logits.options());
   a.t_ids = t_ids.data_ptr<int>();
   a.t_lp = t_lp.data_ptr<float>();
   a.K = (int)t_ids.size(1);
@@ -188,20 +185,36 @@ at::Tensor distill_loss_bwd(const at::Tensor& logits, const at::Tensor& t_ids,
   a.g_rows = g_rows.data_ptr<float>();
   a.g_stride = g_rows.dim() == 0 ? 0 : 1;
   a.g_scale = (float)scale;
+  a.unless_one = unless_one;
   a.grad = grad.data_ptr();
   distill_bwd_launch(a, stream_now());
+}
+
+at::Tensor distill_loss_bwd(const at::Tensor& logits, const at::Tensor& t_ids,
+                            const at::Tensor& t_lp, const OptTensor& weights, double temperature,
+                            bool tail, const at::Tensor& stats, const at::Tensor& g_rows,
+                            double scale) {
+  const char* what = "distill_loss_bwd";
+  const LogitRows in = check_logits(logits, what);
+  c10::cuda::CUDAGuard g(logits.device());
+  auto grad = make({in.rows, in.V}, logits.options());
+  distill_bwd_into(grad, logits, t_ids, t_lp, weights, temperature, tail, stats, g_rows, scale,
+                   false, what);
   return grad;
 }
 
-void scale_by(at::Tensor& x, const at::Tensor& scale) {
-  const bool bf = x.scalar_type() == at::kBFloat16;
-  TORCH_CHECK(x.is_cuda() && x.is_contiguous() && (bf || x.scalar_type() == at::kFloat),
-              "scale_by: contiguous bf16 or fp32 CUDA tensor");
-  TORCH_CHECK((reinterpret_cast<uintptr_t>(x.data_ptr()) & 15) == 0, "scale_by: 16-byte aligned");
-  TORCH_CHECK(scale.device() == x.device() && scale.scalar_type() == at::kFloat &&
-              scale.numel() == 1, "scale_by: one fp32 value on the tensor's device");
-  c10::cuda::CUDAGuard g(x.device());
-  scale_by_launch(x.data_ptr(), bf, x.numel(), scale.data_ptr<float>(), stream_now());
+// The gradient for the upstream scalar `g` over that for 1, which `grad` holds.
+void distill_loss_redo(at::Tensor& grad, const at::Tensor& logits, const at::Tensor& t_ids,
+                       const at::Tensor& t_lp, const OptTensor& weights, double temperature,
+                       bool tail, const at::Tensor& stats, const at::Tensor& g, double scale) {
+  const char* what = "distill_loss_redo";
+  check_logits(logits, what);
+  check_like(grad, logits, logits.scalar_type(), what, "grad");
+  TORCH_CHECK(grad.sizes() == logits.sizes() && g.dim() == 0, what,
+              ": grad must have the logits' shape, the upstream gradient be a scalar");
+  c10::cuda::CUDAGuard guard(logits.device());
+  distill_bwd_into(grad, logits, t_ids, t_lp, weights, temperature, tail, stats, g, scale, true,
+                   what);
 }
 
 // ---------------------------------------------------------------- training
@@ -244,10 +257,12 @@ at::Tensor call_distill_bwd(const at::Tensor& x, const at::Tensor& ids, const at
   g_backward_launches += 1;
   return op.call(x, ids, lp, w, t, tail, stats, g, scale);
 }
-void call_scale_by(at::Tensor& x, const at::Tensor& f) {
-  static auto op = handle<decltype(scale_by)>("_b200_C::scale_by");
+void call_distill_redo(at::Tensor& grad, const at::Tensor& x, const at::Tensor& ids,
+                       const at::Tensor& lp, const OptTensor& w, double t, bool tail,
+                       const at::Tensor& stats, const at::Tensor& g, double scale) {
+  static auto op = handle<decltype(distill_loss_redo)>("_b200_C::distill_loss_redo");
   g_backward_launches += 1;
-  op.call(x, f);
+  op.call(grad, x, ids, lp, w, t, tail, stats, g, scale);
 }
 
 // Neither operator has forward-mode derivatives: a tangent is refused, not
@@ -324,8 +339,8 @@ struct DistillRowsFn : public Function<DistillRowsFn> {
   }
 };
 
-// Loss and gradient in one pass over the logits; the upstream scalar is applied
-// in backward (nothing is written where it is 1).
+// Loss and gradient in one pass over the logits, for the upstream scalar 1;
+// where backward gets another, the gradient is computed anew there.
 struct DistillScalarFn : public Function<DistillScalarFn> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& ids,
                             const at::Tensor& lp, const OptTensor& w, double t, bool tail,
@@ -341,16 +356,16 @@ struct DistillScalarFn : public Function<DistillScalarFn> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto s = ctx->get_saved_variables();
     at::AutoDispatchBelowADInplaceOrView guard;
+    const double t = ctx->saved_data["t"].toDouble(), scale = ctx->saved_data["scale"].toDouble();
+    const bool tail = ctx->saved_data["tail"].toBool();
     auto held = ctx->saved_data.find("grad");
     at::Tensor grad;
     if (held != ctx->saved_data.end()) {
       grad = held->second.toTensor();
       ctx->saved_data.erase(held);
-      call_scale_by(grad, g[0]);
+      call_distill_redo(grad, s[0], s[1], s[2], opt(s[3]), t, tail, s[4], g[0], scale);
     } else {  // the graph is run again: the first run gave its gradient away
-      grad = call_distill_bwd(s[0], s[1], s[2], opt(s[3]), ctx->saved_data["t"].toDouble(),
-                              ctx->saved_data["tail"].toBool(), s[4], g[0],
-                              ctx->saved_data["scale"].toDouble());
+      grad = call_distill_bwd(s[0], s[1], s[2], opt(s[3]), t, tail, s[4], g[0], scale);
     }
     return {once(grad),   at::Tensor(), at::Tensor(), at::Tensor(),
             at::Tensor(), at::Tensor(), at::Tensor()};
@@ -392,7 +407,9 @@ TORCH_LIBRARY_FRAGMENT(_b200_C, m) {
   m.def("distill_loss_bwd(Tensor logits, Tensor teacher_ids, Tensor teacher_logprobs, "
         "Tensor? weights, float temperature, bool tail, Tensor stats, Tensor g_rows, "
         "float scale) -> Tensor");
-  m.def("scale_by(Tensor(a!) x, Tensor scale) -> ()");
+  m.def("distill_loss_redo(Tensor(a!) grad, Tensor logits, Tensor teacher_ids, "
+        "Tensor teacher_logprobs, Tensor? weights, float temperature, bool tail, Tensor stats, "
+        "Tensor g, float scale) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(_b200_C, CUDA, m) {
@@ -400,7 +417,7 @@ TORCH_LIBRARY_IMPL(_b200_C, CUDA, m) {
   m.impl("token_logprobs_bwd", &b200::token_logprobs_bwd);
   m.impl("distill_loss", &b200::distill_loss);
   m.impl("distill_loss_bwd", &b200::distill_loss_bwd);
-  m.impl("scale_by", &b200::scale_by);
+  m.impl("distill_loss_redo", &b200::distill_loss_redo);
 }
 
 TORCH_LIBRARY_IMPL(_b200_C, Autograd, m) {

@@ -64,6 +64,7 @@ constexpr int NT = 256;
 constexpr int kWarps = NT / 32;
 constexpr int U = 4;
 constexpr int kBwdThreads = 128;
+constexpr int kBwdCtas = 10;  // an SM
 static_assert(kMaxTeacherK <= kBwdThreads, "a thread a teacher entry");
 constexpr int kMaxCluster = 8;
 
@@ -913,27 +914,26 @@ __global__ void __launch_bounds__(NT, 4) distill_stream_kernel(const Params p) {
 }
 
 // The same gradient for an upstream value a row: elementwise on the saved
-// numbers. One CTA a (row, chunk of kBwdThreads * U vectors).
+// numbers, a CTA a (row, chunk of kBwdThreads * U vectors).
 struct BwdParams {
   Params f;
   const float* g;
   int g_stride;
+  int chunks;
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kBwdThreads) distill_bwd_kernel(const BwdParams b) {
+__device__ __forceinline__ void bwd_chunk(const BwdParams& b, unsigned r0, unsigned chunk) {
+  const int64_t r = r0;
   using Tr = Traits<T>;
   constexpr int E = Tr::E;
   constexpr int kBits = kBwdThreads * U * E;  // elements of the chunk
   __shared__ uint32_t seen[kBits / 32];
   __shared__ int dup;
-  pdl_wait();
-  pdl_trigger();
   const Params& p = b.f;
-  const int64_t r = blockIdx.y;
   const int tid = threadIdx.x;
   const Row<T> row(p.x, r, p.ld, p.V);
-  const int u_lo = blockIdx.x * (kBwdThreads * U), u_hi = min(u_lo + kBwdThreads * U, row.n_vec);
+  const int u_lo = chunk * (kBwdThreads * U), u_hi = min(u_lo + kBwdThreads * U, row.n_vec);
   if (u_lo >= u_hi) return;
   T* out = reinterpret_cast<T*>(p.grad) + r * p.V;
   const float w = p.weights ? p.weights[r] : 1.f;
@@ -985,6 +985,30 @@ __global__ void __launch_bounds__(kBwdThreads) distill_bwd_kernel(const BwdParam
   out[id] = Tr::from_f((q - (st.k_in == 0.f ? 0.f : mass)) * up);
 }
 
+template <typename T>
+__global__ void __launch_bounds__(kBwdThreads) distill_bwd_kernel(const __grid_constant__ BwdParams b) {
+  pdl_wait();
+  pdl_trigger();
+  bwd_chunk<T>(b, blockIdx.y, blockIdx.x);
+}
+
+// Where the upstream scalar is 1 the forward pass has left the gradient as it
+// has to be. Any other value's is computed anew from the logits (as many bytes
+// as scaling would move), so that it is rounded once too. As many CTAs as run
+// at the same time: as a rule they have nothing to do.
+template <typename T>
+__global__ void __launch_bounds__(kBwdThreads, kBwdCtas) distill_redo_kernel(const __grid_constant__ BwdParams b) {
+  pdl_wait();
+  pdl_trigger();
+  if (*b.g == 1.f) return;
+  const int64_t n = b.f.rows * b.chunks;
+  for (int64_t i = blockIdx.x; i < n; i += gridDim.x) {
+    const int64_t r = i / b.chunks;
+    bwd_chunk<T>(b, (unsigned)r, (unsigned)(i - r * b.chunks));
+    __syncthreads();
+  }
+}
+
 // loss = scale * sum of the rows' losses, one CTA, fixed order.
 __global__ void __launch_bounds__(1024) sum_rows_kernel(const float* x, int64_t n, float scale,
                                                         float* out) {
@@ -1000,30 +1024,6 @@ __global__ void __launch_bounds__(1024) sum_rows_kernel(const float* x, int64_t 
     s = warp_sum(part[threadIdx.x]);
     if (threadIdx.x == 0) *out = s * scale;
   }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(256) scale_by_kernel(T* x, int64_t n, const float* scale) {
-  pdl_wait();
-  pdl_trigger();
-  const float f = *scale;
-  if (f == 1.f) return;
-  constexpr int E = Traits<T>::E;
-  const int64_t stride = (int64_t)gridDim.x * 256;
-  const int64_t nv = n / E;  // x is 16-byte aligned
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < nv; i += stride) {
-    uint4 v = reinterpret_cast<uint4*>(x)[i];
-    float g[E];
-#pragma unroll
-    for (int k = 0; k < E / 2; ++k) {
-      Traits<T>::pair(v, k, g[2 * k], g[2 * k + 1]);
-      g[2 * k] *= f;
-      g[2 * k + 1] *= f;
-    }
-    reinterpret_cast<uint4*>(x)[i] = Traits<T>::pack(g);
-  }
-  for (int64_t i = nv * E + (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += stride)
-    x[i] = Traits<T>::from_f(Traits<T>::to_f(x[i]) * f);
 }
 
 void check(const LogitRows& in, int K, const char* what) {
@@ -1160,11 +1160,14 @@ void distill_launch(const DistillArgs& a, cudaStream_t stream) {
 
 void distill_bwd_launch(const DistillBwdArgs& a, cudaStream_t stream) {
   check(a.in, a.K, "distill_loss_bwd");
+  if (a.in.rows <= 0) return;
   const int E = a.in.bf16 ? 8 : 4;
   const int64_t eb = a.in.bf16 ? 2 : 4;
   const unsigned chunks = (unsigned)((a.in.V + 2 * E - 2) / E + kBwdThreads * U - 1) / (kBwdThreads * U);
-  for (int64_t r0 = 0; r0 < a.in.rows; r0 += 65535) {  // grid.y limit
-    const unsigned n = (unsigned)(a.in.rows - r0 < 65535 ? a.in.rows - r0 : 65535);
+  // grid.y holds at most 65535 rows a launch
+  const int64_t most = a.unless_one ? a.in.rows : 65535;
+  for (int64_t r0 = 0; r0 < a.in.rows; r0 += most) {
+    const int64_t n = a.in.rows - r0 < most ? a.in.rows - r0 : most;
     BwdParams b{};
     b.f = Params{reinterpret_cast<const char*>(a.in.x) + r0 * a.in.ld * eb, a.t_ids + r0 * a.K,
                  a.t_lp + r0 * a.K, a.weights ? a.weights + r0 : nullptr, a.in.ld, a.in.V, a.K, n,
@@ -1174,26 +1177,19 @@ void distill_bwd_launch(const DistillBwdArgs& a, cudaStream_t stream) {
                  reinterpret_cast<char*>(a.grad) + r0 * a.in.V * eb, nullptr, nullptr};
     b.g = a.g_rows + r0 * a.g_stride;
     b.g_stride = a.g_stride;
-    if (a.in.bf16)
-      launch_pdl(distill_bwd_kernel<__nv_bfloat16>, dim3(chunks, n), dim3(kBwdThreads), 0, stream, nullptr,
-                 b);
-    else
-      launch_pdl(distill_bwd_kernel<float>, dim3(chunks, n), dim3(kBwdThreads), 0, stream, nullptr, b);
+    b.chunks = (int)chunks;
+    dim3 grid(chunks, (unsigned)n);
+    if (a.unless_one) {
+      int dev = 0;
+      cudaGetDevice(&dev);
+      const int64_t items = n * chunks, ctas = (int64_t)kBwdCtas * num_sms(dev);
+      grid = dim3((unsigned)(items < ctas ? items : ctas));
+    }
+    auto kernel = a.in.bf16 ? (a.unless_one ? distill_redo_kernel<__nv_bfloat16>
+                                            : distill_bwd_kernel<__nv_bfloat16>)
+                            : (a.unless_one ? distill_redo_kernel<float> : distill_bwd_kernel<float>);
+    launch_pdl(kernel, grid, dim3(kBwdThreads), 0, stream, nullptr, b);
   }
-}
-
-void scale_by_launch(void* x, bool bf16, int64_t n, const float* scale, cudaStream_t stream) {
-  if (n <= 0) return;
-  int dev = 0;
-  cudaGetDevice(&dev);
-  const int64_t want = (n + 256 * 8 - 1) / (256 * 8);
-  const unsigned grid = (unsigned)(want < 8 * num_sms(dev) ? want : 8 * num_sms(dev));
-  if (bf16)
-    launch_pdl(scale_by_kernel<__nv_bfloat16>, dim3(grid), dim3(256), 0, stream, nullptr,
-               (__nv_bfloat16*)x, n, scale);
-  else
-    launch_pdl(scale_by_kernel<float>, dim3(grid), dim3(256), 0, stream, nullptr, (float*)x, n,
-               scale);
 }
 
 }  // namespace b200

@@ -78,11 +78,9 @@ struct DistillBwdArgs {
   const float* g_rows;    // upstream gradient: [rows], or one value for all rows
   int g_stride;           // 1, or 0 for one value
   float g_scale;          // times the upstream gradient
+  bool unless_one;        // one value that is 1: grad stays as it is
   void* grad;
 };
 void distill_bwd_launch(const DistillBwdArgs& a, cudaStream_t stream);
-
-// x *= *scale (fp32 scalar on the device); returns at once where it is 1.
-void scale_by_launch(void* x, bool bf16, int64_t n, const float* scale, cudaStream_t stream);
 
 }  // namespace b200
