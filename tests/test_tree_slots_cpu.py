@@ -18,3 +18,17 @@ def test_rows_of_no_tree_are_left_as_they_are():
     exact = ops.tree_attention(torch.empty_like(q[1:6]), q[1:6], kc, vc, bt, sl, cu - 1, m[1:6],
                                0.125)
     assert torch.equal(out[1:6], exact)
+
+
+def test_lengths_beyond_the_tensors():
+    g = torch.Generator().manual_seed(0)
+    k = [torch.randn(32, 2, 64, generator=g)]
+    kc, vc, bt, sl = build_paged_kv(k, k, 16, generator=g)
+    q, cu = torch.randn(3, 4, 64, generator=g), torch.tensor([0, 3], dtype=torch.int32)
+    m = ops.tree_mask(torch.tensor([-1, 0, 0]), cu)
+    want = ops.tree_attention(torch.empty_like(q), q, kc, vc, bt, sl, cu, m, 0.125)
+    for lens, c in ((40, [0, 3]), (2 ** 31 - 1, [0, 3]), (32, [-4, 3]), (32, [0, 9])):
+        got = ops.tree_attention(torch.empty_like(q), q, kc, vc, bt,
+                                 torch.tensor([lens], dtype=torch.int32),
+                                 torch.tensor(c, dtype=torch.int32), m, 0.125)
+        assert torch.equal(got, want)

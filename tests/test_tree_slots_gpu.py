@@ -119,3 +119,15 @@ def test_rows_of_no_tree_are_left_as_they_are(b200_ops):
         want = ops.tree_attention(torch.empty_like(more[:n]), more[:n], kc, vc, bt, sl, now.clone(),
                                   mm[:n], 0.09)
         assert bool((out[n:] == 7).all()) and torch.equal(out[:n], want)
+
+
+@pytest.mark.parametrize("heads", HEADS[:3])
+def test_lengths_beyond_the_tensors(b200_ops, heads):
+    """Keys beyond the block table and nodes beyond q do not exist."""
+    lens, nodes = [160, 90], [9, 5]
+    q, kc, vc, bt, sl, cu, m = _setup(lens, nodes, heads, 16)
+    kc, vc = kc.nan_to_num(0.5), vc.nan_to_num(0.5)
+    for n in (161, 300, 2 ** 31 - 1):
+        _check(q, kc, vc, bt, torch.tensor([n, 90], dtype=torch.int32, device="cuda"), cu, m)
+    _check(q, kc, vc, bt, sl, torch.tensor([-7, 9, 2 ** 31 - 1], dtype=torch.int32, device="cuda"),
+           m)

@@ -168,10 +168,13 @@ struct Seq {
 };
 template <int FN, int kEdge>
 __device__ __forceinline__ Seq load_seq(const Params& p, int s) {
+  // Both come from the device unseen by the host: nodes beyond q's rows and keys
+  // beyond the block table do not exist, whatever the numbers say. (The host's
+  // bound of `total` rests on that too.)
   Seq r;
-  r.q0 = p.cu_q[s];
+  r.q0 = max(0, p.cu_q[s]);
   r.q_len = (int)max(0ll, min((long long)p.cu_q[s + 1], p.T) - r.q0);
-  r.seq_len = max(0, p.seq_lens[s]);
+  r.seq_len = (int)max(0ll, min((long long)p.seq_lens[s], (long long)p.max_blocks * p.block_size));
   r.nodes = min(r.q_len, r.seq_len);
   r.prefix = r.seq_len - r.nodes;
   // The first key that some node sees: a root sits at position `prefix`.

@@ -64,8 +64,8 @@ def tree_attention_ref(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
     bits = ((mask.to(torch.int64)[:, :, None] >> torch.arange(32, device=q.device)) & 1).bool()
     bits = bits.reshape(T, -1)
     for s in range(seq_lens.numel()):
-        a, b = int(cu_q[s]), min(int(cu_q[s + 1]), T)
-        L = max(0, int(seq_lens[s]))
+        a, b = max(0, int(cu_q[s])), min(int(cu_q[s + 1]), T)
+        L = max(0, min(int(seq_lens[s]), block_table.shape[1] * k_cache.shape[2]))
         if b <= a or L == 0:
             continue
         n = min(b - a, L)  # nodes whose keys exist
@@ -129,7 +129,8 @@ def tree_attention(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor,
     a node of depth 0, and the slots of nodes whose bit no row sets. What one
     node sees has to be finite for the others too. Head sizes 64, 128 and 256, any
     number of query heads a key head, block sizes of a power of two from 8.
-    Lengths are read on the device: a captured graph replays with new ones,
+    Lengths are read on the device (keys beyond the block table and nodes
+    beyond ``T`` do not exist): a captured graph replays with new ones,
     and with fewer nodes than ``T`` (rows of ``out`` that belong to no tree,
     from ``cu_q[B]`` on, are left as they are).
     """
@@ -152,6 +153,6 @@ def tree_attention(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor,
         return out
     r = tree_attention_ref(q, k_cache, v_cache, block_table, seq_lens, cu_q, mask, scale, window,
                            sinks)
-    first, last = int(cu_q[0]), min(int(cu_q[-1]), q.shape[0])
+    first, last = max(0, int(cu_q[0])), min(int(cu_q[-1]), q.shape[0])
     out[first:last] = r[first:last].to(out.dtype)
     return out
