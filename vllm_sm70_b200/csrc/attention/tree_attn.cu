@@ -54,18 +54,23 @@
 //              they may hold anything, and 0 x NaN is not 0.
 // TMEM columns: S0 | S1 | S2 | O.
 //
-// Measured (32 query, 8 key heads of 128, blocks of 16): 64 trees of 16 nodes
-// over 4096 tokens 135 us, 5160 GB/s of the 6454 that a copy reaches; the
-// steady state is HBM's, the rest is the start (~10 us to the first scores),
-// a few us at each unit's edge, and the join. 2 trees of 64 nodes over 60001
-// tokens 129 us (159 when each row tile read its keys from HBM): 730 TFLOP/s,
-// bound by a group's way from scores to P, ~3300 cycles of which 1900 are the
-// exponentials, a tile every ~1900. A third group with a buffer each was no
-// faster (S of tile n + 3 then waits for P V of tile n), nor were exponentials
-// on the FMA pipe or scores fetched ahead.
+// Measured (32 query, 8 key heads of 128, blocks of 16), on inputs that change
+// from call to call: 64 trees of 8 to 16 nodes over contexts of 1024 to 4096
+// tokens (2605 on average, 695 MB) 136 to 143 us, up to 5100 GB/s of the 6454
+// that a copy reaches; the steady state is HBM's, the rest is the start, a few
+// us at each unit's edge, and the join. Trees of 64 and 45 nodes over 60001 and
+// 42812 tokens (94.6 TFLOP) 148 to 152 us, 640 TFLOP/s; on the same inputs again
+// and again, when a part of them stays in L2, 129. Bound by a group's way from
+// scores to P, ~3300 cycles of which 1900 are the exponentials, a tile every
+// ~1900. A third group with a buffer each was no faster (S of tile n + 3 then
+// waits for P V of tile n), nor were exponentials on the FMA pipe or scores
+// fetched ahead.
 //
-// Rounding: P is rounded to bf16 for the tensor core (relative 2^-8 a term at
-// most, as the output's own rounding); scores, maxima, sums and O are fp32.
+// Rounding: P is rounded to bf16, since one product has operands of one type
+// and V is bf16 (relative 2^-8 a term at most, as the output's own rounding; the
+// output's error against 64 bits, relative to its norm, is 0.0023 with it and
+// 0.0017 without). Scores, maxima, sums and O are fp32; a row's sum adds the
+// exponentials before that rounding.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -108,8 +113,10 @@ struct Cfg {
   static constexpr int NV = D == 64 ? 6 : 3;      // V: held until P is there, two tiles on
   // What a unit's edge costs, in tiles: a masked tile, the output, at D = 256
   // also the wait for Q's one buffer. Shares of several short units get fewer
-  // tiles: 16 trees of 24 nodes, 16/2 heads of 256, window 4096: 72 -> 64 us;
-  // 64 of 8 nodes, 16/16 heads of 64: 217 -> 194; long units do not notice.
+  // tiles (16 trees of up to 24 nodes over 2000 to 8000 tokens, 16/2 heads of
+  // 256, window 4096: 72 -> 64 us; 64 of up to 8 nodes over 1024 to 4096 tokens,
+  // 16/16 heads of 64: 217 -> 194); long units do not notice. It moves shares'
+  // borders only.
   static constexpr int kEdge = D <= 128 ? 2 : 10;
   static constexpr int kSmem = NQ * kQBytes + (NK + NV) * kTile + kBarBytes + kRowBytes;
   static_assert(3 * FN + D <= 512, "TMEM columns");

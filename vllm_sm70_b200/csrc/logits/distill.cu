@@ -30,7 +30,7 @@
 //     memory, the row's only meeting. Then each warp writes its part of the
 //     gradient, and as it is done with a vector starts the copy of the next
 //     row's into its place: the clusters are persistent and memory is read
-//     while they work. 4096 x 128256 bf16, K = 64: 438 us, 4800 GB/s of the
+//     while they work. 4096 x 128256 bf16, K = 64: 446 us, 4710 GB/s of the
 //     6454 that a copy reaches. What is left is latency: of a row's ~16000
 //     clocks a third is the gradient, a quarter the sums, the rest the
 //     teacher's elements and the exchange, on six warps a scheduler. (Rows
@@ -39,8 +39,10 @@
 //     gradient's stores.)
 //   * Rows too long for that (more than 8 CTAs' shared memory) and calls
 //     without gradient stream the row; a bitmap of the teacher's ids leaves
-//     them out of the sum. 4096 x 128256 bf16 without gradient: 184 us,
-//     5720 GB/s; the gradient from saved numbers (distill_bwd): 360 us, 5840.
+//     them out of the sum. 4096 x 128256 bf16 without gradient: 176 us,
+//     5970 GB/s; the gradient from saved numbers (distill_bwd): 345 us, 6090.
+//   * fp32, 2048 x 128256, K = 64: 162 us without gradient, 425 with it (4940
+//     GB/s), 329 from saved numbers.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 

@@ -24,11 +24,12 @@
 // that cluster in few threads) raise tau to the exact n-th largest value by
 // bisection first.
 //
-// Bound: bytes, the row read once. 4096 x 128256 bf16: 189 us without
-// alternatives (5560 GB/s of the 6454 that a copy reaches), 224 with one, 241
-// with 20, 277 with 64: a row's last steps are some thousands of clocks of
-// barriers and dependent reads, which the SM's other three CTAs hide in part.
-// fp32 512 x 151936: 63 us (4930 GB/s). Four CTAs of 256 threads an SM, not two
+// Bound: bytes, the row read once. 4096 x 128256 bf16, normal logits: 191 us
+// without alternatives (5500 GB/s of the 6454 that a copy reaches), 223 with one,
+// 242 with 20 (233 where a model's peaks stand out), 282 with 64: a row's last
+// steps are some thousands of clocks of barriers and dependent reads, which the
+// SM's other three CTAs hide in part. fp32 512 x 151936: 55 us without
+// alternatives (5640 GB/s), 71 with 64. Four CTAs of 256 threads an SM, not two
 // of 512 (207 us): more rows end at different times. CTAs that keep to an SM
 // and fetch the next row's start ahead were slower (224 us). The inner loop
 // leaves checks to the two vectors that need them (233 us with them inside).
@@ -542,7 +543,8 @@ __global__ void __launch_bounds__(NT, 4) token_logprobs_kernel(const FwdParams p
 // dx_j = (g_lp ([j = y] - p_j) - g_H p_j (log p_j + H)) / T. Elementwise on
 // the saved (m, 1 / s, log2 s, H): reads the logits once, writes the gradient
 // once. One CTA a (row, chunk of kBwdThreads * U vectors). Bound: bytes; 4096 x
-// 128256 bf16 317 us (6640 GB/s; a copy of the same tensor 322).
+// 128256 bf16 321 us (6550 GB/s; a copy of the same tensor 323), fp32 512 x 151936
+// 102 (6130).
 struct BwdParams {
   const void* x;
   const void* ids;

@@ -124,7 +124,9 @@ def tree_attention(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor,
     node that sees nothing (no prefix, no bits) gets 0. ``window > 0`` limits
     the prefix to the positions ``> prefix + depth - window`` (depth: the bits
     of the row minus one); it has to hold the whole tree (``32 * words``).
-    ``sinks [Hq]`` join the denominators. Cache entries that no node sees may
+    ``sinks [Hq]`` join the denominators. Weights are rounded to bf16 before
+    they meet V, as in :func:`~vllm_sm70_b200.ops.paged_attention`; scores and
+    sums are fp32. Cache entries that no node sees may
     hold anything, NaN too: those from ``seq_lens[s]`` on, before the window of
     a node of depth 0, and the slots of nodes whose bit no row sets. What one
     node sees has to be finite for the others too. Head sizes 64, 128 and 256, any
