@@ -147,3 +147,23 @@ def test_upstream_of_zero(b200_ops):
     loss = ops.distill_loss(x.requires_grad_(True), ids, lp) * 0.0
     g, = torch.autograd.grad(loss, x)
     assert bool((g == 0).all())
+
+
+@pytest.mark.parametrize("V", [64, 5003, 2 ** 21 + 5])
+def test_no_token_and_no_distribution(b200_ops, V):
+    """No id of the teacher's is there: nothing to learn, from a row whose
+    mask leaves nothing neither."""
+    x, ids, lp = _rows(4, V, 5, torch.float32, 1)
+    x[1] = -float("inf")
+    ids[:2] = -1
+    ids[1, 0] = V
+    x[2] = -float("inf")
+    want = L.distill_rows_ref(x, ids, lp, dtype=torch.float64)
+    assert want[:3].tolist() == [0, 0, float("inf")]
+    xg = x.requires_grad_(True)
+    for reduction in ("none", "sum"):
+        rows = ops.distill_loss(xg, ids, lp, reduction=reduction)
+        g, = torch.autograd.grad(rows.sum(), xg)
+        assert bool((g[:3] == 0).all()) and bool((g[3] != 0).any())
+    rows = ops.distill_loss(xg.detach(), ids, lp, reduction="none")
+    torch.testing.assert_close(rows.double(), want, atol=2 * TOL, rtol=TOL)

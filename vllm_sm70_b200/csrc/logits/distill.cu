@@ -239,9 +239,11 @@ __device__ __forceinline__ float row_loss(const Teacher& t, const Params& p, con
   // An empty row: every log q is -inf, the loss inf where the teacher has mass.
   const float l2 = s == 0.f ? 0.f : log2f(s);
   float loss = 0.f;
+  bool any = false;
 #pragma unroll
   for (int i = 0; i < kIds; ++i) {
     const float pk = t.p[i];
+    any |= t.id[i] >= 0 && t.id[i] < p.V;
     if (pk > 0.f)
       loss += pk * (t.lp[i] - fmaf(xk[i] - m0, p.inv_t, -l2 * kLn2));
     else if (pk != pk)
@@ -249,7 +251,8 @@ __device__ __forceinline__ float row_loss(const Teacher& t, const Params& p, con
   }
   loss = warp_sum(loss);
   const float p_t = p.tail ? fmaxf(0.f, 1.f - t.sum_p) : 0.f;
-  if (p_t > 0.f)
+  // (Without any token p_t = q_t = 1, in a row without a distribution too.)
+  if (p_t > 0.f && __any_sync(0xffffffffu, any))
     loss += p_t * (logf(p_t) - fmaf(q.m_out - m0, p.inv_t, (log2f(q.s_out) - l2) * kLn2));
   return loss;
 }
