@@ -198,7 +198,11 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logpro
 
     Ids outside ``[0, V)`` are absent (their mass joins the tail); a repeated
     id's values are both held against that token. A student that gives a
-    teacher's token no probability has loss ``inf``.
+    teacher's token no probability, or one that fp32 has no logarithm for (a
+    mask of the lowest value over a temperature below 1), has loss ``inf``. So
+    has one with no mass outside the tokens where ``p_t`` is not 0: log-probs
+    that hold all of the teacher's mass still sum to 1 only within their
+    rounding, and want ``tail=False`` if the student is masked outside them.
     """
     what = "distill_loss"
     _check_rows(logits, what)
